@@ -38,11 +38,42 @@ XE_OP_MUL_EXP = 6
 XE_OP_LOG_ADD = 7
 XE_OP_RESCALE = 8
 
+XE_F32 = 0
+XE_BF16 = 1
+XE_F16 = 2
+XE_E4M3 = 3
+XE_I8 = 4
+
 _c_i32 = ctypes.c_int32
 _c_i64 = ctypes.c_int64
 _c_size = ctypes.c_size_t
 _c_ptr = ctypes.c_void_p
 _c_i64p = ctypes.POINTER(ctypes.c_int64)
+
+
+class SelectiveScanArgs(ctypes.Structure):
+    """xe_selective_scan_args of include/xe_b200.h."""
+
+    _fields_ = [
+        *((name, _c_ptr) for name in ("x", "delta", "z", "b", "c", "y", "a", "d", "delta_bias", "state", "state_out",
+                                      "checkpoints", "lengths")),
+        *((name, _c_i64) for name in ("x_sb", "x_st", "delta_sb", "delta_st", "z_sb", "z_st", "b_sb", "b_st", "b_sg",
+                                      "c_sb", "c_st", "c_sg", "batch", "length", "channels", "states", "groups")),
+        *((name, _c_i32) for name in ("lengths64", "softplus", "dtype")),
+    ]
+
+
+class SelectiveScanGrads(ctypes.Structure):
+    """xe_selective_scan_grads of include/xe_b200.h."""
+
+    _fields_ = [
+        *((name, _c_ptr) for name in ("dy", "dstate_out", "dx", "ddelta", "dz", "db", "dc", "da", "dd", "dstate")),
+        *((name, _c_i64) for name in ("dy_sb", "dy_st")),
+    ]
+
+
+_scan_args = ctypes.POINTER(SelectiveScanArgs)
+_scan_grads = ctypes.POINTER(SelectiveScanGrads)
 
 # name -> (restype, argtypes); mirrors include/xe_b200.h
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -201,6 +232,61 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "xe_elementwise": (
         _c_i32,
         [_c_i32, _c_ptr, _c_i64p, _c_ptr, _c_i64p, _c_ptr, _c_i64p, _c_ptr, _c_i64p, _c_i32, _c_ptr],
+    ),
+    "xe_causal_conv1d": (
+        _c_i32,
+        [
+            _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,  # x, strides, weight, bias, state, y, state_out
+            _c_ptr, _c_i32, _c_i64, _c_i64, _c_i64, _c_i64,  # lengths, lengths64, batch, length, channels, width
+            _c_i32, _c_i32, _c_ptr,  # activation, dtype, stream
+        ],
+    ),
+    "xe_causal_conv1d_step": (
+        _c_i32,
+        [
+            _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr,  # x, stride, weight, bias, state, y
+            _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_ptr,  # batch, channels, width, activation, dtype, stream
+        ],
+    ),
+    "xe_causal_conv1d_backward_workspace_size": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i64]),
+    "xe_causal_conv1d_backward": (
+        _c_i32,
+        [
+            _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr,  # x, strides, weight, bias, state
+            _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr,  # dy, strides, dstate_out, dx, dstate, dweight
+            _c_ptr, _c_i32, _c_i64, _c_i64, _c_i64, _c_i64,  # lengths, lengths64, batch, length, channels, width
+            _c_i32, _c_i32, _c_ptr, _c_size, _c_ptr,  # activation, dtype, workspace, bytes, stream
+        ],
+    ),
+    "xe_selective_scan_workspace_size": (_c_size, [_c_i64] * 5),
+    "xe_selective_scan_checkpoint_size": (_c_size, [_c_i64] * 4),
+    "xe_selective_scan": (_c_i32, [_scan_args, _c_ptr, _c_size, _c_ptr]),
+    "xe_selective_scan_step": (_c_i32, [_scan_args, _c_ptr]),
+    "xe_selective_scan_backward_workspace_size": (_c_size, [_c_i64] * 5),
+    "xe_selective_scan_backward": (_c_i32, [_scan_args, _scan_grads, _c_ptr, _c_size, _c_ptr]),
+    "xe_rms_norm": (
+        _c_i32,
+        [
+            _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr,  # x, residual (row strides), weight, y, sum, scale
+            _c_i64, _c_i64, ctypes.c_float, _c_i32, _c_i32, _c_i32, _c_i32, _c_ptr,  # rows, columns, eps, types, stream
+        ],
+    ),
+    "xe_rms_norm_backward_workspace_size": (_c_size, [_c_i64, _c_i64]),
+    "xe_rms_norm_backward": (
+        _c_i32,
+        [
+            _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr,  # sum, addend, weight
+            _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr,  # dy, dsum, dx, dweight
+            _c_i64, _c_i64, ctypes.c_float, _c_i32, _c_i32, _c_i32,  # rows, columns, eps, types
+            _c_ptr, _c_size, _c_ptr,  # workspace, bytes, stream
+        ],
+    ),
+    "xe_int4_linear": (
+        _c_i32,
+        [
+            _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr,  # x, row, x_scale, packed, row, scales, zeros, y
+            _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_ptr,  # rows, inputs, outputs, group, types, stream
+        ],
     ),
 }
 

@@ -32,8 +32,9 @@ from __future__ import annotations
 from collections.abc import Sequence
 
 import torch
+from torch.autograd.function import once_differentiable
 
-from . import ops
+from . import ops, sequence
 
 
 def needs_grad(*tensors: torch.Tensor | None) -> bool:
@@ -298,3 +299,88 @@ class Log(torch.autograd.Function):
     def backward(ctx, g):
         (x,) = ctx.saved_tensors
         return ops.elementwise("div", g, x)
+
+
+class CausalConv1d(torch.autograd.Function):
+    """(y, new state) of the causal convolution; the state's gradient joins those of the last inputs."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, activation, lengths):
+        y, new = ops.causal_conv1d(
+            x, weight, bias, activation=activation, state=state, lengths=lengths, return_state=True)
+        ctx.save_for_backward(x, weight, bias, state, lengths)
+        ctx.activation = activation
+        ctx.set_materialize_grads(False)
+        return y, new
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dnew):
+        if dy is None and dnew is None:
+            return (None,) * 6
+        x, weight, bias, state, lengths = ctx.saved_tensors
+        if dy is None:
+            dy = torch.zeros_like(x)
+        dx, dweight, dbias, dstate = sequence.causal_conv1d_backward(
+            x, weight, bias, state, ctx.activation, lengths, dy, dnew, state is not None and ctx.needs_input_grad[3])
+        return dx, dweight, dbias if bias is not None else None, dstate, None, None
+
+
+class SelectiveScan(torch.autograd.Function):
+    """(y, last state) of the selective scan.  The forward call stores the state before every 16th token, and the
+    backward pass runs the states of 16 tokens again from each (csrc/selective_scan.cuh)."""
+
+    @staticmethod
+    def forward(ctx, x, delta, a, b, c, d, z, delta_bias, state, softplus: bool, lengths):
+        y, new, checkpoints = sequence._scan_forward(
+            x, delta, a, b, c, d, z, delta_bias, softplus, state, lengths, True, True)
+        ctx.save_for_backward(x, delta, a, b, c, d, z, delta_bias, state, lengths, checkpoints)
+        ctx.softplus = softplus
+        ctx.set_materialize_grads(False)
+        return y, new
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dnew):
+        if dy is None and dnew is None:
+            return (None,) * 11
+        x, delta, a, b, c, d, z, delta_bias, state, lengths, checkpoints = ctx.saved_tensors
+        if dy is None:
+            dy = torch.zeros_like(x)
+        g = sequence.selective_scan_backward(
+            x, delta, a, b, c, d, z, delta_bias, ctx.softplus, state, lengths, checkpoints, dy, dnew)
+        return (g["x"], g["delta"], g["a"], g["b"], g["c"], g["d"] if d is not None else None, g["z"],
+                g["delta_bias"] if delta_bias is not None else None, g["state"], None, None)
+
+
+class RmsNorm(torch.autograd.Function):
+    """(y, s) of the norm of s = x + residual; ds = rstd (du - u mean(du u)) + ds_out with u = s rstd, du = dy w."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps: float):
+        if residual is None:
+            y, total = ops.rms_norm(x, weight, eps=eps), x
+        else:
+            y, total = ops.rms_norm(x, weight, residual=residual, eps=eps)
+        # a float32 sum stands for itself; a 16-bit one has been rounded, and is added again
+        if residual is None or total.dtype == torch.float32:
+            ctx.save_for_backward(total, None, weight)
+        else:
+            ctx.save_for_backward(residual, x, weight)
+        ctx.eps, ctx.dtype = eps, x.dtype
+        ctx.set_materialize_grads(False)
+        return y, None if residual is None else total
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dtotal):
+        total, addend, weight = ctx.saved_tensors
+        if dy is None:
+            if dtotal is None:
+                return (None,) * 4
+            return dtotal.to(ctx.dtype), None, dtotal, None
+        dx, dweight = sequence.rms_norm_backward(
+            total, addend, weight, dy, dtotal, ctx.eps, weight is not None and ctx.needs_input_grad[1])
+        if dweight is not None:
+            dweight = dweight.to(weight.dtype)
+        return dx.to(ctx.dtype), dweight, dx if ctx.needs_input_grad[2] else None, None

@@ -7,6 +7,7 @@ loads it with ctypes (extended_einsum_b200/_lib.py).
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -16,13 +17,13 @@ PACKAGE_DIR = Path(__file__).resolve().parent
 REPO_ROOT = PACKAGE_DIR.parent
 CSRC = PACKAGE_DIR / "csrc"
 LIBRARY = PACKAGE_DIR / "libxe_b200.so"
-SOURCES = [CSRC / "xe_b200.cu"]
-DEPENDENCIES = sorted(CSRC.glob("*.cuh")) + [REPO_ROOT / "include" / "xe_b200.h"]
+SOURCES = [CSRC / "xe_b200.cu", CSRC / "xe_sequence.cu"]
+DEPENDENCIES = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [REPO_ROOT / "include" / "xe_b200.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
     "--expt-relaxed-constexpr",
 ]
 
@@ -41,17 +42,49 @@ def is_stale() -> bool:
     return any(p.stat().st_mtime > built for p in SOURCES + DEPENDENCIES)
 
 
+def _includes(source: Path) -> list[Path]:
+    """The source and the headers of the repository that it includes, directly or not."""
+    found, todo = [], [source]
+    while todo:
+        path = todo.pop()
+        if path in found or not path.exists():
+            continue
+        found.append(path)
+        for name in re.findall(r'^#include "([^"]+)"', path.read_text(), flags=re.M):
+            todo.append((path.parent / name).resolve())
+    return found
+
+
 def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
-    """Compiles libxe_b200.so for sm_100a if a source is newer than the library."""
+    """Compiles libxe_b200.so for sm_100a if a source is newer than the library.
+
+    Each source becomes an object of its own, compiled side by side; one whose includes are all
+    older than its object is kept (with the default flags)."""
     if not force and not is_stale():
         return LIBRARY
-    cmd = [find_nvcc(), *NVCC_FLAGS, *(extra_flags or []), "-o", str(LIBRARY), *map(str, SOURCES)]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
+    nvcc, running, objects = find_nvcc(), [], []
+    for source in SOURCES:
+        obj = source.with_suffix(".o")
+        objects.append(obj)
+        newest = max(p.stat().st_mtime for p in [*_includes(source), Path(__file__)])
+        if not force and not extra_flags and obj.exists() and obj.stat().st_mtime > newest:
+            continue
+        cmd = [nvcc, *NVCC_FLAGS, *(extra_flags or []), "-c", "-o", str(obj) + ".tmp", str(source)]
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        running.append((obj, cmd, subprocess.Popen(cmd, cwd=str(REPO_ROOT))))
+    failed = [cmd for _, cmd, process in running if process.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    for obj, _, _ in running:
+        os.replace(str(obj) + ".tmp", obj)
     tmp = LIBRARY.with_suffix(".so.tmp")
-    cmd[cmd.index(str(LIBRARY))] = str(tmp)
-    subprocess.run(cmd, check=True, cwd=str(REPO_ROOT))
+    link = [nvcc, *NVCC_FLAGS[:2], "-shared", "-o", str(tmp), *map(str, objects)]
+    subprocess.run(link, check=True, cwd=str(REPO_ROOT))
     os.replace(tmp, LIBRARY)
+    if extra_flags:  # objects of other flags are not kept for a later build
+        for obj in objects:
+            obj.unlink()
     return LIBRARY
 
 

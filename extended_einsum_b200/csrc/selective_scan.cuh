@@ -1,0 +1,681 @@
+// Selective state space scan over the time axis, channel-last.  For channel d and state n
+//
+//   delta_t = softplus(raw_t + bias_d) (or raw_t + bias_d),   e_tn = exp(delta_t A_dn),
+//   h_tn = e_tn h_{t-1,n} + delta_t x_t B_tn,   v_t = sum_n C_tn h_tn + D_d x_t,   y_t = v_t silu(z_t),
+//
+// with B and C shared by the channels of a group.  Bound by the special function unit: one
+// exponential per token, channel and state at 16 results per clock and SM (plus four per token and
+// channel for softplus and the gate); the 8 bytes of x, delta, z and y of a 16-bit type take a third of
+// that time.
+//
+// Layout: kLanes lanes share a channel and hold S states each, so kLanes * S >= states; states past
+// the real ones have A = B = C = 0.  A block stages a tile of tokens: (delta, delta x) pairs, B and
+// C as float32 in shared memory, the recurrence runs over the tile from registers, and v goes back
+// through shared memory to the threads that hold the tile's x and z.
+//
+// Few channels: the length is split into segments.  A first pass runs each segment from a zero state
+// and keeps its last state and sum of delta (the product of its e is exp(A sum delta)), a second
+// joins them into every segment's first state, and the scan then runs all segments at once.
+#pragma once
+
+#include "seq_common.cuh"
+
+namespace xe {
+namespace scan {
+
+using namespace seq;
+
+constexpr int kThreads = 128;
+
+struct Params {
+  const void *x, *delta, *z, *b, *c;
+  void* y;
+  const float *a, *d, *bias;  // (channels, states), (channels) or null, (channels) or null
+  const float* state;         // (batch, channels, states) or null = zeros
+  float* state_out;           // like state, or null
+  float* checkpoints;         // (batch, ceil(length / kCheckpoint), channels, padded states), or null
+  const void* lengths;
+  int lengths64;
+  int64_t x_sb, x_st, delta_sb, delta_st, z_sb, z_st, b_sb, b_st, b_sg, c_sb, c_st, c_sg;
+  int batch, length, channels, states, groups;
+  int softplus;
+  int vec;  // bit 0: x, 1: delta, 2: z, 3: y, 4: b, 5: c, 6: dy
+  int segments, segment_length;
+  float* segment_state;  // (segments, batch, channels, states)
+  float* segment_delta;  // (segments, batch, channels)
+  // backward
+  const void* dy;
+  int64_t dy_sb, dy_st;
+  const float* dstate_out;  // gradient of state_out, or null
+  float* dstate;            // gradient of state, or null
+  void *dx, *ddelta, *dz;   // contiguous (batch, length, channels); dz null without z
+  float* dbc;               // (channel blocks, batch, length, 2, padded states)
+  float* da;                // (segments * batch, channels, states)
+  float* dd;                // (segments * batch, 2, channels): d(D), d(bias)
+};
+
+// Tokens between two stored states (training): the backward pass runs forward again from them.
+constexpr int kCheckpoint = 16;
+
+template <int N>
+__device__ __forceinline__ void load_f32(const float* smem, float (&v)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 q = *reinterpret_cast<const float4*>(smem + i);
+      v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = smem[i];
+  }
+}
+
+// A block's channels lie in one group: blocks [g * per_group, (g + 1) * per_group) are group g's.
+struct Channels {
+  int group, first, count;
+};
+__device__ __forceinline__ Channels block_channels(const Params& p, int per_block) {
+  const int each = p.channels / p.groups;
+  const int per_group = (each + per_block - 1) / per_block;
+  const int group = blockIdx.x / per_group;
+  const int at = (blockIdx.x % per_group) * per_block;
+  return {group, group * each + at, min(per_block, each - at)};
+}
+
+// B and C of a tile as float32, states padded with zeros; tokens at or past `live` read as zero.
+template <typename T, int kTile, int NP>
+struct SharedStates {
+  static constexpr int kVectors = 2 * kTile * (NP / 8);
+  static constexpr int kEach = (kVectors + kThreads - 1) / kThreads;
+  Raw8<T> raw[kEach];
+
+  __device__ __forceinline__ void load(const Params& p, int batch, int group, int t0, int live, int wanted = 3) {
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int i = k * kThreads + threadIdx.x;
+      const int n0 = (i % (NP / 8)) * 8;
+      const int which = (i / (NP / 8)) & 1;
+      const int t = t0 + i / (NP / 8) / 2;
+      const int count = i < kVectors && t < live && (wanted >> which & 1) ? min(8, p.states - n0) : 0;
+      const T* at = which ? static_cast<const T*>(p.c) + batch * p.c_sb + t * p.c_st + group * p.c_sg + n0
+                          : static_cast<const T*>(p.b) + batch * p.b_sb + t * p.b_st + group * p.b_sg + n0;
+      raw[k] = load8<T>(at, count, p.vec & (which ? 32 : 16));
+    }
+  }
+  __device__ __forceinline__ void store(float* smem) {
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int i = k * kThreads + threadIdx.x;
+      if (i < kVectors) {
+        float v[8];
+        unpack8<T>(raw[k], v);
+        float4* at = reinterpret_cast<float4*>(smem + (int64_t)i * 8);
+        at[0] = make_float4(v[0], v[1], v[2], v[3]);
+        at[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    }
+  }
+};
+
+// Sums v[k] over the kLanes lanes of a channel; lane l returns the sum of v[l].
+template <int kLanes>
+__device__ __forceinline__ float transpose_sum(float (&v)[kLanes], int lane) {
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) {
+    const bool upper = lane & o;
+#pragma unroll
+    for (int k = 0; k < kLanes; k += 2 * o) {
+      const float send = upper ? v[k] : v[k + o];
+      const float keep = upper ? v[k + o] : v[k];
+      v[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  return v[0];
+}
+
+// kFull: the scan.  kStates: the last state of each segment from zero, no outputs.  kAdjoint: the
+// same of the reversed recurrence of the backward pass, c_{t-1} = e_t (c_t + C_t dv_t).
+enum Mode { kFull, kStates, kAdjoint };
+
+template <typename T, int S, int kLanes, Mode kMode>
+__global__ void __launch_bounds__(kThreads) selective_scan_kernel(Params p) {
+  constexpr bool kStateOnly = kMode != kFull;
+  constexpr int kChannels = kThreads / kLanes;
+  constexpr int kTile = 8 * kLanes;  // tokens: one group of eight channels per thread
+  constexpr int NP = S * kLanes;
+  constexpr int kPitch = kChannels + 4;
+  __shared__ __align__(16) float2 s_dd[kTile][kChannels + 2];
+  __shared__ __align__(16) float s_bc[kTile * 2 * NP];
+  __shared__ __align__(16) float s_v[kStateOnly ? 1 : kTile][kPitch];
+  const Channels ch = block_channels(p, kChannels);
+  // the first segment needs no adjoint from zero, the last one no state
+  const int batch = blockIdx.y, segment = blockIdx.z + (kMode == kAdjoint ? 1 : 0);
+  const int begin = segment * p.segment_length;
+  const int end = min(begin + p.segment_length, p.length);
+  const int live = min(end, sequence_length(p.lengths, p.lengths64, batch, p.length));
+
+  // staging: this thread's token and eight channels of every tile
+  const int row = threadIdx.x / (kChannels / 8);
+  const int col = (threadIdx.x % (kChannels / 8)) * 8;
+  const int count = max(0, min(8, ch.count - col));
+  float bias[8], skip[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    bias[i] = p.bias && i < count ? p.bias[ch.first + col + i] : 0.0f;
+    skip[i] = p.d && i < count ? p.d[ch.first + col + i] : 0.0f;
+  }
+  const T* x = kMode == kAdjoint ? static_cast<const T*>(p.dy) + batch * p.dy_sb + ch.first + col
+                                 : static_cast<const T*>(p.x) + batch * p.x_sb + ch.first + col;
+  const int64_t x_st = kMode == kAdjoint ? p.dy_st : p.x_st;
+  const int x_vec = p.vec & (kMode == kAdjoint ? 64 : 1);
+  const T* delta = static_cast<const T*>(p.delta) + batch * p.delta_sb + ch.first + col;
+  const T* z = static_cast<const T*>(p.z) + batch * p.z_sb + ch.first + col;
+  T* y = static_cast<T*>(p.y) + (int64_t)batch * p.length * p.channels + ch.first + col;
+
+  // recurrence: this thread's channel and states
+  const int c = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  const bool mine = c < ch.count;
+  const int64_t state_at = ((int64_t)batch * p.channels + ch.first + c) * p.states + lane * S;
+  float a[S], h[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const bool in = mine && lane * S + s < p.states;
+    a[s] = in ? p.a[(int64_t)(ch.first + c) * p.states + lane * S + s] * kLog2e : 0.0f;
+    h[s] = 0.0f;
+    if (!kStateOnly && in) {
+      if (p.segments > 1)
+        h[s] = p.segment_state[(int64_t)segment * p.batch * p.channels * p.states + state_at + s];
+      else if (p.state)
+        h[s] = p.state[state_at + s];
+    }
+  }
+  float delta_sum = 0.0f;
+
+  Raw8<T> raw_x, raw_d, raw_z, next_z;
+  SharedStates<T, kTile, NP> bc;
+  auto fetch = [&](int t0) {
+    const int t = t0 + row;
+    const int n = t < live ? count : 0;
+    raw_x = load8<T>(x + t * x_st, n, x_vec);
+    raw_d = load8<T>(delta + t * p.delta_st, n, p.vec & 2);
+    if (kMode != kStates && p.z) next_z = load8<T>(z + t * p.z_st, n, p.vec & 4);
+    bc.load(p, batch, ch.group, t0, live, kMode == kFull ? 3 : kMode == kStates ? 1 : 2);
+  };
+  const int tiles = (end - begin + kTile - 1) / kTile;
+  const int step = kMode == kAdjoint ? -kTile : kTile;
+  int t0 = kMode == kAdjoint ? begin + (tiles - 1) * kTile : begin;
+  fetch(t0);
+  for (int tile = 0; tile < tiles; ++tile, t0 += step) {
+    const bool in = t0 + row < live;
+    float xv[8], dv[8];
+    unpack8<T>(raw_x, xv);
+    unpack8<T>(raw_d, dv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v = dv[i] + bias[i];
+      if (p.softplus) v = softplus(v);
+      if (kMode != kAdjoint) {
+        s_dd[row][col + i] = in ? make_float2(v, v * xv[i]) : make_float2(0.0f, 0.0f);
+      } else {
+        float dv_t = xv[i];
+        if (p.z) {
+          float zv[8];
+          unpack8<T>(next_z, zv);
+          dv_t *= zv[i] * sigmoid(zv[i]);
+        }
+        s_dd[row][col + i] = in ? make_float2(v, dv_t) : make_float2(0.0f, 0.0f);
+      }
+    }
+    bc.store(s_bc);
+    raw_z = next_z;
+    __syncthreads();
+    if (tile + 1 < tiles) fetch(t0 + step);
+    if (t0 < live || p.checkpoints) {
+#pragma unroll 2
+      for (int t = 0; t < kTile; t += kLanes) {
+        float v[kLanes];
+#pragma unroll
+        for (int k = 0; k < kLanes; ++k) {
+          if (!kStateOnly && p.checkpoints && mine && (t0 + t + k) % kCheckpoint == 0 && t0 + t + k < p.length) {
+            const int64_t rows = (p.length + kCheckpoint - 1) / kCheckpoint;
+            float* at = p.checkpoints +
+                        (((int64_t)batch * rows + (t0 + t + k) / kCheckpoint) * p.channels + ch.first + c) * NP + lane * S;
+#pragma unroll
+            for (int s = 0; s < S; ++s) at[s] = h[s];
+          }
+          const int at = kMode == kAdjoint ? kTile - 1 - (t + k) : t + k;
+          const float2 dd = s_dd[at][c];
+          float bv[S], cv[S];
+          // B, or C in the adjoint recurrence
+          load_f32<S>(s_bc + (at * 2 + (kMode == kAdjoint ? 1 : 0)) * NP + lane * S, bv);
+          if (!kStateOnly) load_f32<S>(s_bc + ((t + k) * 2 + 1) * NP + lane * S, cv);
+          v[k] = 0.0f;
+          delta_sum += dd.x;
+#pragma unroll
+          for (int s = 0; s < S; ++s) {
+            if (kMode == kAdjoint)
+              h[s] = exp2_fast(dd.x * a[s]) * fmaf(dd.y, bv[s], h[s]);
+            else
+              h[s] = fmaf(exp2_fast(dd.x * a[s]), h[s], dd.y * bv[s]);
+            if (!kStateOnly) v[k] = fmaf(cv[s], h[s], v[k]);
+          }
+        }
+        if (!kStateOnly) {
+          const float sum = transpose_sum<kLanes>(v, lane);
+          s_v[t + lane][c] = sum;
+        }
+      }
+    }
+    if (!kStateOnly) {
+      __syncthreads();
+      if (t0 + row < end && count > 0) {
+        float o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = in ? fmaf(skip[i], xv[i], s_v[row][col + i]) : 0.0f;
+        if (p.z && in) {
+          float zv[8];
+          unpack8<T>(raw_z, zv);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] *= zv[i] * sigmoid(zv[i]);
+        }
+        store8<T>(y + (int64_t)(t0 + row) * p.channels, count, p.vec & 8, o);
+      }
+    }
+    __syncthreads();
+  }
+  if (!mine) return;
+  if (kStateOnly) {
+    float* out = p.segment_state + (int64_t)segment * p.batch * p.channels * p.states + state_at;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (lane * S + s < p.states) out[s] = h[s];
+    if (lane == 0) p.segment_delta[((int64_t)segment * p.batch + batch) * p.channels + ch.first + c] = delta_sum;
+  } else if (p.state_out && segment == p.segments - 1) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (lane * S + s < p.states) p.state_out[state_at + s] = h[s];
+  }
+}
+
+// The first states of all segments, in place over their last states from zero; or, kReverse, the
+// adjoints that enter each segment from behind.
+template <bool kReverse>
+__global__ void __launch_bounds__(256) selective_scan_join_kernel(Params p) {
+  const int64_t total = (int64_t)p.batch * p.channels * p.states;
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= total) return;
+  const int64_t bc = i / p.states;
+  const float a = p.a[(bc % p.channels) * p.states + i % p.states] * kLog2e;
+  const float* first = kReverse ? p.dstate_out : p.state;
+  float h = first ? first[i] : 0.0f;
+  for (int j = 0; j < p.segments; ++j) {
+    const bool last = j == p.segments - 1;
+    const int k = kReverse ? p.segments - 1 - j : j;
+    const float own = last ? 0.0f : p.segment_state[k * total + i];
+    const float sum = last ? 0.0f : p.segment_delta[k * (total / p.states) + bc];
+    p.segment_state[k * total + i] = h;
+    h = fmaf(exp2_fast(sum * a), h, own);
+  }
+}
+
+// Sums v[0 .. 7] over the eight channels of a warp (lane bits 2 to 4); a lane returns the sum of
+// v[(its channel)].
+__device__ __forceinline__ float channel_sum(float (&v)[8], int lane_in_warp) {
+#pragma unroll
+  for (int o = 16, half = 4; half > 0; o >>= 1, half >>= 1) {
+    const bool upper = lane_in_warp & o;
+#pragma unroll
+    for (int k = 0; k < half; ++k) {
+      const float send = upper ? v[k] : v[k + half];
+      const float keep = upper ? v[k + half] : v[k];
+      v[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  return v[0];
+}
+
+// The backward pass.  With dv_t = dy_t silu(z_t) the adjoint of the state is
+//
+//   g_t = C_t dv_t + c_t,  c_{t-1} = e_t g_t  (c at the end: the gradient of the last state),
+//   w_t = c_{t-1} h_{t-1} = g_t e_t h_{t-1}:
+//   dx = D dv + delta sum_n g B,  ddelta = x sum_n g B + sum_n A w,  dA = sum_t delta w,
+//   dB = sum_d g delta x,  dC = sum_d dv h,  dD = sum dv x,  dz = dy v silu'(z).
+//
+// Tiles of 32 tokens are taken from the last to the first, in halves of kCheckpoint tokens: the states
+// of a half are run again from its stored first state and stay in registers, with their e, for the
+// way back.  Sixteen states at a time (four lanes of four); more states take further turns over
+// the staged tile.  Sums over the states of a channel and over the channels of a warp are
+// transposed butterflies; the warps' parts of dB and dC go through shared memory, the blocks' through
+// global memory, all in a fixed order.
+template <typename T, int kBlocks>
+__global__ void __launch_bounds__(kThreads, 2) selective_scan_backward_kernel(Params p) {
+  constexpr int S = 4, kLanes = 4, kChannels = kThreads / kLanes, kTile = 32, kWarps = kThreads / 32;
+  constexpr int NP = 16 * kBlocks;
+  constexpr int kHalf = kCheckpoint;
+  extern __shared__ __align__(16) float smem[];
+  constexpr int kPitch = kChannels + 4;
+  float2(*s_dx)[kChannels + 2] = reinterpret_cast<float2(*)[kChannels + 2]>(smem);  // (delta, x)
+  float* at_smem = smem + kTile * (kChannels + 2) * 2;
+  float(*s_dv)[kPitch] = reinterpret_cast<float(*)[kPitch]>(at_smem);
+  float(*s_v)[kPitch] = s_dv + kTile;   // sum C h
+  float(*s_gb)[kPitch] = s_v + kTile;   // sum g B
+  float(*s_ga)[kPitch] = s_gb + kTile;  // sum A w / ln 2
+  float* s_bc = at_smem + 4 * kTile * kPitch;
+  float* s_red = s_bc + kTile * 2 * NP;  // [kWarps][kTile][2][16]
+
+  const Channels ch = block_channels(p, kChannels);
+  const int batch = blockIdx.y, segment = blockIdx.z;
+  const int begin = segment * p.segment_length;
+  const int end = min(begin + p.segment_length, p.length);
+  const int live = min(end, sequence_length(p.lengths, p.lengths64, batch, p.length));
+  const int row = threadIdx.x / (kChannels / 8);
+  const int col = (threadIdx.x % (kChannels / 8)) * 8;
+  const int count = max(0, min(8, ch.count - col));
+  float bias[8], skip[8], dd[8], dbias[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    bias[i] = p.bias && i < count ? p.bias[ch.first + col + i] : 0.0f;
+    skip[i] = p.d && i < count ? p.d[ch.first + col + i] : 0.0f;
+    dd[i] = dbias[i] = 0.0f;
+  }
+  const T* x = static_cast<const T*>(p.x) + batch * p.x_sb + ch.first + col;
+  const T* delta = static_cast<const T*>(p.delta) + batch * p.delta_sb + ch.first + col;
+  const T* z = static_cast<const T*>(p.z) + batch * p.z_sb + ch.first + col;
+  const T* dy = static_cast<const T*>(p.dy) + batch * p.dy_sb + ch.first + col;
+  const int64_t out_at = (int64_t)batch * p.length * p.channels + ch.first + col;
+
+  const int c = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  const int warp = threadIdx.x / 32, warp_lane = threadIdx.x % 32;
+  const bool mine = c < ch.count;
+  const int64_t state_at = ((int64_t)batch * p.channels + ch.first + c) * p.states;
+  float a[kBlocks][S], carry[kBlocks][S], da[kBlocks][S];
+  for (int nb = 0; nb < kBlocks; ++nb) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int n = nb * 16 + lane * S + s;
+      const bool in = mine && n < p.states;
+      a[nb][s] = in ? p.a[(int64_t)(ch.first + c) * p.states + n] * kLog2e : 0.0f;
+      carry[nb][s] = da[nb][s] = 0.0f;
+      if (in) {
+        if (p.segments > 1)
+          carry[nb][s] = p.segment_state[(int64_t)segment * p.batch * p.channels * p.states + state_at + n];
+        else if (p.dstate_out)
+          carry[nb][s] = p.dstate_out[state_at + n];
+      }
+    }
+  }
+  const int64_t checkpoint_rows = (p.length + kCheckpoint - 1) / kCheckpoint;
+
+  Raw8<T> raw_x, raw_d, raw_z, raw_g;
+  SharedStates<T, kTile, NP> bc;
+  auto fetch = [&](int t0) {
+    const int t = t0 + row;
+    const int n = t < live ? count : 0;
+    raw_x = load8<T>(x + t * p.x_st, n, p.vec & 1);
+    raw_d = load8<T>(delta + t * p.delta_st, n, p.vec & 2);
+    raw_g = load8<T>(dy + t * p.dy_st, n, p.vec & 64);
+    if (p.z) raw_z = load8<T>(z + t * p.z_st, n, p.vec & 4);
+    bc.load(p, batch, ch.group, t0, live);
+  };
+  const int tiles = (end - begin + kTile - 1) / kTile;
+  if (tiles > 0) fetch(begin + (tiles - 1) * kTile);
+  for (int t0 = begin + (tiles - 1) * kTile; t0 >= begin; t0 -= kTile) {
+    const bool in = t0 + row < live;
+    float slope[8], dgate[8];  // softplus'(raw), dy silu'(z)
+    {
+      float xv[8], rv[8], gv[8], zv[8];
+      unpack8<T>(raw_x, xv);
+      unpack8<T>(raw_d, rv);
+      unpack8<T>(raw_g, gv);
+      if (p.z) unpack8<T>(raw_z, zv);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float r = rv[i] + bias[i];
+        slope[i] = p.softplus ? sigmoid(r) : 1.0f;
+        const float dl = p.softplus ? softplus(r) : r;
+        float dv = gv[i];
+        dgate[i] = 0.0f;
+        if (p.z) {
+          const float s = sigmoid(zv[i]);
+          dv *= zv[i] * s;
+          dgate[i] = gv[i] * s * (1.0f + zv[i] * (1.0f - s));
+        }
+        s_dx[row][col + i] = in ? make_float2(dl, xv[i]) : make_float2(0.0f, 0.0f);
+        s_dv[row][col + i] = in ? dv : 0.0f;
+      }
+    }
+    bc.store(s_bc);
+    __syncthreads();
+    if (t0 > begin) fetch(t0 - kTile);
+    for (int nb = 0; nb < kBlocks; ++nb) {
+      for (int half = kTile / kHalf - 1; half >= 0; --half) {
+        const int u0 = half * kHalf;
+        if (t0 + u0 >= p.length) {
+          // past the end: nothing comes from these tokens
+          for (int t = lane; t < kHalf; t += kLanes) {
+            if (nb == 0) s_v[u0 + t][c] = s_gb[u0 + t][c] = s_ga[u0 + t][c] = 0.0f;
+          }
+          if (warp_lane < 16)
+            for (int t = 0; t < kHalf; ++t)
+              s_red[((warp * kTile + u0 + t) * 2 + 0) * 16 + warp_lane] =
+                  s_red[((warp * kTile + u0 + t) * 2 + 1) * 16 + warp_lane] = 0.0f;
+          continue;
+        }
+        float h0[S], h[kHalf][S], e[kHalf][S], da_half[S] = {};
+        {
+          float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (mine)
+            q = *reinterpret_cast<const float4*>(
+                p.checkpoints +
+                (((int64_t)batch * checkpoint_rows + (t0 + u0) / kCheckpoint) * p.channels + ch.first + c) * NP + nb * 16 +
+                lane * S);
+          h0[0] = q.x, h0[1] = q.y, h0[2] = q.z, h0[3] = q.w;
+        }
+#pragma unroll
+        for (int t4 = 0; t4 < kHalf; t4 += 4) {
+          float v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int t = t4 + k;
+            const float2 q = s_dx[u0 + t][c];
+            float bv[S], cv[S];
+            load_f32<S>(s_bc + ((u0 + t) * 2) * NP + nb * 16 + lane * S, bv);
+            load_f32<S>(s_bc + ((u0 + t) * 2 + 1) * NP + nb * 16 + lane * S, cv);
+            v[k] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+              e[t][s] = exp2_fast(q.x * a[nb][s]);
+              h[t][s] = fmaf(e[t][s], t == 0 ? h0[s] : h[t - 1][s], q.x * q.y * bv[s]);
+              v[k] = fmaf(cv[s], h[t][s], v[k]);
+            }
+          }
+          const float sum = transpose_sum<4>(v, lane);
+          float& out = s_v[u0 + t4 + lane][c];
+          out = nb == 0 ? sum : out + sum;
+        }
+#pragma unroll
+        for (int t4 = kHalf - 4; t4 >= 0; t4 -= 4) {
+          float gb[4], ga[4];
+#pragma unroll
+          for (int k2 = 2; k2 >= 0; k2 -= 2) {
+            float db[8], dc[8];
+#pragma unroll
+            for (int k1 = 1; k1 >= 0; --k1) {
+              const int k = k2 + k1, t = t4 + k;
+              const float2 q = s_dx[u0 + t][c];
+              const float dv = s_dv[u0 + t][c];
+              float bv[S], cv[S];
+              load_f32<S>(s_bc + ((u0 + t) * 2) * NP + nb * 16 + lane * S, bv);
+              load_f32<S>(s_bc + ((u0 + t) * 2 + 1) * NP + nb * 16 + lane * S, cv);
+              gb[k] = ga[k] = 0.0f;
+#pragma unroll
+              for (int s = 0; s < S; ++s) {
+                const float g = fmaf(cv[s], dv, carry[nb][s]);
+                gb[k] = fmaf(g, bv[s], gb[k]);
+                db[k1 * 4 + s] = g * q.x * q.y;
+                dc[k1 * 4 + s] = dv * h[t][s];
+                carry[nb][s] = g * e[t][s];
+                const float w = carry[nb][s] * (t == 0 ? h0[s] : h[t - 1][s]);
+                ga[k] = fmaf(a[nb][s], w, ga[k]);
+                da_half[s] = fmaf(q.x, w, da_half[s]);
+              }
+            }
+            const float rb = channel_sum(db, warp_lane);
+            const float rc = channel_sum(dc, warp_lane);
+            const int index = ((warp_lane >> 4 & 1) << 2) | ((warp_lane >> 3 & 1) << 1) | (warp_lane >> 2 & 1);
+            float* out = s_red + ((warp * kTile + u0 + t4 + k2 + (index >> 2)) * 2) * 16 + lane * S + (index & 3);
+            out[0] = rb;
+            out[16] = rc;
+          }
+          const float sb = transpose_sum<4>(gb, lane);
+          const float sa = transpose_sum<4>(ga, lane);
+          float& ob = s_gb[u0 + t4 + lane][c];
+          float& oa = s_ga[u0 + t4 + lane][c];
+          ob = nb == 0 ? sb : ob + sb;
+          oa = nb == 0 ? sa : oa + sa;
+        }
+        // sums of sums: one running sum over thousands of tokens would lose its last bits
+#pragma unroll
+        for (int s = 0; s < S; ++s) da[nb][s] += da_half[s];
+      }
+      __syncthreads();
+      // the warps' parts of dB and dC of these sixteen states
+      for (int i = threadIdx.x; i < kTile * 2 * 16; i += kThreads) {
+        const int t = t0 + i / 32;
+        if (t < end) {
+          float sum = s_red[i];
+#pragma unroll
+          for (int k = 1; k < kWarps; ++k) sum += s_red[k * kTile * 32 + i];
+          p.dbc[(((int64_t)blockIdx.x * p.batch + batch) * p.length + t) * 2 * NP + (i / 16 % 2) * NP + nb * 16 + i % 16] = sum;
+        }
+      }
+      if (kBlocks > 1 && nb + 1 < kBlocks) __syncthreads();
+    }
+    if (t0 + row < end && count > 0) {
+      float o_x[8], o_d[8], o_z[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 q = s_dx[row][col + i];
+        const float dv = s_dv[row][col + i], gb = s_gb[row][col + i];
+        o_x[i] = fmaf(dv, skip[i], q.x * gb);
+        // past a sequence's end delta is a constant zero, though the adjoint still passes through
+        o_d[i] = in ? fmaf(q.y, gb, kLn2 * s_ga[row][col + i]) * slope[i] : 0.0f;
+        o_z[i] = in ? dgate[i] * fmaf(skip[i], q.y, s_v[row][col + i]) : 0.0f;
+        dd[i] = fmaf(dv, q.y, dd[i]);
+        dbias[i] += o_d[i];
+      }
+      const int64_t at = out_at + (int64_t)(t0 + row) * p.channels;
+      store8<T>(static_cast<T*>(p.dx) + at, count, p.vec & 8, o_x);
+      store8<T>(static_cast<T*>(p.ddelta) + at, count, p.vec & 8, o_d);
+      if (p.z) store8<T>(static_cast<T*>(p.dz) + at, count, p.vec & 8, o_z);
+    }
+    __syncthreads();
+  }
+  const int64_t part = (int64_t)segment * p.batch + batch;
+  if (mine) {
+    for (int nb = 0; nb < kBlocks; ++nb) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const int n = nb * 16 + lane * S + s;
+        if (n < p.states) {
+          p.da[(part * p.channels + ch.first + c) * p.states + n] = da[nb][s];
+          if (p.dstate && segment == 0) p.dstate[state_at + n] = carry[nb][s];
+        }
+      }
+    }
+  }
+  // d(D) and d(bias): the 32 tokens' threads of each channel, in a fixed order
+  float* s_sum = smem;  // [kTile][2][kChannels]
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    s_sum[(row * 2 + 0) * kChannels + col + i] = dd[i];
+    s_sum[(row * 2 + 1) * kChannels + col + i] = dbias[i];
+  }
+  __syncthreads();
+  if (threadIdx.x < 2 * kChannels) {
+    const int which = threadIdx.x / kChannels, k = threadIdx.x % kChannels;
+    float sum = 0.0f;
+    for (int t = 0; t < kTile; ++t) sum += s_sum[(t * 2 + which) * kChannels + k];
+    if (k < ch.count) p.dd[(part * 2 + which) * p.channels + ch.first + k] = sum;
+  }
+}
+
+template <int kBlocks>
+constexpr int backward_smem_bytes() {
+  return (32 * (32 + 2) * 2 + 4 * 32 * 36 + 32 * 2 * 16 * kBlocks + 4 * 32 * 2 * 16) * 4;
+}
+
+// dB and dC from the channel blocks' parts, in the order of the blocks.
+template <typename T>
+__global__ void __launch_bounds__(256) selective_scan_dbc_kernel(const float* parts, T* db, T* dc, int64_t tokens, int groups,
+                                                                 int per_group, int states, int padded) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int64_t total = tokens * groups * 2 * padded;
+  if (i >= total) return;
+  const int n = (int)(i % padded);
+  const int which = (int)(i / padded % 2);
+  const int64_t token = i / (2 * padded) / groups;
+  const int group = (int)(i / (2 * padded) % groups);
+  if (n >= states) return;
+  float sum = 0.0f;
+  for (int k = 0; k < per_group; ++k)
+    sum += parts[((int64_t)(group * per_group + k) * tokens + token) * 2 * padded + which * padded + n];
+  (which ? dc : db)[(token * groups + group) * states + n] = from_f32<T>(sum);
+}
+
+// One token: every state is read and written once, kLanes lanes on a channel.
+template <typename T, int kLanes>
+__global__ void __launch_bounds__(128) selective_scan_step_kernel(Params p) {
+  const int64_t at = (int64_t)blockIdx.x * (blockDim.x / kLanes) + threadIdx.x / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const bool in = at < (int64_t)p.batch * p.channels;
+  const int b = in ? (int)(at / p.channels) : 0;
+  const int c = in ? (int)(at % p.channels) : 0;
+  const int group = c / (p.channels / p.groups);
+  const float x = to_f32(static_cast<const T*>(p.x)[b * p.x_sb + c]);
+  float delta = to_f32(static_cast<const T*>(p.delta)[b * p.delta_sb + c]) + (p.bias ? p.bias[c] : 0.0f);
+  if (p.softplus) delta = softplus(delta);
+  const T* bv = static_cast<const T*>(p.b) + b * p.b_sb + group * p.b_sg;
+  const T* cv = static_cast<const T*>(p.c) + b * p.c_sb + group * p.c_sg;
+  float v = 0.0f;
+  if (in) {
+    float* state = p.state_out + at * p.states;
+    const float* a = p.a + (int64_t)c * p.states;
+    const bool four = p.states % 4 == 0 && (p.vec & 8);
+    if (four) {
+      for (int n = lane * 4; n < p.states; n += kLanes * 4) {
+        float4 h = *reinterpret_cast<const float4*>(state + n);
+        const float4 r = *reinterpret_cast<const float4*>(a + n);
+        h.x = fmaf(exp2_fast(delta * kLog2e * r.x), h.x, delta * x * to_f32(bv[n]));
+        h.y = fmaf(exp2_fast(delta * kLog2e * r.y), h.y, delta * x * to_f32(bv[n + 1]));
+        h.z = fmaf(exp2_fast(delta * kLog2e * r.z), h.z, delta * x * to_f32(bv[n + 2]));
+        h.w = fmaf(exp2_fast(delta * kLog2e * r.w), h.w, delta * x * to_f32(bv[n + 3]));
+        v = fmaf(to_f32(cv[n]), h.x, v);
+        v = fmaf(to_f32(cv[n + 1]), h.y, v);
+        v = fmaf(to_f32(cv[n + 2]), h.z, v);
+        v = fmaf(to_f32(cv[n + 3]), h.w, v);
+        *reinterpret_cast<float4*>(state + n) = h;
+      }
+    } else {
+      for (int n = lane; n < p.states; n += kLanes) {
+        const float h = fmaf(exp2_fast(delta * kLog2e * a[n]), state[n], delta * x * to_f32(bv[n]));
+        v = fmaf(to_f32(cv[n]), h, v);
+        state[n] = h;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (in && lane == 0) {
+    if (p.d) v = fmaf(p.d[c], x, v);
+    if (p.z) {
+      const float zv = to_f32(static_cast<const T*>(p.z)[b * p.z_sb + c]);
+      v *= zv * sigmoid(zv);
+    }
+    static_cast<T*>(p.y)[at] = from_f32<T>(v);
+  }
+}
+
+}  // namespace scan
+}  // namespace xe

@@ -1,0 +1,170 @@
+// Shared device helpers of the sequence operators: element types, groups of eight
+// consecutive elements, and the exponential family in float32.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/xe_b200.h"
+
+namespace xe {
+namespace seq {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+  return static_cast<float>(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __float2half_rn(v);
+}
+
+// Eight consecutive elements as they lie in memory: 16 bytes of a 16-bit type, 32 of float.
+template <typename T>
+struct Raw8 {
+  uint4 q[sizeof(T) / 2];
+};
+
+__device__ __forceinline__ uint4 ldg16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+// `count` of the eight elements are in bounds (the others read as zero); `vec`: p is 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const T* p, int count, bool vec) {
+  Raw8<T> r;
+  if (vec && count >= 8) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.q[i] = ldg16(reinterpret_cast<const uint4*>(p) + i);
+    return r;
+  }
+  if constexpr (sizeof(T) == 2) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = 2 * i < count ? reinterpret_cast<const unsigned short*>(p)[2 * i] : 0u;
+      const uint32_t hi = 2 * i + 1 < count ? reinterpret_cast<const unsigned short*>(p)[2 * i + 1] : 0u;
+      w[i] = lo | (hi << 16);
+    }
+    r.q[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = i < count ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+    r.q[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    r.q[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2 && __is_same(T, __nv_bfloat16)) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+  } else {
+    const uint32_t w[8] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w, r.q[1].x, r.q[1].y, r.q[1].z, r.q[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8f(const T* p, int count, bool vec, float (&v)[8]) {
+  unpack8<T>(load8<T>(p, count, vec), v);
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int count, bool vec, const float (&v)[8]) {
+  if (vec && count >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (__is_same(T, __nv_bfloat16)) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < count) p[i] = from_f32<T>(v[i]);
+}
+
+// 2^x and 1/x of the special function unit: relative errors of 2^-22 and 2^-23.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float sigmoid(float v) { return rcp_fast(1.0f + exp2_fast(-kLog2e * v)); }
+
+// softplus(v) = max(v, 0) + log1p(u), u = exp(-|v|) in (0, 1].  log1p(u) = 2 artanh(s) with
+// s = u / (2 + u) <= 1/3, and artanh(s) / s is a polynomial of degree 4 in s^2 <= 1/9 (minimax,
+// relative error 4e-9): the logarithm instruction would lose the small results of negative v.
+__device__ __forceinline__ float softplus(float v) {
+  const float u = exp2_fast(-kLog2e * fabsf(v));
+  const float s = u * rcp_fast(2.0f + u);
+  const float q = s * s;
+  float p = fmaf(0.28178335f, q, 0.27960603f);
+  p = fmaf(p, q, 0.40024910f);
+  p = fmaf(p, q, 0.66666315f);
+  p = fmaf(p, q, 2.0f);
+  return (v > 0.0f || v != v ? v : 0.0f) + s * p;  // a NaN stays
+}
+
+// Length of sequence i of a ragged batch, clamped to [0, most]; `lengths` may be null (all whole).
+__device__ __forceinline__ int sequence_length(const void* lengths, int is64, int i, int most) {
+  if (!lengths) return most;
+  const long long n = is64 ? reinterpret_cast<const long long*>(lengths)[i] : reinterpret_cast<const int*>(lengths)[i];
+  return (int)(n < 0 ? 0 : (n > most ? most : n));
+}
+
+}  // namespace seq
+}  // namespace xe

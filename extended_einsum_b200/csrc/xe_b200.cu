@@ -1,5 +1,6 @@
 // C ABI of the sm_100a kernels (declared in include/xe_b200.h).  One
-// translation unit so that the device status word is shared by all kernels.
+// translation unit so that the device status word is shared by all kernels with
+// bounded waits; the sequence operators, which have none, are in xe_sequence.cu.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
@@ -14,6 +15,7 @@
 #include <string>
 
 #include "../../include/xe_b200.h"
+#include "host_status.h"
 #include "lse_gemm.cuh"
 #include "cp_layer.cuh"
 #include "cp_backward.cuh"
@@ -24,15 +26,25 @@ namespace {
 
 thread_local std::string g_last_error;
 
-xe_status fail(xe_status code, const char* fmt, ...) {
+}  // namespace
+
+namespace xe {
+
+xe_status fail(xe_status code, const char* format, ...) {
   char buf[512];
   va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_start(ap, format);
+  vsnprintf(buf, sizeof(buf), format, ap);
   va_end(ap);
   g_last_error = buf;
   return code;
 }
+
+}  // namespace xe
+
+namespace {
+
+using xe::fail;
 
 xe_status check_launch(const char* what) {
   cudaError_t e = cudaGetLastError();

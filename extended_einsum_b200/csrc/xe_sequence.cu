@@ -1,0 +1,656 @@
+// C ABI of the sequence operators (declared in include/xe_b200.h): the causal convolution, the
+// selective scan, the root-mean-square norm and the products with 4-bit weights.  Their kernels have
+// no device-side waits, so this translation unit has no use of the device status word.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+
+#include "../../include/xe_b200.h"
+#include "causal_conv.cuh"
+#include "host_status.h"
+#include "int4_linear.cuh"
+#include "rms_norm.cuh"
+#include "selective_scan.cuh"
+
+namespace {
+
+using xe::fail;
+
+xe_status launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? XE_OK : fail(XE_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+inline bool is_float(int32_t dtype) { return dtype == XE_F32 || dtype == XE_BF16 || dtype == XE_F16; }
+inline int64_t size_of(int32_t dtype) { return dtype == XE_F32 ? 4 : dtype == XE_BF16 || dtype == XE_F16 ? 2 : 1; }
+
+// Whether rows of eight elements start on 16-byte boundaries everywhere.
+bool vectors(const void* p, int32_t dtype, std::initializer_list<int64_t> strides) {
+  if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  for (int64_t s : strides)
+    if (s * size_of(dtype) % 16) return false;
+  return true;
+}
+
+template <typename F>
+void by_type(int32_t dtype, F f) {
+  if (dtype == XE_F32)
+    f(float{});
+  else if (dtype == XE_BF16)
+    f(__nv_bfloat16{});
+  else
+    f(__half{});
+}
+
+xe_status sum_rows(const float* partial, int64_t rows, int64_t columns, float* out, cudaStream_t stream) {
+  xe::seq::sum_rows_kernel<<<(unsigned)ceil_div(columns, 32), dim3(32, 8), 0, stream>>>(partial, rows, columns, out);
+  return launched("sum_rows");
+}
+
+// ------------------------------------------------------------------ convolution
+
+xe_status check_conv(const char* what, const void* x, const void* weight, const void* y, int64_t batch, int64_t length,
+                     int64_t channels, int64_t width, int32_t activation, int32_t dtype) {
+  // an empty tensor may have no address
+  if (batch * length * channels != 0 && (!x || !y)) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (batch * channels != 0 && !weight) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (!is_float(dtype)) return fail(XE_ERR_NOT_SUPPORTED, "%s: element type %d", what, dtype);
+  if (batch < 0 || length < 0 || channels < 0 || width < 1)
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: negative size or width below 1", what);
+  if (width > 4) return fail(XE_ERR_NOT_SUPPORTED, "%s: width %lld above 4", what, (long long)width);
+  if (activation != 0 && activation != 1) return fail(XE_ERR_INVALID_ARGUMENT, "%s: activation %d", what, activation);
+  if (batch > 65535 || length > INT_MAX / 2 || channels > INT_MAX / 2)
+    return fail(XE_ERR_NOT_SUPPORTED, "%s: a size is above its limit", what);
+  return XE_OK;
+}
+
+template <typename F>
+void by_width(int64_t width, F f) {
+  switch (width) {
+    case 1: f(std::integral_constant<int, 1>{}); break;
+    case 2: f(std::integral_constant<int, 2>{}); break;
+    case 3: f(std::integral_constant<int, 3>{}); break;
+    default: f(std::integral_constant<int, 4>{});
+  }
+}
+
+// Tokens of one thread: enough chunks to fill the device, few enough that the W - 1 rows read again
+// stay a small part.
+int64_t conv_chunk(int64_t batch, int64_t length, int64_t channels) {
+  const int64_t threads = batch * ceil_div(channels, 8);
+  int64_t chunk = 128;
+  while (chunk > 8 && threads * ceil_div(length, chunk) < 148 * 1024) chunk /= 2;
+  return std::max<int64_t>(chunk, ceil_div(length, 65535));
+}
+
+}  // namespace
+
+extern "C" {
+
+xe_status xe_causal_conv1d(const void* x, int64_t x_sb, int64_t x_st, const float* weight, const float* bias,
+                           const void* state, void* y, void* state_out, const void* lengths, int32_t lengths64,
+                           int64_t batch, int64_t length, int64_t channels, int64_t width, int32_t activation,
+                           int32_t dtype, void* stream) {
+  if (xe_status s = check_conv("xe_causal_conv1d", x, weight, y, batch, length, channels, width, activation, dtype)) return s;
+  if (batch == 0 || channels == 0) return XE_OK;
+  xe::conv::Params p{};
+  p.x = x, p.weight = weight, p.bias = bias, p.state = state, p.y = y, p.state_out = state_out;
+  p.lengths = lengths, p.lengths64 = lengths64;
+  p.x_sb = x_sb, p.x_st = x_st;
+  p.batch = (int)batch, p.length = (int)length, p.channels = (int)channels;
+  p.chunk = (int)conv_chunk(batch, length, channels);
+  p.silu = activation;
+  p.vec = (vectors(x, dtype, {x_sb, x_st}) ? 1 : 0) | (vectors(state, dtype, {channels}) ? 2 : 0) |
+          (vectors(y, dtype, {channels}) && vectors(state_out, dtype, {}) ? 4 : 0);
+  const dim3 grid((unsigned)ceil_div(channels, 8 * 128), (unsigned)std::max<int64_t>(1, ceil_div(length, p.chunk)),
+                  (unsigned)batch);
+  by_type(dtype, [&](auto t) {
+    by_width(width, [&](auto w) {
+      xe::conv::causal_conv_kernel<decltype(t), decltype(w)::value><<<grid, 128, 0, as_stream(stream)>>>(p);
+    });
+  });
+  return launched("xe_causal_conv1d");
+}
+
+xe_status xe_causal_conv1d_step(const void* x, int64_t x_sb, const float* weight, const float* bias, void* state, void* y,
+                                int64_t batch, int64_t channels, int64_t width, int32_t activation, int32_t dtype,
+                                void* stream) {
+  if (xe_status s = check_conv("xe_causal_conv1d_step", x, weight, y, batch > 65535 ? 1 : batch, 1, channels, width,
+                               activation, dtype))
+    return s;
+  if (width > 1 && batch * channels != 0 && !state)
+    return fail(XE_ERR_INVALID_ARGUMENT, "xe_causal_conv1d_step: null state");
+  if (batch < 0 || batch > INT_MAX / 2) return fail(XE_ERR_NOT_SUPPORTED, "xe_causal_conv1d_step: batch out of range");
+  if (batch == 0 || channels == 0) return XE_OK;
+  xe::conv::Params p{};
+  p.x = x, p.weight = weight, p.bias = bias, p.y = y, p.state_out = state;
+  p.x_sb = x_sb;
+  p.batch = (int)batch, p.channels = (int)channels, p.silu = activation;
+  p.vec = (vectors(x, dtype, {x_sb}) ? 1 : 0) | (vectors(state, dtype, {channels}) ? 2 : 0) |
+          (vectors(y, dtype, {channels}) ? 4 : 0);
+  const unsigned grid = (unsigned)ceil_div(batch * ceil_div(channels, 8), 128);
+  by_type(dtype, [&](auto t) {
+    by_width(width, [&](auto w) {
+      xe::conv::causal_conv_step_kernel<decltype(t), decltype(w)::value><<<grid, 128, 0, as_stream(stream)>>>(p);
+    });
+  });
+  return launched("xe_causal_conv1d_step");
+}
+
+size_t xe_causal_conv1d_backward_workspace_size(int64_t batch, int64_t length, int64_t channels, int64_t width) {
+  if (batch <= 0 || length < 0 || channels <= 0 || width < 1 || width > 4) return 0;
+  const int64_t chunks = std::max<int64_t>(1, ceil_div(length, conv_chunk(batch, length, channels)));
+  return padded((size_t)(batch * chunks * channels * (width + 1)) * 4);
+}
+
+xe_status xe_causal_conv1d_backward(const void* x, int64_t x_sb, int64_t x_st, const float* weight, const float* bias,
+                                    const void* state, const void* dy, int64_t dy_sb, int64_t dy_st,
+                                    const void* dstate_out, void* dx, void* dstate, float* dweight,
+                                    const void* lengths, int32_t lengths64, int64_t batch, int64_t length,
+                                    int64_t channels, int64_t width, int32_t activation, int32_t dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  const char* what = "xe_causal_conv1d_backward";
+  if (xe_status s = check_conv(what, x, weight, dx, batch, length, channels, width, activation, dtype)) return s;
+  if (channels == 0) return XE_OK;
+  if ((batch * length != 0 && !dy) || !dweight) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (batch == 0) return fail(XE_ERR_INVALID_ARGUMENT, "%s: an empty batch has no gradients", what);
+  if (!workspace || workspace_bytes < xe_causal_conv1d_backward_workspace_size(batch, length, channels, width))
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+  xe::conv::Params p{};
+  p.x = x, p.weight = weight, p.bias = bias, p.state = state;
+  p.dy = dy, p.dy_sb = dy_sb, p.dy_st = dy_st, p.dstate_out = dstate_out, p.dx = dx, p.dstate = dstate;
+  p.partial = static_cast<float*>(workspace);
+  p.lengths = lengths, p.lengths64 = lengths64;
+  p.x_sb = x_sb, p.x_st = x_st;
+  p.batch = (int)batch, p.length = (int)length, p.channels = (int)channels;
+  p.chunk = (int)conv_chunk(batch, length, channels);
+  p.silu = activation;
+  p.vec = (vectors(x, dtype, {x_sb, x_st}) ? 1 : 0) | (vectors(state, dtype, {channels}) ? 2 : 0) |
+          (vectors(dx, dtype, {channels}) ? 4 : 0) | (vectors(dy, dtype, {dy_sb, dy_st}) ? 8 : 0) |
+          (vectors(dstate_out, dtype, {channels}) && vectors(dstate, dtype, {}) ? 16 : 0);
+  const int64_t chunks = std::max<int64_t>(1, ceil_div(length, p.chunk));
+  const dim3 grid((unsigned)ceil_div(channels, 8 * 128), (unsigned)chunks, (unsigned)batch);
+  by_type(dtype, [&](auto t) {
+    by_width(width, [&](auto w) {
+      xe::conv::causal_conv_backward_kernel<decltype(t), decltype(w)::value><<<grid, 128, 0, as_stream(stream)>>>(p);
+    });
+  });
+  if (xe_status s = launched(what)) return s;
+  return sum_rows(p.partial, batch * chunks, channels * (width + 1), dweight, as_stream(stream));
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ scan
+
+namespace {
+
+using ScanParams = xe::scan::Params;
+
+int scan_blocks(int64_t states) { return states <= 16 ? 1 : states <= 32 ? 2 : 4; }
+
+struct ScanPlan {
+  int segments, segment_length;
+  int64_t channel_blocks;
+};
+
+// How many segments the length is split into.  A split costs a pass of its own over x, delta and B, so
+// it is taken only where the whole sequences give the device too few blocks.
+ScanPlan scan_plan(int64_t batch, int64_t length, int64_t channels, int64_t groups) {
+  ScanPlan plan;
+  plan.channel_blocks = groups * ceil_div(channels / groups, 32);
+  const int64_t blocks = plan.channel_blocks * batch;
+  int64_t segments = 1;
+  if (blocks < 296) segments = std::max<int64_t>(1, std::min<int64_t>(ceil_div(592, blocks), length / 128));
+  plan.segment_length = (int)std::max<int64_t>(32, ceil_div(ceil_div(length, segments), 32) * 32);
+  plan.segments = (int)std::max<int64_t>(1, ceil_div(length, plan.segment_length));
+  return plan;
+}
+
+size_t scan_segment_bytes(const ScanPlan& plan, int64_t batch, int64_t channels, int64_t states) {
+  if (plan.segments == 1) return 0;
+  return padded((size_t)(plan.segments * batch * channels * states) * 4) + padded((size_t)(plan.segments * batch * channels) * 4);
+}
+
+xe_status check_scan(const char* what, const xe_selective_scan_args* q, bool step) {
+  if (!q) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
+  // an empty tensor may have no address
+  const int64_t tokens = q->batch * (step ? 1 : q->length);
+  if ((tokens * q->channels != 0 && (!q->x || !q->delta || !q->b || !q->c || !q->a)) ||
+      (q->batch * q->channels != 0 && !q->a))
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (!is_float(q->dtype)) return fail(XE_ERR_NOT_SUPPORTED, "%s: element type %d", what, q->dtype);
+  if (q->batch < 0 || q->length < 0 || q->channels < 0 || q->states < 1 || q->groups < 1)
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: negative size, or no states or groups", what);
+  if (q->channels % q->groups)
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: %lld channels do not divide into %lld groups", what, (long long)q->channels,
+                (long long)q->groups);
+  if (q->states > 64 && !step) return fail(XE_ERR_NOT_SUPPORTED, "%s: %lld states above 64", what, (long long)q->states);
+  if ((!step && q->batch > 65535) || q->batch > INT_MAX / 2 || q->length > INT_MAX / 2 || q->channels > INT_MAX / 2 ||
+      q->states > 65536)
+    return fail(XE_ERR_NOT_SUPPORTED, "%s: a size is above its limit", what);
+  return XE_OK;
+}
+
+ScanParams scan_params(const xe_selective_scan_args* q) {
+  ScanParams p{};
+  p.x = q->x, p.delta = q->delta, p.z = q->z, p.b = q->b, p.c = q->c, p.y = q->y;
+  p.a = q->a, p.d = q->d, p.bias = q->delta_bias;
+  p.state = q->state, p.state_out = q->state_out, p.checkpoints = q->checkpoints;
+  p.lengths = q->lengths, p.lengths64 = q->lengths64;
+  p.x_sb = q->x_sb, p.x_st = q->x_st, p.delta_sb = q->delta_sb, p.delta_st = q->delta_st;
+  p.z_sb = q->z_sb, p.z_st = q->z_st;
+  p.b_sb = q->b_sb, p.b_st = q->b_st, p.b_sg = q->b_sg;
+  p.c_sb = q->c_sb, p.c_st = q->c_st, p.c_sg = q->c_sg;
+  p.batch = (int)q->batch, p.length = (int)q->length, p.channels = (int)q->channels;
+  p.states = (int)q->states, p.groups = (int)q->groups;
+  p.softplus = q->softplus;
+  const int64_t each = q->channels / q->groups;  // a group's first channel starts a vector
+  p.vec = (vectors(q->x, q->dtype, {q->x_sb, q->x_st, each}) ? 1 : 0) |
+          (vectors(q->delta, q->dtype, {q->delta_sb, q->delta_st, each}) ? 2 : 0) |
+          (vectors(q->z, q->dtype, {q->z_sb, q->z_st, each}) ? 4 : 0) |
+          (vectors(q->y, q->dtype, {q->channels, each}) ? 8 : 0) |
+          (vectors(q->b, q->dtype, {q->b_sb, q->b_st, q->b_sg}) ? 16 : 0) |
+          (vectors(q->c, q->dtype, {q->c_sb, q->c_st, q->c_sg}) ? 32 : 0);
+  return p;
+}
+
+void scan_segments(ScanParams& p, const ScanPlan& plan, void* workspace) {
+  p.segments = plan.segments, p.segment_length = plan.segment_length;
+  if (plan.segments == 1) return;
+  p.segment_state = static_cast<float*>(workspace);
+  p.segment_delta = reinterpret_cast<float*>(
+      static_cast<char*>(workspace) + padded((size_t)p.segments * p.batch * p.channels * p.states * 4));
+}
+
+template <xe::scan::Mode kMode>
+xe_status launch_scan(const ScanParams& p, const ScanPlan& plan, int32_t dtype, cudaStream_t stream) {
+  using namespace xe::scan;
+  const dim3 grid((unsigned)plan.channel_blocks, (unsigned)p.batch, (unsigned)(kMode == kFull ? p.segments : p.segments - 1));
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (p.states <= 16)
+      selective_scan_kernel<T, 4, 4, kMode><<<grid, kThreads, 0, stream>>>(p);
+    else if (p.states <= 32)
+      selective_scan_kernel<T, 8, 4, kMode><<<grid, kThreads, 0, stream>>>(p);
+    else
+      selective_scan_kernel<T, 16, 4, kMode><<<grid, kThreads, 0, stream>>>(p);
+  });
+  return launched("selective scan");
+}
+
+template <bool kReverse>
+xe_status join_scan(const ScanParams& p, cudaStream_t stream) {
+  const int64_t total = (int64_t)p.batch * p.channels * p.states;
+  xe::scan::selective_scan_join_kernel<kReverse><<<(unsigned)ceil_div(total, 256), 256, 0, stream>>>(p);
+  return launched("selective scan join");
+}
+
+template <typename T, int kBlocks>
+xe_status launch_scan_backward(const ScanParams& p, const ScanPlan& plan, cudaStream_t stream) {
+  using namespace xe::scan;
+  constexpr int kBytes = backward_smem_bytes<kBlocks>();
+  static std::atomic<uint32_t> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!(done.load() >> (dev & 31) & 1u)) {
+    const cudaError_t e = cudaFuncSetAttribute(selective_scan_backward_kernel<T, kBlocks>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e != cudaSuccess) return fail(XE_ERR_CUDA, "selective scan backward: %s", cudaGetErrorString(e));
+    done.fetch_or(1u << (dev & 31));
+  }
+  const dim3 grid((unsigned)plan.channel_blocks, (unsigned)p.batch, (unsigned)p.segments);
+  selective_scan_backward_kernel<T, kBlocks><<<grid, kThreads, kBytes, stream>>>(p);
+  return launched("selective scan backward");
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t xe_selective_scan_workspace_size(int64_t batch, int64_t length, int64_t channels, int64_t states, int64_t groups) {
+  if (batch <= 0 || length < 0 || channels <= 0 || states < 1 || groups < 1 || channels % groups) return 0;
+  return scan_segment_bytes(scan_plan(batch, length, channels, groups), batch, channels, states);
+}
+
+size_t xe_selective_scan_checkpoint_size(int64_t batch, int64_t length, int64_t channels, int64_t states) {
+  if (batch <= 0 || length <= 0 || channels <= 0 || states < 1 || states > 64) return 0;
+  return (size_t)(batch * ceil_div(length, xe::scan::kCheckpoint) * channels * 16 * scan_blocks(states)) * 4;
+}
+
+xe_status xe_selective_scan(const xe_selective_scan_args* q, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "xe_selective_scan";
+  if (xe_status s = check_scan(what, q, false)) return s;
+  if (q->batch == 0 || q->channels == 0) return XE_OK;
+  if (q->length > 0 && !q->y) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  const ScanPlan plan = scan_plan(q->batch, q->length, q->channels, q->groups);
+  if (workspace_bytes < scan_segment_bytes(plan, q->batch, q->channels, q->states) || (plan.segments > 1 && !workspace))
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+  ScanParams p = scan_params(q);
+  scan_segments(p, plan, workspace);
+  if (p.segments > 1) {
+    if (xe_status s = launch_scan<xe::scan::kStates>(p, plan, q->dtype, as_stream(stream))) return s;
+    if (xe_status s = join_scan<false>(p, as_stream(stream))) return s;
+  }
+  return launch_scan<xe::scan::kFull>(p, plan, q->dtype, as_stream(stream));
+}
+
+xe_status xe_selective_scan_step(const xe_selective_scan_args* q, void* stream) {
+  const char* what = "xe_selective_scan_step";
+  if (xe_status s = check_scan(what, q, true)) return s;
+  if (q->batch == 0 || q->channels == 0) return XE_OK;
+  if (!q->y || !q->state_out) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  ScanParams p = scan_params(q);
+  // bit 3: states and A in groups of four
+  p.vec = reinterpret_cast<uintptr_t>(q->state_out) % 16 == 0 && reinterpret_cast<uintptr_t>(q->a) % 16 == 0 ? 8 : 0;
+  constexpr int kLanes = 4;
+  const int64_t blocks = ceil_div(q->batch * q->channels, 128 / kLanes);
+  if (blocks > INT_MAX) return fail(XE_ERR_NOT_SUPPORTED, "%s: a size is above its limit", what);
+  by_type(q->dtype, [&](auto t) {
+    xe::scan::selective_scan_step_kernel<decltype(t), kLanes><<<(unsigned)blocks, 128, 0, as_stream(stream)>>>(p);
+  });
+  return launched(what);
+}
+
+size_t xe_selective_scan_backward_workspace_size(int64_t batch, int64_t length, int64_t channels, int64_t states,
+                                                 int64_t groups) {
+  if (batch <= 0 || length < 0 || channels <= 0 || states < 1 || states > 64 || groups < 1 || channels % groups) return 0;
+  const ScanPlan plan = scan_plan(batch, length, channels, groups);
+  return scan_segment_bytes(plan, batch, channels, states) +
+         padded((size_t)(plan.channel_blocks * batch * length * 2 * 16 * scan_blocks(states)) * 4) +
+         padded((size_t)(plan.segments * batch * channels * states) * 4) + padded((size_t)(plan.segments * batch * 2 * channels) * 4);
+}
+
+xe_status xe_selective_scan_backward(const xe_selective_scan_args* q, const xe_selective_scan_grads* g, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  const char* what = "xe_selective_scan_backward";
+  if (xe_status s = check_scan(what, q, false)) return s;
+  if (!g) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
+  if (q->channels == 0) return XE_OK;
+  if (!g->da || !g->dd || (q->batch * q->length > 0 && (!g->dy || !g->dx || !g->ddelta || !g->db || !g->dc ||
+                                                        (q->z && !g->dz) || !q->checkpoints)))
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (q->batch == 0) return fail(XE_ERR_INVALID_ARGUMENT, "%s: an empty batch has no gradients", what);
+  if (!workspace || workspace_bytes < xe_selective_scan_backward_workspace_size(q->batch, q->length, q->channels, q->states, q->groups))
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+  const ScanPlan plan = scan_plan(q->batch, q->length, q->channels, q->groups);
+  ScanParams p = scan_params(q);
+  scan_segments(p, plan, workspace);
+  p.dy = g->dy, p.dy_sb = g->dy_sb, p.dy_st = g->dy_st, p.dstate_out = g->dstate_out, p.dstate = g->dstate;
+  p.dx = g->dx, p.ddelta = g->ddelta, p.dz = g->dz;
+  const int64_t each = q->channels / q->groups;
+  p.vec = (p.vec & ~8) | (vectors(g->dy, q->dtype, {g->dy_sb, g->dy_st, each}) ? 64 : 0) |
+          (vectors(g->dx, q->dtype, {q->channels, each}) && vectors(g->ddelta, q->dtype, {}) && vectors(g->dz, q->dtype, {}) ? 8 : 0);
+  const int blocks = scan_blocks(q->states);
+  char* at = static_cast<char*>(workspace) + scan_segment_bytes(plan, q->batch, q->channels, q->states);
+  p.dbc = reinterpret_cast<float*>(at);
+  at += padded((size_t)(plan.channel_blocks * q->batch * q->length * 2 * 16 * blocks) * 4);
+  p.da = reinterpret_cast<float*>(at);
+  at += padded((size_t)(plan.segments * q->batch * q->channels * q->states) * 4);
+  p.dd = reinterpret_cast<float*>(at);
+  cudaStream_t st = as_stream(stream);
+  if (p.segments > 1) {
+    if (xe_status s = launch_scan<xe::scan::kAdjoint>(p, plan, q->dtype, st)) return s;
+    if (xe_status s = join_scan<true>(p, st)) return s;
+  }
+  xe_status status = XE_OK;
+  by_type(q->dtype, [&](auto t) {
+    using T = decltype(t);
+    status = blocks == 1   ? launch_scan_backward<T, 1>(p, plan, st)
+             : blocks == 2 ? launch_scan_backward<T, 2>(p, plan, st)
+                           : launch_scan_backward<T, 4>(p, plan, st);
+    const int64_t tokens = q->batch * q->length;
+    const int64_t total = tokens * q->groups * 2 * 16 * blocks;
+    if (status == XE_OK && total > 0) {
+      xe::scan::selective_scan_dbc_kernel<T><<<(unsigned)ceil_div(total, 256), 256, 0, st>>>(
+          p.dbc, static_cast<T*>(g->db), static_cast<T*>(g->dc), tokens, (int)q->groups,
+          (int)(plan.channel_blocks / q->groups), (int)q->states, 16 * blocks);
+      status = launched(what);
+    }
+  });
+  if (status != XE_OK) return status;
+  const int64_t parts = plan.segments * q->batch;
+  if (xe_status s = sum_rows(p.da, parts, q->channels * q->states, g->da, st)) return s;
+  return sum_rows(p.dd, parts, 2 * q->channels, g->dd, st);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ norm
+
+namespace {
+
+struct NormShape {
+  int groups, warps_per_row, threads, rows_per_block;
+};
+
+// Groups of eight elements per thread and warps per row.
+bool norm_shape(int64_t columns, int64_t rows, bool backward, NormShape& s) {
+  const int64_t groups = ceil_div(columns, 8);
+  if (groups <= 256)
+    s.groups = 1;
+  else if (groups <= 1024)
+    s.groups = 2;
+  else if (groups <= 2048)
+    s.groups = 4;
+  else if (groups <= 8192)
+    s.groups = 8;
+  else
+    return false;
+  (void)rows;
+  (void)backward;
+  int wpr = 1;
+  while ((int64_t)wpr * 32 * s.groups < groups) wpr *= 2;
+  s.warps_per_row = wpr;
+  s.threads = std::max(256, wpr * 32);
+  s.rows_per_block = s.threads / (wpr * 32);
+  return true;
+}
+
+template <typename F>
+void by_groups(int groups, F f) {
+  switch (groups) {
+    case 1: f(std::integral_constant<int, 1>{}); break;
+    case 2: f(std::integral_constant<int, 2>{}); break;
+    case 4: f(std::integral_constant<int, 4>{}); break;
+    default: f(std::integral_constant<int, 8>{});
+  }
+}
+
+// The residual stream is of the input's type or float32.
+template <typename F>
+void by_types(int32_t dtype, int32_t residual_dtype, F f) {
+  by_type(dtype, [&](auto t) {
+    if (residual_dtype == XE_F32)
+      f(t, float{});
+    else
+      f(t, t);
+  });
+}
+
+xe_status check_norm(const char* what, int64_t rows, int64_t columns, int32_t dtype, int32_t residual_dtype,
+                     int32_t weight_dtype) {
+  if (!is_float(dtype)) return fail(XE_ERR_NOT_SUPPORTED, "%s: element type %d", what, dtype);
+  if (residual_dtype != dtype && residual_dtype != XE_F32)
+    return fail(XE_ERR_NOT_SUPPORTED, "%s: residual type %d with elements of type %d", what, residual_dtype, dtype);
+  if (weight_dtype != dtype && weight_dtype != XE_F32)
+    return fail(XE_ERR_NOT_SUPPORTED, "%s: weight type %d with elements of type %d", what, weight_dtype, dtype);
+  if (rows < 0 || columns < 1) return fail(XE_ERR_INVALID_ARGUMENT, "%s: negative rows, or no columns", what);
+  if (columns > 65536) return fail(XE_ERR_NOT_SUPPORTED, "%s: %lld columns above 65536", what, (long long)columns);
+  return XE_OK;
+}
+
+int64_t norm_backward_blocks(int64_t rows, const NormShape& s) {
+  return std::min<int64_t>(ceil_div(rows, s.rows_per_block), 148 * 2);
+}
+
+}  // namespace
+
+extern "C" {
+
+xe_status xe_rms_norm(const void* x, int64_t x_row, const void* residual, int64_t residual_row, const void* weight, void* y,
+                      void* sum, float* scale, int64_t rows, int64_t columns, float eps, int32_t dtype,
+                      int32_t residual_dtype, int32_t weight_dtype, int32_t out_dtype, void* stream) {
+  const char* what = "xe_rms_norm";
+  if (xe_status s = check_norm(what, rows, columns, dtype, residual_dtype, weight_dtype)) return s;
+  if (rows > 0 && (!x || !y || (residual && !sum))) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  const bool quantize = out_dtype == XE_E4M3 || out_dtype == XE_I8;
+  if (!quantize && out_dtype != dtype) return fail(XE_ERR_NOT_SUPPORTED, "%s: output type %d", what, out_dtype);
+  if (quantize && rows > 0 && !scale) return fail(XE_ERR_INVALID_ARGUMENT, "%s: 8-bit outputs need scales", what);
+  if (rows == 0) return XE_OK;
+  NormShape shape;
+  if (!norm_shape(columns, rows, false, shape)) return fail(XE_ERR_NOT_SUPPORTED, "%s: too many columns", what);
+  const int64_t blocks = ceil_div(rows, shape.rows_per_block);
+  if (blocks > INT_MAX) return fail(XE_ERR_NOT_SUPPORTED, "%s: too many rows", what);
+  xe::norm::Params p{};
+  p.x = x, p.residual = residual, p.weight = weight, p.y = y, p.sum = sum, p.scale = scale;
+  p.x_row = x_row, p.r_row = residual_row, p.rows = rows, p.columns = (int)columns, p.eps = eps;
+  p.quantize = quantize ? out_dtype : 0;
+  p.weight_f32 = weight_dtype == XE_F32;
+  const bool vec = vectors(x, dtype, {x_row, columns}) && vectors(residual, residual_dtype, {residual_row}) &&
+                   vectors(sum, residual_dtype, {columns}) && vectors(weight, weight_dtype, {}) && vectors(y, dtype, {}) &&
+                   columns % 8 == 0;
+  by_types(dtype, residual_dtype, [&](auto t, auto r) {
+    by_groups(shape.groups, [&](auto g) {
+      auto kernel = vec ? xe::norm::rms_norm_kernel<decltype(t), decltype(r), decltype(g)::value, true>
+                        : xe::norm::rms_norm_kernel<decltype(t), decltype(r), decltype(g)::value, false>;
+      kernel<<<(unsigned)blocks, shape.threads, 0, as_stream(stream)>>>(p, shape.warps_per_row);
+    });
+  });
+  return launched(what);
+}
+
+size_t xe_rms_norm_backward_workspace_size(int64_t rows, int64_t columns) {
+  NormShape shape;
+  if (rows <= 0 || columns < 1 || !norm_shape(columns, rows, true, shape)) return 0;
+  return padded((size_t)(norm_backward_blocks(rows, shape) * shape.rows_per_block * columns) * 4);
+}
+
+xe_status xe_rms_norm_backward(const void* sum, int64_t sum_row, const void* addend, int64_t addend_row, const void* weight, const void* dy, int64_t dy_row,
+                               const void* dsum, int64_t dsum_row, void* dx, float* dweight, int64_t rows,
+                               int64_t columns, float eps, int32_t dtype, int32_t residual_dtype, int32_t weight_dtype,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "xe_rms_norm_backward";
+  if (xe_status s = check_norm(what, rows, columns, dtype, residual_dtype, weight_dtype)) return s;
+  if (!sum || !dy || !dx) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (rows == 0) return fail(XE_ERR_INVALID_ARGUMENT, "%s: no rows, no gradients", what);
+  if (dweight && (!workspace || workspace_bytes < xe_rms_norm_backward_workspace_size(rows, columns)))
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+  NormShape shape;
+  if (!norm_shape(columns, rows, true, shape)) return fail(XE_ERR_NOT_SUPPORTED, "%s: too many columns", what);
+  const int64_t blocks = norm_backward_blocks(rows, shape);
+  xe::norm::BackwardParams p{};
+  p.sum = sum, p.addend = addend, p.a_row = addend_row, p.weight = weight, p.dy = dy, p.dsum = dsum, p.dx = dx;
+  p.partial = dweight ? static_cast<float*>(workspace) : nullptr;
+  p.s_row = sum_row, p.dy_row = dy_row, p.dsum_row = dsum_row;
+  p.rows = rows, p.columns = (int)columns, p.eps = eps, p.weight_f32 = weight_dtype == XE_F32;
+  const bool vec = vectors(sum, residual_dtype, {sum_row, columns}) && vectors(addend, dtype, {addend_row}) && vectors(dy, dtype, {dy_row}) &&
+                   vectors(dsum, residual_dtype, {dsum_row}) && vectors(weight, weight_dtype, {}) &&
+                   vectors(dx, residual_dtype, {}) && columns % 8 == 0;
+  by_types(dtype, residual_dtype, [&](auto t, auto r) {
+    by_groups(shape.groups, [&](auto g) {
+      auto kernel = vec ? xe::norm::rms_norm_backward_kernel<decltype(t), decltype(r), decltype(g)::value, true>
+                        : xe::norm::rms_norm_backward_kernel<decltype(t), decltype(r), decltype(g)::value, false>;
+      kernel<<<(unsigned)blocks, shape.threads, 0, as_stream(stream)>>>(p, shape.warps_per_row);
+    });
+  });
+  if (xe_status s = launched(what)) return s;
+  if (!dweight) return XE_OK;
+  return sum_rows(p.partial, blocks * shape.rows_per_block, columns, dweight, as_stream(stream));
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ 4-bit weights
+
+namespace {
+
+constexpr int kStages = 4;
+
+template <typename X, int kTiles, bool kSplit>
+xe_status launch_int4(xe::int4::Params& p, int64_t rows, cudaStream_t stream) {
+  using namespace xe::int4;
+  constexpr int kRing = kWarps * kStages * kStageBytes;
+  constexpr int kBudget = 65536;
+  const int64_t whole = ceil_div(p.inputs, kStageK) * kStageK;
+  p.chunk = (int)std::min<int64_t>(whole, kBudget / (kTiles * 8 * 2) / kStageK * kStageK);
+  p.pitch = p.chunk + 32;  // bytes: 64 past a multiple of 128, two columns' reads in different banks
+  p.warps_k = kTiles == 1 ? 8 : kTiles == 2 ? 4 : 2;
+  const int bytes = kRing + kTiles * 8 * p.pitch * 2;
+  constexpr int kMost = kRing + kBudget + kTiles * 8 * 32 * 2;
+  static std::atomic<uint32_t> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!(done.load() >> (dev & 31) & 1u)) {
+    const cudaError_t e = cudaFuncSetAttribute(int4_linear_kernel<X, kTiles, kSplit, kStages>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (e != cudaSuccess) return fail(XE_ERR_CUDA, "xe_int4_linear: %s", cudaGetErrorString(e));
+    done.fetch_or(1u << (dev & 31));
+  }
+  const int per_block = 16 * (kWarps / p.warps_k);
+  const dim3 grid((unsigned)ceil_div(p.outputs, per_block), (unsigned)ceil_div(rows, p.tokens));
+  int4_linear_kernel<X, kTiles, kSplit, kStages><<<grid, kWarps * 32, bytes, stream>>>(p);
+  return launched("xe_int4_linear");
+}
+
+template <typename X>
+xe_status run_int4(xe::int4::Params& p, cudaStream_t stream) {
+  const int most = 64 / p.pieces;  // tokens of a block
+  p.tokens = std::min(p.rows, most);
+  const int columns = p.tokens * p.pieces;
+  const bool split = p.group % xe::int4::kStageK != 0;
+  auto go = [&](auto tiles) {
+    constexpr int n = decltype(tiles)::value;
+    return split ? launch_int4<X, n, true>(p, p.rows, stream) : launch_int4<X, n, false>(p, p.rows, stream);
+  };
+  if (columns <= 8) return go(std::integral_constant<int, 1>{});
+  if (columns <= 16) return go(std::integral_constant<int, 2>{});
+  if (columns <= 32) return go(std::integral_constant<int, 4>{});
+  return go(std::integral_constant<int, 8>{});
+}
+
+}  // namespace
+
+extern "C" {
+
+xe_status xe_int4_linear(const void* x, int64_t x_row, const float* x_scale, const void* packed, int64_t packed_row,
+                         const void* scales, const void* zeros, void* y, int64_t rows, int64_t inputs, int64_t outputs,
+                         int64_t group, int32_t x_dtype, int32_t scale_dtype, int32_t y_dtype, void* stream) {
+  const char* what = "xe_int4_linear";
+  if (rows * outputs != 0 && (!x || !packed || !scales || !y))
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (!is_float(x_dtype) && x_dtype != XE_E4M3 && x_dtype != XE_I8)
+    return fail(XE_ERR_NOT_SUPPORTED, "%s: activations of type %d", what, x_dtype);
+  if (!is_float(scale_dtype) || !is_float(y_dtype))
+    return fail(XE_ERR_NOT_SUPPORTED, "%s: scales of type %d, result of type %d", what, scale_dtype, y_dtype);
+  if (rows < 0 || outputs < 0 || inputs < 1 || group < 1 || inputs % group)
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: %lld inputs in groups of %lld", what, (long long)inputs, (long long)group);
+  if (group % 32) return fail(XE_ERR_NOT_SUPPORTED, "%s: groups of %lld, not a multiple of 32", what, (long long)group);
+  if (reinterpret_cast<uintptr_t>(packed) % 16 || packed_row % 16)
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: rows of codes must start on 16-byte boundaries", what);
+  if (rows > INT_MAX / 4 || inputs > INT_MAX / 4 || outputs > INT_MAX / 4 || ceil_div(rows, 21) > 65535)
+    return fail(XE_ERR_NOT_SUPPORTED, "%s: a size is above its limit", what);
+  if (rows == 0 || outputs == 0) return XE_OK;
+  xe::int4::Params p{};
+  p.x = x, p.x_scale = x_scale, p.packed = static_cast<const uint8_t*>(packed), p.scales = scales;
+  p.zeros = static_cast<const uint8_t*>(zeros), p.y = y;
+  p.x_row = x_row, p.packed_row = packed_row;
+  p.rows = (int)rows, p.inputs = (int)inputs, p.outputs = (int)outputs, p.group = (int)group;
+  p.scale_dtype = scale_dtype, p.y_dtype = y_dtype;
+  p.pieces = x_dtype == XE_F32 ? 3 : 1;
+  cudaStream_t st = as_stream(stream);
+  switch (x_dtype) {
+    case XE_F32: return run_int4<float>(p, st);
+    case XE_BF16: return run_int4<__nv_bfloat16>(p, st);
+    case XE_F16: return run_int4<__half>(p, st);
+    case XE_E4M3: return run_int4<__nv_fp8_e4m3>(p, st);
+    default: return run_int4<int8_t>(p, st);
+  }
+}
+
+}  // extern "C"

@@ -864,3 +864,18 @@ def set_wait_timeout_ns(ns: int) -> None:
     if torch.cuda.is_available():
         torch.cuda.synchronize()
     _lib.check(_lib.load().xe_set_wait_timeout_ns(int(ns)), "xe_set_wait_timeout_ns")
+
+
+# ---------------------------------------------------------------------------
+# operators along an ordered axis (sequence.py)
+
+from .sequence import (  # noqa: E402
+    causal_conv1d,
+    causal_conv1d_step,
+    int4_linear,
+    int4_pack,
+    int4_quantize,
+    rms_norm,
+    selective_scan,
+    selective_scan_step,
+)

@@ -455,6 +455,128 @@ xe_status xe_elementwise(int32_t op, const float* a, const int64_t* a_strides, c
                          const float* c, const int64_t* c_strides, float* y, const int64_t* shape, int32_t ndim,
                          void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Sequence operators: a norm, 4-bit products, a short causal convolution and a
+ * selective state space scan, the parts of a layer that runs along an ordered axis.
+ * No counterpart in the reference, where a chain of T stable einsums is T nodes of
+ * the graph (interface/tensor_expression.py:196-265) and parameters are float32.
+ *
+ * Tensors are channel-last, (batch, length, channels), with the channels
+ * contiguous and the other strides given in elements; outputs are contiguous.
+ * Parameters (filters, A, D, biases) and states of the scan are float32, sums,
+ * statistics and states are held in float32, and each output is rounded once.
+ * Results do not depend on the order in which blocks run. */
+
+/* Element types. */
+typedef enum { XE_F32 = 0, XE_BF16 = 1, XE_F16 = 2, XE_E4M3 = 3, XE_I8 = 4 } xe_dtype;
+
+/* y[b,t,c] = act(bias[c] + sum_j weight[c,j] v[b, t - width + 1 + j, c]), where v is x
+ * and, before t = 0, the state: the width - 1 inputs before, (batch, width - 1,
+ * channels), or zeros where `state` is NULL.  activation: 0 none, 1 SiLU.
+ * state_out (or NULL) receives the last width - 1 entries of [state, x[:length]].
+ * `lengths` (or NULL): per sequence, int32 or (lengths64 != 0) int64 on the
+ * device, clamped to [0, length]; positions past it are not read and their y is 0.
+ * width 1 to 4; XE_F32, XE_BF16 or XE_F16. */
+xe_status xe_causal_conv1d(const void* x, int64_t x_sb, int64_t x_st, const float* weight, const float* bias,
+                           const void* state, void* y, void* state_out, const void* lengths, int32_t lengths64,
+                           int64_t batch, int64_t length, int64_t channels, int64_t width, int32_t activation,
+                           int32_t dtype, void* stream);
+
+/* One token of the convolution: y (batch, channels); `state` is read and shifted in place. */
+xe_status xe_causal_conv1d_step(const void* x, int64_t x_sb, const float* weight, const float* bias, void* state, void* y,
+                                int64_t batch, int64_t channels, int64_t width, int32_t activation, int32_t dtype,
+                                void* stream);
+
+/* Gradients of xe_causal_conv1d: dx, dstate (or NULL) and dweight, float32 (channels,
+ * width + 1) with the bias's gradient in the last column.  dstate_out (or NULL) is the
+ * gradient of the new state. */
+size_t xe_causal_conv1d_backward_workspace_size(int64_t batch, int64_t length, int64_t channels, int64_t width);
+xe_status xe_causal_conv1d_backward(const void* x, int64_t x_sb, int64_t x_st, const float* weight, const float* bias,
+                                    const void* state, const void* dy, int64_t dy_sb, int64_t dy_st,
+                                    const void* dstate_out, void* dx, void* dstate, float* dweight,
+                                    const void* lengths, int32_t lengths64, int64_t batch, int64_t length,
+                                    int64_t channels, int64_t width, int32_t activation, int32_t dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* The selective scan.  For channel d of group g = d / (channels / groups):
+ *   delta_t = raw + delta_bias[d], then softplus if `softplus`
+ *   h_t[n]  = exp(delta_t a[d,n]) h_{t-1}[n] + delta_t x_t b_t[g,n]
+ *   y_t     = (sum_n c_t[g,n] h_t[n] + d[d] x_t) * silu(z_t)
+ * d, z, delta_bias may be NULL (their terms fall away).  state (batch, channels,
+ * states) is h before the first token (NULL: zero), state_out (or NULL) h after the
+ * last.  `lengths` as above: positions past a sequence's length leave its state as it is
+ * and have y = 0.  x, delta, z, b, c and y share one type (XE_F32, XE_BF16, XE_F16); at
+ * most 64 states (any number in the single-token form).
+ * checkpoints (or NULL) receives the states that xe_selective_scan_backward starts from,
+ * xe_selective_scan_checkpoint_size() bytes. */
+typedef struct {
+  const void *x, *delta, *z, *b, *c;
+  void* y;
+  const float *a, *d, *delta_bias;
+  const float* state;
+  float* state_out;
+  float* checkpoints;
+  const void* lengths;
+  int64_t x_sb, x_st, delta_sb, delta_st, z_sb, z_st, b_sb, b_st, b_sg, c_sb, c_st, c_sg;
+  int64_t batch, length, channels, states, groups;
+  int32_t lengths64, softplus, dtype;
+} xe_selective_scan_args;
+
+size_t xe_selective_scan_workspace_size(int64_t batch, int64_t length, int64_t channels, int64_t states, int64_t groups);
+size_t xe_selective_scan_checkpoint_size(int64_t batch, int64_t length, int64_t channels, int64_t states);
+xe_status xe_selective_scan(const xe_selective_scan_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token (length and the token strides are not used): state_out is read and
+ * overwritten in place, y is (batch, channels). */
+xe_status xe_selective_scan_step(const xe_selective_scan_args* args, void* stream);
+
+/* Gradients of xe_selective_scan; args as in the forward call, with its checkpoints (y
+ * and state_out are not used).  dx, ddelta, dz: like x, contiguous; da (channels,
+ * states) and dd (2, channels; row 0 of d, row 1 of delta_bias) float32; db, dc
+ * (batch, length, groups, states) of x's type; dstate_out (or NULL) the gradient of
+ * state_out, dstate (or NULL) receives that of state. */
+typedef struct {
+  const void* dy;
+  const float* dstate_out;
+  void *dx, *ddelta, *dz, *db, *dc;
+  float *da, *dd, *dstate;
+  int64_t dy_sb, dy_st;
+} xe_selective_scan_grads;
+
+size_t xe_selective_scan_backward_workspace_size(int64_t batch, int64_t length, int64_t channels, int64_t states,
+                                                 int64_t groups);
+xe_status xe_selective_scan_backward(const xe_selective_scan_args* args, const xe_selective_scan_grads* grads,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = s rsqrt(mean(s^2) + eps) weight over rows of `columns`, s = x + residual (or x
+ * where `residual` is NULL); `sum` receives s (needed with a residual).  residual and sum
+ * are of x's type or XE_F32, weight (or NULL) likewise.  out_dtype: x's type, or XE_E4M3 /
+ * XE_I8 with one float32 scale per row, scale = max(max|y| / (448 or 127), 2^-126),
+ * y ~ q * scale. */
+xe_status xe_rms_norm(const void* x, int64_t x_row, const void* residual, int64_t residual_row, const void* weight, void* y,
+                      void* sum, float* scale, int64_t rows, int64_t columns, float eps, int32_t dtype,
+                      int32_t residual_dtype, int32_t weight_dtype, int32_t out_dtype, void* stream);
+
+/* Gradients: dx (of residual_dtype, for x and the residual alike) with dsum (or NULL) the
+ * gradient of the forward call's `sum`, dweight (or NULL) float32 (columns).  The normed
+ * values are `sum` (residual_dtype) plus `addend` (dtype, or NULL): the residual and x, or
+ * a float32 sum alone; a 16-bit sum would carry its rounding into dweight. */
+size_t xe_rms_norm_backward_workspace_size(int64_t rows, int64_t columns);
+xe_status xe_rms_norm_backward(const void* sum, int64_t sum_row, const void* addend, int64_t addend_row, const void* weight, const void* dy, int64_t dy_row,
+                               const void* dsum, int64_t dsum_row, void* dx, float* dweight, int64_t rows,
+                               int64_t columns, float eps, int32_t dtype, int32_t residual_dtype, int32_t weight_dtype,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* y[m,o] = x_scale[m] sum_k x[m,k] scales[o, k / group] (q[o,k] - zeros[o, k / group]).
+ * q: two codes to a byte, the even k in the low nibble, rows `packed_row` bytes apart on
+ * 16-byte boundaries; scales (outputs, inputs / group) contiguous, of type XE_F32, XE_BF16 or
+ * XE_F16; zeros one byte each, 0 to 15, or NULL for 8.  x: XE_F32, XE_BF16, XE_F16, or XE_E4M3 /
+ * XE_I8 with x_scale per row (or NULL: 1).  `group` is a multiple of 32 that divides `inputs`.
+ * Made for few rows (the weights are read again for every 64 of them, 21 with XE_F32). */
+xe_status xe_int4_linear(const void* x, int64_t x_row, const float* x_scale, const void* packed, int64_t packed_row,
+                         const void* scales, const void* zeros, void* y, int64_t rows, int64_t inputs, int64_t outputs,
+                         int64_t group, int32_t x_dtype, int32_t scale_dtype, int32_t y_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
