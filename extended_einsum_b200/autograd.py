@@ -359,9 +359,9 @@ class RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps: float):
         if residual is None:
-            y, total = ops.rms_norm(x, weight, eps=eps), x
+            y, total = sequence._norm_forward(x, weight, None, eps, None), x
         else:
-            y, total = ops.rms_norm(x, weight, residual=residual, eps=eps)
+            y, total = sequence._norm_forward(x, weight, residual, eps, None)
         # a float32 sum stands for itself; a 16-bit one has been rounded, and is added again
         if residual is None or total.dtype == torch.float32:
             ctx.save_for_backward(total, None, weight)

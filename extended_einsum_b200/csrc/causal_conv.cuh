@@ -7,9 +7,14 @@
 //
 //   dpre = dy * silu'(pre),  dv[t] = sum_j w_j dpre[t + W - 1 - j],  dw_j = sum_t dpre[t] v[t - W + 1 + j].
 //
-// Bound by memory: a thread owns eight channels (16 bytes of a 16-bit type) and walks a chunk of
-// tokens with the window in registers, so that x is read once and W - 1 rows again per chunk.
+// Bound by memory: a thread owns V channels (four where rows are aligned to four elements, else one, so
+// that a warp's accesses stay contiguous) and walks a chunk of tokens with the window in registers, so that x
+// is read once and W - 1 rows again per chunk.  Eight rows are on their way per thread, through shared
+// memory places of its own (no barrier), so that they cost no registers.
 #pragma once
+
+#include <algorithm>
+#include <type_traits>
 
 #include "seq_common.cuh"
 
@@ -17,6 +22,9 @@ namespace xe {
 namespace conv {
 
 using namespace seq;
+
+constexpr int kThreads = 128;
+constexpr int kDepth = 8;  // rows in flight per thread
 
 struct Params {
   const void* x;
@@ -28,172 +36,229 @@ struct Params {
   const void* lengths;
   int lengths64;
   int64_t x_sb, x_st;
-  int batch, length, channels, chunk;
+  int batch, length, channels, chunk, chunks;
   int silu;
-  int vec;  // bit 0: x, 1: state, 2: y and state_out, 3: dy, 4: dstate
   // backward
   const void* dy;
   int64_t dy_sb, dy_st;
   const void* dstate_out;  // gradient of the new state, contiguous, or null
   void* dx;
   void* dstate;    // gradient of the state, contiguous, or null
-  float* partial;  // (batch * chunks, channels, width + 1)
+  float* partial;  // (batch * chunks, width + 1, channels)
 };
 
-template <typename T, int W>
-__device__ __forceinline__ void load_filter(const Params& p, int c0, int count, float (&w)[W][8], float (&b)[8]) {
+// V neighbouring channels as they lie in memory.
+template <typename T, int V>
+struct Pack {
+  static_assert(V == 1 || V == 4, "one element or four");
+  using Q = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
+  union {
+    T e[V];
+    typename std::conditional<V == 1, T, Q>::type q;
+  };
+  __device__ __forceinline__ Pack() {}
+  __device__ __forceinline__ void load(const T* p) { q = *reinterpret_cast<const decltype(q)*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<decltype(q)*>(p) = q; }
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    b[i] = p.bias && i < count ? p.bias[c0 + i] : 0.0f;
+    for (int i = 0; i < V; ++i) e[i] = from_f32<T>(0.0f);
+  }
+  __device__ __forceinline__ float get(int i) const { return to_f32(e[i]); }
+  __device__ __forceinline__ void set(int i, float v) { e[i] = from_f32<T>(v); }
+};
+
+// kDepth rows on their way.  All indices are compile-time constants where V == 1 holds them in registers.
+template <typename T, int V>
+struct Rows {
+  static constexpr int kBytes = V == 1 ? 0 : kDepth * kThreads * V * (int)sizeof(T);  // shared memory of a block
+  Pack<T, V> held[V == 1 ? kDepth : 1];
+  uint32_t base;
+
+  __device__ __forceinline__ explicit Rows(uint32_t smem) : base(smem + threadIdx.x * V * sizeof(T)) {}
+  __device__ __forceinline__ void issue(int k, const T* p) {
+    if constexpr (V == 1) {
+      held[k].load(p);
+    } else {
+      const uint32_t at = base + k * (kThreads * V * sizeof(T));
+      if constexpr (sizeof(T) == 2)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(at), "l"(p) : "memory");
+      else
+        cp_async16(at, p);
+    }
+  }
+  __device__ __forceinline__ Pack<T, V> get(int k) const {
+    if constexpr (V == 1) {
+      return held[k];
+    } else {
+      Pack<T, V> r;
+      const uint32_t at = base + k * (kThreads * V * sizeof(T));
+      if constexpr (sizeof(T) == 2)
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.q.x), "=r"(r.q.y) : "r"(at) : "memory");
+      else
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.q.x), "=r"(r.q.y), "=r"(r.q.z), "=r"(r.q.w) : "r"(at) : "memory");
+      return r;
+    }
+  }
+};
+
+// This thread's place: channels c0 .. c0 + V - 1 and a chunk of tokens of batch entry b.
+struct Place {
+  int b, c0, chunk;
+  bool in;
+};
+template <int V>
+__device__ __forceinline__ Place place(const Params& p) {
+  const int vectors = p.channels / V;
+  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  return {(int)blockIdx.y, (int)(at % vectors) * V, (int)(at / vectors), at < (int64_t)vectors * p.chunks};
+}
+
+template <int W, int V>
+__device__ __forceinline__ void load_filter(const Params& p, int c0, float (&w)[W][V], float (&b)[V]) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) w[j][i] = i < count ? p.weight[(int64_t)(c0 + i) * W + j] : 0.0f;
+  for (int i = 0; i < V; ++i) {
+    b[i] = p.bias ? p.bias[c0 + i] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j][i] = p.weight[(int64_t)(c0 + i) * W + j];
   }
 }
 
 // v[t] of the sequence with the state in front: t in [-(W - 1), length).
-template <typename T, int W>
-__device__ __forceinline__ Raw8<T> value_at(const Params& p, int b, int t, int c0, int count) {
+template <typename T, int W, int V>
+__device__ __forceinline__ Pack<T, V> value_at(const Params& p, int b, int t, int c0) {
+  Pack<T, V> r;
   if (t >= 0)
-    return load8<T>(static_cast<const T*>(p.x) + b * p.x_sb + t * p.x_st + c0, count, p.vec & 1);
-  if (p.state)
-    return load8<T>(static_cast<const T*>(p.state) + ((int64_t)b * (W - 1) + (t + W - 1)) * p.channels + c0, count,
-                    p.vec & 2);
-  Raw8<T> z;
-#pragma unroll
-  for (int i = 0; i < (int)(sizeof(T) / 2); ++i) z.q[i] = make_uint4(0, 0, 0, 0);
-  return z;
+    r.load(static_cast<const T*>(p.x) + b * p.x_sb + t * p.x_st + c0);
+  else if (p.state)
+    r.load(static_cast<const T*>(p.state) + ((int64_t)b * (W - 1) + (t + W - 1)) * p.channels + c0);
+  else
+    r.zero();
+  return r;
 }
 
-template <typename T>
-__device__ __forceinline__ void store_raw(T* p, int count, bool vec, const Raw8<T>& r) {
-  float v[8];
-  unpack8<T>(r, v);
-  store8<T>(p, count, vec, v);
-}
-
-template <typename T, int W>
-__global__ void __launch_bounds__(128) causal_conv_kernel(Params p) {
-  const int c0 = (blockIdx.x * blockDim.x + threadIdx.x) * 8;
-  if (c0 >= p.channels) return;
-  const int count = min(8, p.channels - c0);
-  const int b = blockIdx.z;
-  const int first = blockIdx.y * p.chunk;
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kThreads) causal_conv_kernel(const __grid_constant__ Params p) {
+  __shared__ __align__(16) uint8_t smem[std::max(16, Rows<T, V>::kBytes)];
+  const Place at = place<V>(p);
+  if (!at.in) return;
+  const int b = at.b, c0 = at.c0;
+  const int first = at.chunk * p.chunk;
   const int last = min(first + p.chunk, p.length);
   const int length = sequence_length(p.lengths, p.lengths64, b, p.length);
-  T* y = static_cast<T*>(p.y) + (int64_t)b * p.length * p.channels + c0;
-  if (p.state_out && blockIdx.y == 0) {
+  const int live = min(last, length);
+  if (p.state_out && at.chunk == 0) {
 #pragma unroll
     for (int j = 0; j < W - 1; ++j)
-      store_raw<T>(static_cast<T*>(p.state_out) + ((int64_t)b * (W - 1) + j) * p.channels + c0, count, p.vec & 4,
-                   value_at<T, W>(p, b, length - (W - 1) + j, c0, count));
+      value_at<T, W, V>(p, b, length - (W - 1) + j, c0)
+          .store(static_cast<T*>(p.state_out) + ((int64_t)b * (W - 1) + j) * p.channels + c0);
   }
-  float w[W][8], bias[8];
-  load_filter<T, W>(p, c0, count, w, bias);
-  float window[W][8];  // v[t - W + 1 .. t]
+  const T* x = static_cast<const T*>(p.x) + b * p.x_sb + first * p.x_st + c0;
+  T* y = static_cast<T*>(p.y) + ((int64_t)b * p.length + first) * p.channels + c0;
+  Rows<T, V> rows((uint32_t)__cvta_generic_to_shared(smem));
+#pragma unroll
+  for (int k = 0; k < kDepth; ++k) {
+    if (first + k < live) rows.issue(k, x + k * p.x_st);
+    cp_async_commit();
+  }
+  float w[W][V], bias[V];
+  load_filter<W, V>(p, c0, w, bias);
+  float window[W][V];  // v[t - W + 1 .. t]
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
     const int t = first - (W - 1) + j;
     if (t < length) {
-      unpack8<T>(value_at<T, W>(p, b, t, c0, count), window[j + 1]);
-    } else {
+      const Pack<T, V> r = value_at<T, W, V>(p, b, t, c0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) window[j + 1][i] = 0.0f;
+      for (int i = 0; i < V; ++i) window[j + 1][i] = r.get(i);
     }
   }
-  const int live = min(last, length);
-  constexpr int kAhead = 4;
   int t = first;
-  for (; t < live; t += kAhead) {
-    Raw8<T> raw[kAhead];
+  auto token = [&](const Pack<T, V>& raw) {
+    Pack<T, V> o;
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (t + k < live) raw[k] = value_at<T, W>(p, b, t + k, c0, count);
+    for (int i = 0; i < V; ++i) {
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (t + k < live) {
+      for (int j = 0; j < W - 1; ++j) window[j][i] = window[j + 1][i];
+      window[W - 1][i] = raw.get(i);
+      float v = bias[i];
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) window[j][i] = window[j + 1][i];
-        unpack8<T>(raw[k], window[W - 1]);
-        float o[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          o[i] = bias[i];
-#pragma unroll
-          for (int j = 0; j < W; ++j) o[i] = fmaf(w[j][i], window[j][i], o[i]);
-          if (p.silu) o[i] *= sigmoid(o[i]);
-        }
-        store8<T>(y + (int64_t)(t + k) * p.channels, count, p.vec & 4, o);
-      }
+      for (int j = 0; j < W; ++j) v = fmaf(w[j][i], window[j][i], v);
+      if (p.silu) v *= sigmoid(v);
+      o.set(i, v);
     }
+    o.store(y);
+    y += p.channels;
+  };
+  for (; t + kDepth <= live; t += kDepth) {
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k) {
+      cp_async_wait<kDepth - 1>();
+      token(rows.get(k));
+      if (t + k + kDepth < live) rows.issue(k, x + (k + kDepth) * p.x_st);
+      cp_async_commit();
+    }
+    x += kDepth * p.x_st;
   }
-  const float zero[8] = {};
-  for (t = max(first, live); t < last; ++t) store8<T>(y + (int64_t)t * p.channels, count, p.vec & 4, zero);
+  cp_async_wait<0>();
+#pragma unroll
+  for (int k = 0; k < kDepth; ++k)
+    if (t + k < live) token(rows.get(k));
+  t = live;
+  Pack<T, V> zero;
+  zero.zero();
+  for (t = max(first, live); t < last; ++t) {
+    zero.store(y);
+    y += p.channels;
+  }
 }
 
 // One token: the state is shifted in place.
-template <typename T, int W>
-__global__ void __launch_bounds__(128) causal_conv_step_kernel(Params p) {
-  const int vectors = (p.channels + 7) / 8;
-  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kThreads) causal_conv_step_kernel(const __grid_constant__ Params p) {
+  const int vectors = p.channels / V;
+  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (at >= (int64_t)p.batch * vectors) return;
   const int b = (int)(at / vectors);
-  const int c0 = (int)(at % vectors) * 8;
-  const int count = min(8, p.channels - c0);
+  const int c0 = (int)(at % vectors) * V;
   T* state = static_cast<T*>(p.state_out) + (int64_t)b * (W - 1) * p.channels + c0;
-  Raw8<T> window[W];
+  Pack<T, V> window[W];
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) {
-    // plain loads: the same thread writes these places below
-    float v[8];
+  for (int j = 0; j < W - 1; ++j) window[j].load(state + (int64_t)j * p.channels);
+  window[W - 1].load(static_cast<const T*>(p.x) + b * p.x_sb + c0);
+  float w[W][V], bias[V];
+  load_filter<W, V>(p, c0, w, bias);
+  Pack<T, V> o;
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) window[j].q[i] = make_uint4(0, 0, 0, 0);
-    if ((p.vec & 2) && count == 8) {
+  for (int i = 0; i < V; ++i) {
+    float v = bias[i];
 #pragma unroll
-      for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
-        window[j].q[i] = reinterpret_cast<const uint4*>(state + (int64_t)j * p.channels)[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < count) reinterpret_cast<T*>(&window[j])[i] = state[(int64_t)j * p.channels + i];
-    }
-    (void)v;
-  }
-  window[W - 1] = load8<T>(static_cast<const T*>(p.x) + b * p.x_sb + c0, count, p.vec & 1);
-  float w[W][8], o[8];
-  load_filter<T, W>(p, c0, count, w, o);
-#pragma unroll
-  for (int j = 0; j < W; ++j) {
-    float v[8];
-    unpack8<T>(window[j], v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = fmaf(w[j][i], v[i], o[i]);
-    if (j > 0) store8<T>(state + (int64_t)(j - 1) * p.channels, count, p.vec & 2, v);
+    for (int j = 0; j < W; ++j) v = fmaf(w[j][i], window[j].get(i), v);
+    if (p.silu) v *= sigmoid(v);
+    o.set(i, v);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (p.silu) o[i] *= sigmoid(o[i]);
-  store8<T>(static_cast<T*>(p.y) + (int64_t)b * p.channels + c0, count, p.vec & 4, o);
+  for (int j = 1; j < W; ++j) window[j].store(state + (int64_t)(j - 1) * p.channels);
+  o.store(static_cast<T*>(p.y) + (int64_t)b * p.channels + c0);
 }
 
 // Backward of a chunk of tokens: a thread walks t over [first, last + W - 1), keeps the W newest
 // v and the W newest dpre, and completes dx[t - W + 1] at t.  dw and dbias count dpre of the
 // chunk's own tokens only.
-template <typename T, int W>
-__global__ void __launch_bounds__(128) causal_conv_backward_kernel(Params p) {
-  const int c0 = (blockIdx.x * blockDim.x + threadIdx.x) * 8;
-  if (c0 >= p.channels) return;
-  const int count = min(8, p.channels - c0);
-  const int b = blockIdx.z;
-  const int first = blockIdx.y * p.chunk;
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kThreads) causal_conv_backward_kernel(const __grid_constant__ Params p) {
+  __shared__ __align__(16) uint8_t smem[std::max(16, 2 * Rows<T, V>::kBytes)];
+  const Place at = place<V>(p);
+  if (!at.in) return;
+  const int b = at.b, c0 = at.c0;
+  const int first = at.chunk * p.chunk;
   const int last = min(first + p.chunk, p.length);
   const int length = sequence_length(p.lengths, p.lengths64, b, p.length);
-  float w[W][8], bias[8];
-  load_filter<T, W>(p, c0, count, w, bias);
-  float window[W][8], dpre[W][8], dw[W][8], db[8];
+  const int live = min(last + W - 1, length);
+  float w[W][V], bias[V];
+  load_filter<W, V>(p, c0, w, bias);
+  float window[W][V], dpre[W][V], dw[W][V], db[V];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < V; ++i) {
     db[i] = 0.0f;
 #pragma unroll
     for (int j = 0; j < W; ++j) dw[j][i] = dpre[j][i] = window[j][i] = 0.0f;
@@ -201,74 +266,135 @@ __global__ void __launch_bounds__(128) causal_conv_backward_kernel(Params p) {
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
     const int t = first - (W - 1) + j;
-    if (t < length) unpack8<T>(value_at<T, W>(p, b, t, c0, count), window[j + 1]);
+    if (t < length) {
+      const Pack<T, V> r = value_at<T, W, V>(p, b, t, c0);
+#pragma unroll
+      for (int i = 0; i < V; ++i) window[j + 1][i] = r.get(i);
+    }
   }
-  const T* dy = static_cast<const T*>(p.dy) + b * p.dy_sb + c0;
-  T* dx = static_cast<T*>(p.dx) + (int64_t)b * p.length * p.channels + c0;
+  const T* x = static_cast<const T*>(p.x) + b * p.x_sb + first * p.x_st + c0;
+  const T* dy = static_cast<const T*>(p.dy) + b * p.dy_sb + first * p.dy_st + c0;
+  T* dx = static_cast<T*>(p.dx) + ((int64_t)b * p.length + first) * p.channels + c0;
   const T* ds = p.dstate_out ? static_cast<const T*>(p.dstate_out) + (int64_t)b * (W - 1) * p.channels + c0 : nullptr;
   // the first chunk also completes the gradients of the state, at negative t
-  T* dstate = p.dstate ? static_cast<T*>(p.dstate) + (int64_t)b * (W - 1) * p.channels + c0 : nullptr;
-  for (int t = first; t < last + W - 1; ++t) {
+  T* dstate = p.dstate && first == 0 ? static_cast<T*>(p.dstate) + (int64_t)b * (W - 1) * p.channels + c0 : nullptr;
+  Rows<T, V> rows_x((uint32_t)__cvta_generic_to_shared(smem));
+  Rows<T, V> rows_g((uint32_t)__cvta_generic_to_shared(smem) + Rows<T, V>::kBytes);
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j)
+  for (int k = 0; k < kDepth; ++k) {
+    if (first + k < live) {
+      rows_x.issue(k, x + k * p.x_st);
+      rows_g.issue(k, dy + k * p.dy_st);
+    }
+    cp_async_commit();
+  }
+  // shifts the windows to token t; is_live: it is inside its sequence, own: inside the chunk
+  auto take = [&](const Pack<T, V>& raw_x, const Pack<T, V>& raw_g, auto is_live, bool own) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) {
         window[j][i] = window[j + 1][i];
         dpre[j][i] = dpre[j + 1][i];
       }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) dpre[W - 1][i] = 0.0f;
-    if (t < length) {
-      float g[8];
-      unpack8<T>(value_at<T, W>(p, b, t, c0, count), window[W - 1]);
-      load8f<T>(dy + t * p.dy_st, count, p.vec & 8, g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      float g = 0.0f;
+      if (decltype(is_live)::value) {
+        window[W - 1][i] = raw_x.get(i);
+        g = raw_g.get(i);
         if (p.silu) {
           float pre = bias[i];
 #pragma unroll
           for (int j = 0; j < W; ++j) pre = fmaf(w[j][i], window[j][i], pre);
           const float s = sigmoid(pre);
-          g[i] *= s * (1.0f + pre * (1.0f - s));
+          g *= s * (1.0f + pre * (1.0f - s));
         }
-        dpre[W - 1][i] = g[i];
-        if (t < last) {
-          db[i] += g[i];
+        if (own) {
+          db[i] += g;
 #pragma unroll
-          for (int j = 0; j < W; ++j) dw[j][i] = fmaf(g[i], window[j][i], dw[j][i]);
+          for (int j = 0; j < W; ++j) dw[j][i] = fmaf(g, window[j][i], dw[j][i]);
         }
       }
+      dpre[W - 1][i] = g;
     }
-    const int at = t - (W - 1);  // complete: dpre holds [at, at + W - 1]
-    if (at < first && !(first == 0 && dstate)) continue;
-    float o[8];
+  };
+  // dv of the token W - 1 before the newest: dpre holds it and the W - 1 after it
+  auto gradient = [&](float (&o)[V]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < V; ++i) {
       o[i] = 0.0f;
 #pragma unroll
       for (int j = 0; j < W; ++j) o[i] = fmaf(w[W - 1 - j][i], dpre[j][i], o[i]);
     }
-    // entry `at` of [state, x[:length]] is also entry at - (length - W + 1) of the new state
-    const int kept = at - (length - (W - 1));
-    if (ds && kept >= 0 && kept < W - 1) {
-      float e[8];
-      load8f<T>(ds + (int64_t)kept * p.channels, count, p.vec & 16, e);
+  };
+  auto put = [&](T* at, const float (&o)[V]) {
+    Pack<T, V> r;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] += e[i];
-    }
-    if (at < 0)
-      store8<T>(dstate + (int64_t)(at + W - 1) * p.channels, count, p.vec & 16, o);
+    for (int i = 0; i < V; ++i) r.set(i, o[i]);
+    r.store(at);
+  };
+  // any token, and what becomes complete with it
+  auto careful = [&](int t, int k) {
+    if (t < live)
+      take(rows_x.get(k), rows_g.get(k), std::true_type{}, t < last);
     else
-      store8<T>(dx + (int64_t)at * p.channels, count, p.vec & 4, o);
-  }
-  float* out = p.partial + (((int64_t)b * gridDim.y + blockIdx.y) * p.channels + c0) * (W + 1);
+      take(Pack<T, V>(), Pack<T, V>(), std::false_type{}, false);
+    const int done = t - (W - 1);
+    if (done < first && !dstate) return;
+    float o[V];
+    gradient(o);
+    // entry `done` of [state, x[:length]] is also entry done - (length - W + 1) of the new state
+    const int kept = done - (length - (W - 1));
+    if (ds && kept >= 0 && kept < W - 1) {
+      Pack<T, V> e;
+      e.load(ds + (int64_t)kept * p.channels);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (i < count) {
-#pragma unroll
-      for (int j = 0; j < W; ++j) out[i * (W + 1) + j] = dw[j][i];
-      out[i * (W + 1) + W] = db[i];
+      for (int i = 0; i < V; ++i) o[i] += e.get(i);
     }
+    if (done < 0) {
+      put(dstate + (int64_t)(done + W - 1) * p.channels, o);
+    } else {
+      put(dx, o);
+      dx += p.channels;
+    }
+  };
+  int t0 = first;
+  const int plain = min(last, length - (W - 1));  // tokens before it are no part of the new state
+  for (; t0 < last + W - 1; t0 += kDepth) {
+    if (t0 >= first + W - 1 && t0 + kDepth <= plain) {
+#pragma unroll
+      for (int k = 0; k < kDepth; ++k) {
+        cp_async_wait<kDepth - 1>();
+        take(rows_x.get(k), rows_g.get(k), std::true_type{}, true);
+        float o[V];
+        gradient(o);
+        put(dx, o);
+        dx += p.channels;
+        if (t0 + k + kDepth < live) {
+          rows_x.issue(k, x + (k + kDepth) * p.x_st);
+          rows_g.issue(k, dy + (k + kDepth) * p.dy_st);
+        }
+        cp_async_commit();
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kDepth; ++k) {
+        cp_async_wait<kDepth - 1>();
+        if (t0 + k < last + W - 1) careful(t0 + k, k);
+        if (t0 + k + kDepth < live) {
+          rows_x.issue(k, x + (k + kDepth) * p.x_st);
+          rows_g.issue(k, dy + (k + kDepth) * p.dy_st);
+        }
+        cp_async_commit();
+      }
+    }
+    x += kDepth * p.x_st;
+    dy += kDepth * p.dy_st;
+  }
+  float* out = p.partial + ((int64_t)b * p.chunks + at.chunk) * (W + 1) * p.channels + c0;
+#pragma unroll
+  for (int j = 0; j <= W; ++j) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[(int64_t)j * p.channels + i] = j < W ? dw[j < W ? j : 0][i] : db[i];
   }
 }
 

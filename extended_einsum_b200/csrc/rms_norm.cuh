@@ -13,6 +13,8 @@
 // and written once.
 #pragma once
 
+#include <algorithm>
+
 #include "seq_common.cuh"
 
 namespace xe {
@@ -37,29 +39,64 @@ struct Params {
 
 // The widest block of a kernel that holds `groups` groups of eight elements per thread.
 template <int kGroups>
-constexpr int kMaxThreads = kGroups == 1 ? 1024 : kGroups <= 4 ? 512 : 1024;
+constexpr int kMaxThreads = kGroups == 1 ? 1024 : kGroups == 8 ? 1024 : 512;
+template <int kGroups>
+constexpr int kMaxBackwardThreads = kGroups == 8 ? 1024 : 512;
 
-// Sums (or maxima) over the threads of each row of the block: `wpr` warps per row.
-template <bool kMax>
-__device__ __forceinline__ float row_reduce(float v, int wpr, float* smem) {
+// Sums over the threads of each row of the block (`wpr` warps per row, at most 32 warps in all), and maxima
+// of values held as the bits of their sizes, among which a NaN is the largest: both with one barrier.
+// `turn` alternates the buffer: a thread that writes a buffer again has passed the barrier of the
+// reduction in between, which all readers of the buffer reach after reading.
+struct RowBuffers {
+  float sum[2][32];
+  uint32_t most[2][32];  // or second sums
+};
+
+__device__ __forceinline__ float warp_sum(float v, int from = 16) {
+  for (int o = from; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return __shfl_sync(0xffffffffu, v, 0);
+}
+__device__ __forceinline__ int first_step(int wpr) { return wpr > 16 ? 16 : wpr > 8 ? 8 : wpr > 4 ? 4 : wpr > 2 ? 2 : 1; }
+
+template <bool kMost>
+__device__ __forceinline__ void row_reduce(float& v, uint32_t& most, int wpr, RowBuffers& smem, int& turn) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (kMost) most = __reduce_max_sync(0xffffffffu, most);
+  if (wpr == 1) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) {
+    smem.sum[turn][warp] = v;
+    if (kMost) smem.most[turn][warp] = most;
+  }
+  __syncthreads();
+  const int at = warp / wpr * wpr + lane;
+  v = lane < wpr ? smem.sum[turn][at] : 0.0f;
+  if (kMost) most = __reduce_max_sync(0xffffffffu, lane < wpr ? smem.most[turn][at] : 0u);
+  turn ^= 1;
+  v = warp_sum(v, first_step(wpr));
+}
+
+// Two sums with one barrier.
+__device__ __forceinline__ void row_sums(float& v, float& u, int wpr, RowBuffers& smem, int& turn) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const float other = __shfl_xor_sync(0xffffffffu, v, o);
-    // a NaN wins the maximum
-    v = kMax ? ((other > v || other != other) ? other : v) : v + other;
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+    u += __shfl_xor_sync(0xffffffffu, u, o);
   }
-  if (wpr == 1) return v;
-  const int warp = threadIdx.x >> 5;
-  if ((threadIdx.x & 31) == 0) smem[warp] = v;
-  __syncthreads();
-  const int first = warp / wpr * wpr;
-  float r = smem[first];
-  for (int i = 1; i < wpr; ++i) {
-    const float other = smem[first + i];
-    r = kMax ? ((other > r || other != other) ? other : r) : r + other;
+  if (wpr == 1) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) {
+    smem.sum[turn][warp] = v;
+    smem.most[turn][warp] = __float_as_uint(u);
   }
   __syncthreads();
-  return r;
+  const int at = warp / wpr * wpr + lane;
+  v = lane < wpr ? smem.sum[turn][at] : 0.0f;
+  u = lane < wpr ? __uint_as_float(smem.most[turn][at]) : 0.0f;
+  turn ^= 1;
+  v = warp_sum(v, first_step(wpr));
+  u = warp_sum(u, first_step(wpr));
 }
 
 // Where a thread's element groups lie.  kVec: groups of 8 consecutive elements; otherwise the
@@ -69,23 +106,72 @@ __device__ __forceinline__ int element(int group, int i, int lane, int lanes) {
   return kVec ? (group * lanes + lane) * 8 + i : (group * 8 + i) * lanes + lane;
 }
 
+// One group as it lies in memory.
 template <typename T, bool kVec>
-__device__ __forceinline__ void load_group(const T* row, int g, int lane, int lanes, int columns, float (&v)[8]) {
-  if constexpr (kVec) {
-    const int at = element<true>(g, 0, lane, lanes);
-    if (at < columns) {
-      load8f<T>(row + at, 8, true, v);
+struct Group {
+  Raw8<T> raw;
+
+  __device__ __forceinline__ void load(const T* row, int g, int lane, int lanes, int columns) {
+    if constexpr (kVec) {
+      const int at = element<true>(g, 0, lane, lanes);
+      raw = load8<T>(row + at, at < columns ? 8 : 0, true);
     } else {
+      T* e = reinterpret_cast<T*>(&raw);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int at = element<false>(g, i, lane, lanes);
-      v[i] = at < columns ? to_f32(row[at]) : 0.0f;
+      for (int i = 0; i < 8; ++i) {
+        const int at = element<false>(g, i, lane, lanes);
+        e[i] = at < columns ? row[at] : from_f32<T>(0.0f);
+      }
     }
   }
+  __device__ __forceinline__ void get(float (&v)[8]) const { unpack8<T>(raw, v); }
+};
+
+// Rows on their way: kStages of them, a thread's groups of kTensors tensors in shared memory places of its
+// own (so that no barrier is needed), filled by cp.async.  A place is 16 bytes per thread; consecutive
+// threads' places are adjacent.  As many as fit for the widest block, at most four.
+template <int kGroups>
+constexpr bool kRing = kGroups <= 2;
+constexpr int ring_stages(int threads, int bytes) { return std::min(4, 196608 / (threads * bytes)); }
+template <typename T, typename R, int kGroups>
+constexpr int kForwardBytes = kGroups * 8 * (sizeof(T) + sizeof(R));  // of a stage, per thread
+template <typename T, typename R, int kGroups>
+constexpr int kBackwardBytes = kGroups * 16 * (sizeof(T) + sizeof(R));
+template <typename T, typename R, int kGroups>
+constexpr int kForwardStages = kRing<kGroups> ? ring_stages(kMaxThreads<kGroups>, kForwardBytes<T, R, kGroups>) : 0;
+template <typename T, typename R, int kGroups>
+constexpr int kBackwardStages = kRing<kGroups> ? ring_stages(kMaxBackwardThreads<kGroups>, kBackwardBytes<T, R, kGroups>) : 0;
+
+__device__ __forceinline__ uint32_t ring_place(uint32_t base, int index) {
+  return base + (index * blockDim.x + threadIdx.x) * 16;
+}
+template <typename T>
+__device__ __forceinline__ void ring_load(uint32_t base, int index, const T* row, int g, int lane, int lanes, int columns) {
+  const int at = element<true>(g, 0, lane, lanes);
+  if (at < columns) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
+      cp_async16(ring_place(base, index + i), reinterpret_cast<const uint4*>(row + at) + i);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void ring_get(uint32_t base, int index, bool in, float (&v)[8]) {
+  Raw8<T> raw;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 2); ++i) {
+    uint4 q = make_uint4(0, 0, 0, 0);
+    if (in)
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(ring_place(base, index + i)));
+    raw.q[i] = q;
+  }
+  unpack8<T>(raw, v);
+}
+
+template <typename T, bool kVec>
+__device__ __forceinline__ void load_group(const T* row, int g, int lane, int lanes, int columns, float (&v)[8]) {
+  Group<T, kVec> q;
+  q.load(row, g, lane, lanes, columns);
+  q.get(v);
 }
 
 template <typename T, bool kVec>
@@ -102,97 +188,146 @@ __device__ __forceinline__ void store_group(T* row, int g, int lane, int lanes, 
   }
 }
 
+// Weights are read by every row's threads: plain loads, which the L1 cache keeps.
 template <typename T, bool kVec>
-__device__ __forceinline__ void load_weight(const Params& p, int g, int lane, int lanes, float (&w)[8]) {
-  if (!p.weight) {
+__device__ __forceinline__ void load_weight(const void* weight, int weight_f32, int columns, int g, int lane, int lanes,
+                                            float (&w)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = 1.0f;
-  } else if (p.weight_f32) {
-    load_group<float, kVec>(static_cast<const float*>(p.weight), g, lane, lanes, p.columns, w);
-  } else {
-    load_group<T, kVec>(static_cast<const T*>(p.weight), g, lane, lanes, p.columns, w);
+  for (int i = 0; i < 8; ++i) {
+    const int at = element<kVec>(g, i, lane, lanes);
+    w[i] = 1.0f;
+    if (weight && at < columns)
+      w[i] = weight_f32 ? static_cast<const float*>(weight)[at] : to_f32(static_cast<const T*>(weight)[at]);
   }
 }
 
-__device__ __forceinline__ uint32_t code8(float v, int quantize) {
-  if (quantize == XE_E4M3) return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
-  return (uint32_t)(uint8_t)(int8_t)max(-127, min(127, __float2int_rn(v)));
+// Two codes in the low 16 bits.
+__device__ __forceinline__ uint32_t codes8(float a, float b, int quantize) {
+  if (quantize == XE_E4M3) return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const int i = max(-127, min(127, __float2int_rn(a))), j = max(-127, min(127, __float2int_rn(b)));
+  return (uint32_t)(i & 255) | (uint32_t)(j & 255) << 8;
 }
 
-// A block handles blockDim.x / 32 / wpr rows, `wpr` warps on each; a thread holds kGroups groups of
-// eight elements.
+// `wpr` warps on each row, blockDim.x / 32 / wpr rows at a time, the blocks persistent over the rows; a
+// thread holds kGroups groups of eight elements.  Rows to come are loaded ahead (aligned ones through the
+// ring), since the reductions' barriers would otherwise leave the memory idle.
 template <typename T, typename R, int kGroups, bool kVec>
-__global__ void __launch_bounds__(kMaxThreads<kGroups>) rms_norm_kernel(Params p, int wpr) {
-  __shared__ float smem[32];
+__global__ void __launch_bounds__(kMaxThreads<kGroups>, 1) rms_norm_kernel(const __grid_constant__ Params p, int wpr) {
+  constexpr bool kKeep = kGroups <= 2;  // weights stay in registers
+  constexpr bool kRinged = kVec && kRing<kGroups>;
+  constexpr int kStages = std::max(1, kForwardStages<T, R, kGroups>);
+  constexpr int kPlaces = kGroups * (sizeof(T) + sizeof(R)) / 2;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ RowBuffers smem;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const uint32_t stage_bytes = kPlaces * blockDim.x * 16;
+  int turn = 0;
   const int lanes = wpr * 32;
   const int lane = threadIdx.x % lanes;
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes;
-  const bool live = row < p.rows;
-  const int columns = live ? p.columns : 0;
-  const T* x = static_cast<const T*>(p.x) + (live ? row : 0) * p.x_row;
-  float v[kGroups][8];
+  const int slots = blockDim.x / lanes;
+  const int64_t stride = (int64_t)gridDim.x * slots;
+  int64_t row = (int64_t)blockIdx.x * slots + threadIdx.x / lanes;
+  auto issue = [&](int64_t at, int stage) {
+    if (at < p.rows) {
+      const T* x = static_cast<const T*>(p.x) + at * p.x_row;
+      const R* r = static_cast<const R*>(p.residual) + at * p.r_row;
+      const uint32_t base = ring_at + stage * stage_bytes;
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) load_group<T, kVec>(x, g, lane, lanes, columns, v[g]);
-  if (p.residual) {
-    const R* r = static_cast<const R*>(p.residual) + (live ? row : 0) * p.r_row;
-    R* sum = static_cast<R*>(p.sum) + (live ? row : 0) * p.columns;
+      for (int g = 0; g < kGroups; ++g) {
+        ring_load<T>(base, g * (sizeof(T) / 2), x, g, lane, lanes, p.columns);
+        if (p.residual)
+          ring_load<R>(base, kGroups * (sizeof(T) / 2) + g * (sizeof(R) / 2), r, g, lane, lanes, p.columns);
+      }
+    }
+    cp_async_commit();
+  };
+  if (kRinged) {
+#pragma unroll
+    for (int k = 0; k < kStages - 1; ++k) issue(row + k * stride, k);
+  }
+  float w[kKeep ? kGroups : 1][8];
+  if (kKeep) {
+#pragma unroll
+    for (int g = 0; g < (kKeep ? kGroups : 1); ++g)
+      load_weight<T, kVec>(p.weight, p.weight_f32, p.columns, g, lane, lanes, w[g]);
+  }
+  int stage = 0;
+  // all slots of a block take the same number of turns: the reductions are block-wide barriers
+  for (int64_t base = (int64_t)blockIdx.x * slots; base < p.rows; base += stride, row += stride) {
+    const int columns = row < p.rows ? p.columns : 0;
+    const int64_t out = (columns ? row : 0) * p.columns;
+    float v[kGroups][8];
+    float total = 0.0f;
+    if (kRinged) {
+      issue(row + (kStages - 1) * stride, (stage + kStages - 1) % kStages);
+      cp_async_wait<kStages - 1>();
+    }
+    const uint32_t at = ring_at + stage * stage_bytes;
+    stage = (stage + 1) % kStages;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      float a[8];
-      load_group<R, kVec>(r, g, lane, lanes, columns, a);
+      const bool in = element<kVec>(g, 0, lane, lanes) < columns;
+      if (kRinged)
+        ring_get<T>(at, g * (sizeof(T) / 2), in, v[g]);
+      else
+        load_group<T, kVec>(static_cast<const T*>(p.x) + (columns ? row : 0) * p.x_row, g, lane, lanes, columns, v[g]);
+      if (p.residual) {
+        float a[8];
+        if (kRinged)
+          ring_get<R>(at, kGroups * (sizeof(T) / 2) + g * (sizeof(R) / 2), in, a);
+        else
+          load_group<R, kVec>(static_cast<const R*>(p.residual) + (columns ? row : 0) * p.r_row, g, lane, lanes, columns, a);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[g][i] += a[i];
-      store_group<R, kVec>(sum, g, lane, lanes, columns, v[g]);
+        for (int i = 0; i < 8; ++i) v[g][i] += a[i];
+        store_group<R, kVec>(static_cast<R*>(p.sum) + out, g, lane, lanes, columns, v[g]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) total = fmaf(v[g][i], v[g][i], total);
     }
-  }
-  float total = 0.0f;
+    // max |y| = rstd max |s w|, so that one reduction serves both statistics
+    uint32_t most = 0;
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) total = fmaf(v[g][i], v[g][i], total);
-  total = row_reduce<false>(total, wpr, smem);
-  const float rstd = rsqrtf(total / (float)p.columns + p.eps);
-  float most = 0.0f;
-#pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    float w[8];
-    load_weight<T, kVec>(p, g, lane, lanes, w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool in = element<kVec>(g, i, lane, lanes) < columns;
-      v[g][i] = v[g][i] * rstd * w[i];
-      const float m = fabsf(v[g][i]);
-      if (in && (m > most || m != m)) most = m;
-    }
-  }
-  if (p.quantize == 0) {
-    T* y = static_cast<T*>(p.y) + (live ? row : 0) * p.columns;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) store_group<T, kVec>(y, g, lane, lanes, columns, v[g]);
-    return;
-  }
-  most = row_reduce<true>(most, wpr, smem);
-  const float limit = p.quantize == XE_E4M3 ? 448.0f : 127.0f;
-  float scale = most / limit;
-  if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;  // a NaN stays
-  if (live && lane == 0) p.scale[row] = scale;
-  const float inverse = 1.0f / scale;
-  uint8_t* q = static_cast<uint8_t*>(p.y) + (live ? row : 0) * p.columns;
-#pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    uint32_t c[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = code8(v[g][i] * inverse, p.quantize);
-    if constexpr (kVec) {
-      const int at = element<true>(g, 0, lane, lanes);
-      if (at < columns)
-        *reinterpret_cast<uint2*>(q + at) = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24,
-                                                       c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
-    } else {
+    for (int g = 0; g < kGroups; ++g) {
+      if (!kKeep) load_weight<T, kVec>(p.weight, p.weight_f32, p.columns, g, lane, lanes, w[0]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int at = element<false>(g, i, lane, lanes);
-        if (at < columns) q[at] = (uint8_t)c[i];
+        v[g][i] *= w[kKeep ? g : 0][i];
+        most = max(most, __float_as_uint(fabsf(v[g][i])));
+      }
+    }
+    if (p.quantize)
+      row_reduce<true>(total, most, wpr, smem, turn);
+    else
+      row_reduce<false>(total, most, wpr, smem, turn);
+    const float rstd = rsqrtf(total / (float)p.columns + p.eps);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[g][i] *= rstd;
+    if (p.quantize == 0) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) store_group<T, kVec>(static_cast<T*>(p.y) + out, g, lane, lanes, columns, v[g]);
+      continue;
+    }
+    float scale = __uint_as_float(most) * rstd / (p.quantize == XE_E4M3 ? 448.0f : 127.0f);
+    if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;  // a NaN stays
+    if (columns && lane == 0) p.scale[row] = scale;
+    const float inverse = 1.0f / scale;
+    uint8_t* q = static_cast<uint8_t*>(p.y) + out;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      uint32_t c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = codes8(v[g][2 * i] * inverse, v[g][2 * i + 1] * inverse, p.quantize);
+      if constexpr (kVec) {
+        const int at = element<true>(g, 0, lane, lanes);
+        if (at < columns) *reinterpret_cast<uint2*>(q + at) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int at = element<false>(g, i, lane, lanes);
+          if (at < columns) q[at] = (uint8_t)(c[i / 2] >> (8 * (i % 2)));
+        }
       }
     }
   }
@@ -213,69 +348,123 @@ struct BackwardParams {
   int weight_f32;
 };
 
-// Persistent blocks over rows; each block (wpr warps on a row at a time) keeps its dw sums in
-// registers and writes them once, and rms_norm_dweight adds the blocks in a fixed order.
+// Persistent blocks over the rows as above; each slot keeps its dw sums in registers and writes them once,
+// and sum_rows adds them in a fixed order.
 template <typename T, typename R, int kGroups, bool kVec>
-__global__ void __launch_bounds__(kMaxThreads<kGroups>) rms_norm_backward_kernel(BackwardParams p, int wpr) {
-  __shared__ float smem[32];
+__global__ void __launch_bounds__(kMaxBackwardThreads<kGroups>, 1)
+    rms_norm_backward_kernel(const __grid_constant__ BackwardParams p, int wpr) {
+  constexpr bool kKeep = kGroups <= 2;
+  constexpr bool kRinged = kVec && kRing<kGroups>;
+  constexpr int kStages = std::max(1, kBackwardStages<T, R, kGroups>);
+  constexpr int kR = sizeof(R) / 2, kT = sizeof(T) / 2;
+  constexpr int kPlaces = kGroups * (2 * kR + 2 * kT);  // sum, dsum, dy, addend
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ RowBuffers smem;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const uint32_t stage_bytes = kPlaces * blockDim.x * 16;
+  int turn = 0;
   const int lanes = wpr * 32;
   const int lane = threadIdx.x % lanes;
   const int slots = blockDim.x / lanes;
   const int slot = threadIdx.x / lanes;
-  Params wp{};
-  wp.weight = p.weight;
-  wp.weight_f32 = p.weight_f32;
-  wp.columns = p.columns;
-  float dw[kGroups][8];
+  const int64_t stride = (int64_t)gridDim.x * slots;
+  int64_t row = (int64_t)blockIdx.x * slots + slot;
+  auto issue = [&](int64_t at, int stage) {
+    if (at < p.rows) {
+      const uint32_t base = ring_at + stage * stage_bytes;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const int place = g * (2 * kR + 2 * kT);
+        ring_load<R>(base, place, static_cast<const R*>(p.sum) + at * p.s_row, g, lane, lanes, p.columns);
+        if (p.dsum)
+          ring_load<R>(base, place + kR, static_cast<const R*>(p.dsum) + at * p.dsum_row, g, lane, lanes, p.columns);
+        ring_load<T>(base, place + 2 * kR, static_cast<const T*>(p.dy) + at * p.dy_row, g, lane, lanes, p.columns);
+        if (p.addend)
+          ring_load<T>(base, place + 2 * kR + kT, static_cast<const T*>(p.addend) + at * p.a_row, g, lane, lanes, p.columns);
+      }
+    }
+    cp_async_commit();
+  };
+  if (kRinged) {
+#pragma unroll
+    for (int k = 0; k < kStages - 1; ++k) issue(row + k * stride, k);
+  }
+  float dw[kGroups][8], w[kKeep ? kGroups : 1][8];
 #pragma unroll
   for (int g = 0; g < kGroups; ++g)
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[g][i] = 0.0f;
-  // every slot of a block takes the same number of turns: the reductions are block-wide barriers
-  const int64_t stride = (int64_t)gridDim.x * slots;
-  for (int64_t base = (int64_t)blockIdx.x * slots; base < p.rows; base += stride) {
-    const int64_t row = base + slot;
-    const bool live = row < p.rows;
-    const int columns = live ? p.columns : 0;
-    const int64_t at = live ? row : 0;
+  if (kKeep) {
+#pragma unroll
+    for (int g = 0; g < (kKeep ? kGroups : 1); ++g)
+      load_weight<T, kVec>(p.weight, p.weight_f32, p.columns, g, lane, lanes, w[g]);
+  }
+  int stage = 0;
+  for (int64_t base = (int64_t)blockIdx.x * slots; base < p.rows; base += stride, row += stride) {
+    const int columns = row < p.rows ? p.columns : 0;
+    const int64_t at = columns ? row : 0;
     float s[kGroups][8], du[kGroups][8];
     float square = 0.0f;
+    if (kRinged) {
+      issue(row + (kStages - 1) * stride, (stage + kStages - 1) % kStages);
+      cp_async_wait<kStages - 1>();
+    }
+    const uint32_t ring_stage = ring_at + stage * stage_bytes;
+    stage = (stage + 1) % kStages;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      load_group<R, kVec>(static_cast<const R*>(p.sum) + at * p.s_row, g, lane, lanes, columns, s[g]);
-      load_group<T, kVec>(static_cast<const T*>(p.dy) + at * p.dy_row, g, lane, lanes, columns, du[g]);
+      const bool in = element<kVec>(g, 0, lane, lanes) < columns;
+      const int place = g * (2 * kR + 2 * kT);
+      if (kRinged) {
+        ring_get<R>(ring_stage, place, in, s[g]);
+        ring_get<T>(ring_stage, place + 2 * kR, in, du[g]);
+      } else {
+        load_group<R, kVec>(static_cast<const R*>(p.sum) + at * p.s_row, g, lane, lanes, columns, s[g]);
+        load_group<T, kVec>(static_cast<const T*>(p.dy) + at * p.dy_row, g, lane, lanes, columns, du[g]);
+      }
       if (p.addend) {
         float a[8];
-        load_group<T, kVec>(static_cast<const T*>(p.addend) + at * p.a_row, g, lane, lanes, columns, a);
+        if (kRinged)
+          ring_get<T>(ring_stage, place + 2 * kR + kT, in, a);
+        else
+          load_group<T, kVec>(static_cast<const T*>(p.addend) + at * p.a_row, g, lane, lanes, columns, a);
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[g][i] += a[i];
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) square = fmaf(s[g][i], s[g][i], square);
     }
-    const float rstd = rsqrtf(row_reduce<false>(square, wpr, smem) / (float)p.columns + p.eps);
+    // sum du u = rstd sum dy w s, so that one reduction serves both sums
     float dot = 0.0f;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      float w[8];
-      load_weight<T, kVec>(wp, g, lane, lanes, w);
+      if (!kKeep) load_weight<T, kVec>(p.weight, p.weight_f32, p.columns, g, lane, lanes, w[0]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot = fmaf(du[g][i] * w[kKeep ? g : 0][i], s[g][i], dot);
+    }
+    row_sums(square, dot, wpr, smem, turn);
+    const float rstd = rsqrtf(square / (float)p.columns + p.eps);
+    dot = dot * rstd / (float)p.columns;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      if (!kKeep) load_weight<T, kVec>(p.weight, p.weight_f32, p.columns, g, lane, lanes, w[0]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         s[g][i] *= rstd;
         dw[g][i] = fmaf(du[g][i], s[g][i], dw[g][i]);
-        du[g][i] *= w[i];
-        dot = fmaf(du[g][i], s[g][i], dot);
+        du[g][i] *= w[kKeep ? g : 0][i];
       }
     }
-    dot = row_reduce<false>(dot, wpr, smem) / (float)p.columns;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       float o[8];
-      if (p.dsum) {
-        load_group<R, kVec>(static_cast<const R*>(p.dsum) + at * p.dsum_row, g, lane, lanes, columns, o);
-      } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = 0.0f;
+      for (int i = 0; i < 8; ++i) o[i] = 0.0f;
+      if (p.dsum) {
+        if (kRinged)
+          ring_get<R>(ring_stage, g * (2 * kR + 2 * kT) + kR, element<kVec>(g, 0, lane, lanes) < columns, o);
+        else
+          load_group<R, kVec>(static_cast<const R*>(p.dsum) + at * p.dsum_row, g, lane, lanes, columns, o);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = fmaf(rstd, du[g][i] - s[g][i] * dot, o[i]);
@@ -293,22 +482,24 @@ __global__ void __launch_bounds__(kMaxThreads<kGroups>) rms_norm_backward_kernel
 
 namespace seq {
 
-// out[j] = sum over i of partial[i, j], in the order of i within each of 8 interleaved threads and
-// then of the threads: 32 columns to a block of 32 x 8 threads.
-__global__ void __launch_bounds__(256) sum_rows_kernel(const float* partial, int64_t rows, int64_t columns, float* out) {
-  __shared__ float s[8][33];
+// out[j] = sum over i of partial[i, j]: 32 columns to a block, each of 32 threads adds every 32nd row, and
+// then the threads' sums are added as a tree.
+__global__ void __launch_bounds__(1024) sum_rows_kernel(const float* partial, int64_t rows, int64_t columns, float* out) {
+  __shared__ float s[32][33];
   const int64_t j = (int64_t)blockIdx.x * 32 + threadIdx.x;
   float acc = 0.0f;
-  if (j < columns)
-    for (int64_t i = threadIdx.y; i < rows; i += 8) acc += partial[i * columns + j];
+  if (j < columns) {
+#pragma unroll 4
+    for (int64_t i = threadIdx.y; i < rows; i += 32) acc += partial[i * columns + j];
+  }
   s[threadIdx.y][threadIdx.x] = acc;
   __syncthreads();
-  if (threadIdx.y == 0 && j < columns) {
-    float t = s[0][threadIdx.x];
+  // warp y sums column y
+  float t = s[threadIdx.x][threadIdx.y];
 #pragma unroll
-    for (int k = 1; k < 8; ++k) t += s[k][threadIdx.x];
-    out[j] = t;
-  }
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  const int64_t column = (int64_t)blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && column < columns) out[column] = t;
 }
 
 }  // namespace seq

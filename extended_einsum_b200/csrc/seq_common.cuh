@@ -131,6 +131,16 @@ __device__ __forceinline__ void store8(T* p, int count, bool vec, const float (&
     if (i < count) p[i] = from_f32<T>(v[i]);
 }
 
+// Copies of 16 bytes into shared memory, awaited by the thread that issued them.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // 2^x and 1/x of the special function unit: relative errors of 2^-22 and 2^-23.
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;

@@ -29,13 +29,14 @@ inline size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 inline bool is_float(int32_t dtype) { return dtype == XE_F32 || dtype == XE_BF16 || dtype == XE_F16; }
 inline int64_t size_of(int32_t dtype) { return dtype == XE_F32 ? 4 : dtype == XE_BF16 || dtype == XE_F16 ? 2 : 1; }
 
-// Whether rows of eight elements start on 16-byte boundaries everywhere.
-bool vectors(const void* p, int32_t dtype, std::initializer_list<int64_t> strides) {
-  if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+// Whether every row starts on a multiple of `bytes`.
+bool aligned(int64_t bytes, const void* p, int32_t dtype, std::initializer_list<int64_t> strides) {
+  if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
   for (int64_t s : strides)
-    if (s * size_of(dtype) % 16) return false;
+    if (s * size_of(dtype) % bytes) return false;
   return true;
 }
+bool vectors(const void* p, int32_t dtype, std::initializer_list<int64_t> strides) { return aligned(16, p, dtype, strides); }
 
 template <typename F>
 void by_type(int32_t dtype, F f) {
@@ -48,7 +49,7 @@ void by_type(int32_t dtype, F f) {
 }
 
 xe_status sum_rows(const float* partial, int64_t rows, int64_t columns, float* out, cudaStream_t stream) {
-  xe::seq::sum_rows_kernel<<<(unsigned)ceil_div(columns, 32), dim3(32, 8), 0, stream>>>(partial, rows, columns, out);
+  xe::seq::sum_rows_kernel<<<(unsigned)ceil_div(columns, 32), dim3(32, 32), 0, stream>>>(partial, rows, columns, out);
   return launched("sum_rows");
 }
 
@@ -79,13 +80,43 @@ void by_width(int64_t width, F f) {
   }
 }
 
-// Tokens of one thread: enough chunks to fill the device, few enough that the W - 1 rows read again
-// stay a small part.
-int64_t conv_chunk(int64_t batch, int64_t length, int64_t channels) {
-  const int64_t threads = batch * ceil_div(channels, 8);
-  int64_t chunk = 128;
-  while (chunk > 8 && threads * ceil_div(length, chunk) < 148 * 1024) chunk /= 2;
-  return std::max<int64_t>(chunk, ceil_div(length, 65535));
+// Four channels per thread where every row allows it, else one.
+bool fours(const void* p, int32_t dtype, std::initializer_list<int64_t> strides) {
+  return aligned(4 * size_of(dtype), p, dtype, strides);
+}
+template <typename F>
+void by_vector(int32_t dtype, bool vec, F f) {
+  by_type(dtype, [&](auto t) {
+    if (vec)
+      f(t, std::integral_constant<int, 4>{});
+    else
+      f(t, std::integral_constant<int, 1>{});
+  });
+}
+
+// How the length is cut into chunks.  A chunk reads width - 1 rows twice, so there are only as many
+// as fill the device's resident threads (`resident` an SM at the kernel's registers) a whole number of times, of at
+// most 256 tokens.  The backward pass is planned for vectors of four whatever the alignment, so that its
+// workspace depends on the sizes alone.
+struct ConvPlan {
+  int64_t chunk, chunks;
+};
+constexpr int64_t kConvResident = 896, kConvBackwardResident = 512;
+ConvPlan conv_plan(int64_t batch, int64_t length, int64_t vectors, int64_t resident) {
+  if (length < 1) return {1, 1};
+  const int64_t rows = std::max<int64_t>(1, batch * vectors), device = 148 * resident;
+  const int64_t turns = std::max<int64_t>(1, ceil_div(rows * ceil_div(length, 256), device));
+  int64_t chunks = std::max<int64_t>(1, std::min<int64_t>(turns * device / rows, ceil_div(length, 8)));
+  const int64_t chunk = ceil_div(length, chunks);
+  return {chunk, ceil_div(length, chunk)};
+}
+
+template <typename F>
+xe_status launch_conv(const char* what, const xe::conv::Params& p, int V, F kernel, cudaStream_t stream) {
+  const int64_t blocks = ceil_div((int64_t)(p.channels / V) * p.chunks, xe::conv::kThreads);
+  if (blocks > INT_MAX) return fail(XE_ERR_NOT_SUPPORTED, "%s: a size is above its limit", what);
+  kernel<<<dim3((unsigned)blocks, (unsigned)p.batch), xe::conv::kThreads, 0, stream>>>(p);
+  return launched(what);
 }
 
 }  // namespace
@@ -96,56 +127,56 @@ xe_status xe_causal_conv1d(const void* x, int64_t x_sb, int64_t x_st, const floa
                            const void* state, void* y, void* state_out, const void* lengths, int32_t lengths64,
                            int64_t batch, int64_t length, int64_t channels, int64_t width, int32_t activation,
                            int32_t dtype, void* stream) {
-  if (xe_status s = check_conv("xe_causal_conv1d", x, weight, y, batch, length, channels, width, activation, dtype)) return s;
+  const char* what = "xe_causal_conv1d";
+  if (xe_status s = check_conv(what, x, weight, y, batch, length, channels, width, activation, dtype)) return s;
   if (batch == 0 || channels == 0) return XE_OK;
   xe::conv::Params p{};
   p.x = x, p.weight = weight, p.bias = bias, p.state = state, p.y = y, p.state_out = state_out;
   p.lengths = lengths, p.lengths64 = lengths64;
   p.x_sb = x_sb, p.x_st = x_st;
   p.batch = (int)batch, p.length = (int)length, p.channels = (int)channels;
-  p.chunk = (int)conv_chunk(batch, length, channels);
   p.silu = activation;
-  p.vec = (vectors(x, dtype, {x_sb, x_st}) ? 1 : 0) | (vectors(state, dtype, {channels}) ? 2 : 0) |
-          (vectors(y, dtype, {channels}) && vectors(state_out, dtype, {}) ? 4 : 0);
-  const dim3 grid((unsigned)ceil_div(channels, 8 * 128), (unsigned)std::max<int64_t>(1, ceil_div(length, p.chunk)),
-                  (unsigned)batch);
-  by_type(dtype, [&](auto t) {
+  const bool vec = fours(x, dtype, {x_sb, x_st}) && fours(y, dtype, {channels}) && fours(state, dtype, {}) &&
+                   fours(state_out, dtype, {});
+  xe_status status = XE_OK;
+  by_vector(dtype, vec, [&](auto t, auto v) {
+    constexpr int V = decltype(v)::value;
+    const ConvPlan plan = conv_plan(batch, length, channels / V, kConvResident);
+    p.chunk = (int)plan.chunk, p.chunks = (int)plan.chunks;
     by_width(width, [&](auto w) {
-      xe::conv::causal_conv_kernel<decltype(t), decltype(w)::value><<<grid, 128, 0, as_stream(stream)>>>(p);
+      status = launch_conv(what, p, V, xe::conv::causal_conv_kernel<decltype(t), decltype(w)::value, V>, as_stream(stream));
     });
   });
-  return launched("xe_causal_conv1d");
+  return status;
 }
 
 xe_status xe_causal_conv1d_step(const void* x, int64_t x_sb, const float* weight, const float* bias, void* state, void* y,
                                 int64_t batch, int64_t channels, int64_t width, int32_t activation, int32_t dtype,
                                 void* stream) {
-  if (xe_status s = check_conv("xe_causal_conv1d_step", x, weight, y, batch > 65535 ? 1 : batch, 1, channels, width,
-                               activation, dtype))
-    return s;
-  if (width > 1 && batch * channels != 0 && !state)
-    return fail(XE_ERR_INVALID_ARGUMENT, "xe_causal_conv1d_step: null state");
-  if (batch < 0 || batch > INT_MAX / 2) return fail(XE_ERR_NOT_SUPPORTED, "xe_causal_conv1d_step: batch out of range");
+  const char* what = "xe_causal_conv1d_step";
+  if (xe_status s = check_conv(what, x, weight, y, batch > 65535 ? 1 : batch, 1, channels, width, activation, dtype)) return s;
+  if (width > 1 && batch * channels != 0 && !state) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null state", what);
+  if (batch > INT_MAX / 2) return fail(XE_ERR_NOT_SUPPORTED, "%s: a size is above its limit", what);
   if (batch == 0 || channels == 0) return XE_OK;
   xe::conv::Params p{};
   p.x = x, p.weight = weight, p.bias = bias, p.y = y, p.state_out = state;
   p.x_sb = x_sb;
   p.batch = (int)batch, p.channels = (int)channels, p.silu = activation;
-  p.vec = (vectors(x, dtype, {x_sb}) ? 1 : 0) | (vectors(state, dtype, {channels}) ? 2 : 0) |
-          (vectors(y, dtype, {channels}) ? 4 : 0);
-  const unsigned grid = (unsigned)ceil_div(batch * ceil_div(channels, 8), 128);
-  by_type(dtype, [&](auto t) {
+  const bool vec = fours(x, dtype, {x_sb}) && fours(y, dtype, {channels}) && fours(state, dtype, {});
+  by_vector(dtype, vec, [&](auto t, auto v) {
+    constexpr int V = decltype(v)::value;
+    const unsigned grid = (unsigned)ceil_div(batch * (channels / V), xe::conv::kThreads);
     by_width(width, [&](auto w) {
-      xe::conv::causal_conv_step_kernel<decltype(t), decltype(w)::value><<<grid, 128, 0, as_stream(stream)>>>(p);
+      xe::conv::causal_conv_step_kernel<decltype(t), decltype(w)::value, V>
+          <<<grid, xe::conv::kThreads, 0, as_stream(stream)>>>(p);
     });
   });
-  return launched("xe_causal_conv1d_step");
+  return launched(what);
 }
 
 size_t xe_causal_conv1d_backward_workspace_size(int64_t batch, int64_t length, int64_t channels, int64_t width) {
   if (batch <= 0 || length < 0 || channels <= 0 || width < 1 || width > 4) return 0;
-  const int64_t chunks = std::max<int64_t>(1, ceil_div(length, conv_chunk(batch, length, channels)));
-  return padded((size_t)(batch * chunks * channels * (width + 1)) * 4);
+  return padded((size_t)(batch * conv_plan(batch, length, ceil_div(channels, 4), kConvBackwardResident).chunks * channels * (width + 1)) * 4);
 }
 
 xe_status xe_causal_conv1d_backward(const void* x, int64_t x_sb, int64_t x_st, const float* weight, const float* bias,
@@ -168,20 +199,21 @@ xe_status xe_causal_conv1d_backward(const void* x, int64_t x_sb, int64_t x_st, c
   p.lengths = lengths, p.lengths64 = lengths64;
   p.x_sb = x_sb, p.x_st = x_st;
   p.batch = (int)batch, p.length = (int)length, p.channels = (int)channels;
-  p.chunk = (int)conv_chunk(batch, length, channels);
   p.silu = activation;
-  p.vec = (vectors(x, dtype, {x_sb, x_st}) ? 1 : 0) | (vectors(state, dtype, {channels}) ? 2 : 0) |
-          (vectors(dx, dtype, {channels}) ? 4 : 0) | (vectors(dy, dtype, {dy_sb, dy_st}) ? 8 : 0) |
-          (vectors(dstate_out, dtype, {channels}) && vectors(dstate, dtype, {}) ? 16 : 0);
-  const int64_t chunks = std::max<int64_t>(1, ceil_div(length, p.chunk));
-  const dim3 grid((unsigned)ceil_div(channels, 8 * 128), (unsigned)chunks, (unsigned)batch);
-  by_type(dtype, [&](auto t) {
+  const bool vec = fours(x, dtype, {x_sb, x_st}) && fours(dx, dtype, {channels}) && fours(state, dtype, {}) &&
+                   fours(dy, dtype, {dy_sb, dy_st}) && fours(dstate_out, dtype, {}) && fours(dstate, dtype, {});
+  const ConvPlan plan = conv_plan(batch, length, ceil_div(channels, 4), kConvBackwardResident);
+  p.chunk = (int)plan.chunk, p.chunks = (int)plan.chunks;
+  xe_status status = XE_OK;
+  by_vector(dtype, vec, [&](auto t, auto v) {
+    constexpr int V = decltype(v)::value;
     by_width(width, [&](auto w) {
-      xe::conv::causal_conv_backward_kernel<decltype(t), decltype(w)::value><<<grid, 128, 0, as_stream(stream)>>>(p);
+      status = launch_conv(what, p, V, xe::conv::causal_conv_backward_kernel<decltype(t), decltype(w)::value, V>,
+                           as_stream(stream));
     });
   });
-  if (xe_status s = launched(what)) return s;
-  return sum_rows(p.partial, batch * chunks, channels * (width + 1), dweight, as_stream(stream));
+  if (status != XE_OK) return status;
+  return sum_rows(p.partial, batch * plan.chunks, channels * (width + 1), dweight, as_stream(stream));
 }
 
 }  // extern "C"
@@ -429,10 +461,12 @@ struct NormShape {
   int groups, warps_per_row, threads, rows_per_block;
 };
 
-// Groups of eight elements per thread and warps per row.
-bool norm_shape(int64_t columns, int64_t rows, bool backward, NormShape& s) {
+// Groups of eight elements per thread and warps per row.  One group needs the fewest registers, so that
+// many rows are in flight; few rows want the most threads on each.
+bool norm_shape(int64_t columns, bool backward, int64_t rows, NormShape& s) {
   const int64_t groups = ceil_div(columns, 8);
-  if (groups <= 256)
+  const int64_t one = backward ? 512 : rows <= 148 ? 1024 : 256;
+  if (groups <= one)
     s.groups = 1;
   else if (groups <= 1024)
     s.groups = 2;
@@ -442,14 +476,27 @@ bool norm_shape(int64_t columns, int64_t rows, bool backward, NormShape& s) {
     s.groups = 8;
   else
     return false;
-  (void)rows;
-  (void)backward;
-  int wpr = 1;
-  while ((int64_t)wpr * 32 * s.groups < groups) wpr *= 2;
-  s.warps_per_row = wpr;
-  s.threads = std::max(256, wpr * 32);
-  s.rows_per_block = s.threads / (wpr * 32);
+  s.warps_per_row = (int)ceil_div(groups, 32 * s.groups);
+  s.rows_per_block = std::max(1, 8 / s.warps_per_row);
+  s.threads = s.warps_per_row * 32 * s.rows_per_block;
   return true;
+}
+
+// Prepares a persistent kernel and gives its number of blocks: what the device holds at once, or fewer.
+// `Tag`: a type of its own for each kernel, since kernels of one signature share a pointer type.
+template <typename Tag, typename K>
+int64_t persistent_blocks(K kernel, int threads, int bytes, int64_t wanted) {
+  static std::atomic<int> known[32][33];  // by device and warps
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::atomic<int>& at = known[dev & 31][threads / 32];
+  int each = at.load();
+  if (each == 0) {
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, threads, bytes) != cudaSuccess || each < 1) each = 1;
+    at.store(each);
+  }
+  return std::min<int64_t>(wanted, 148ll * each);
 }
 
 template <typename F>
@@ -485,8 +532,9 @@ xe_status check_norm(const char* what, int64_t rows, int64_t columns, int32_t dt
   return XE_OK;
 }
 
+// The most blocks of the backward kernel (the workspace is planned for them).
 int64_t norm_backward_blocks(int64_t rows, const NormShape& s) {
-  return std::min<int64_t>(ceil_div(rows, s.rows_per_block), 148 * 2);
+  return std::min<int64_t>(ceil_div(rows, s.rows_per_block), 148ll * std::max(1, 1024 / s.threads));
 }
 
 }  // namespace
@@ -504,9 +552,7 @@ xe_status xe_rms_norm(const void* x, int64_t x_row, const void* residual, int64_
   if (quantize && rows > 0 && !scale) return fail(XE_ERR_INVALID_ARGUMENT, "%s: 8-bit outputs need scales", what);
   if (rows == 0) return XE_OK;
   NormShape shape;
-  if (!norm_shape(columns, rows, false, shape)) return fail(XE_ERR_NOT_SUPPORTED, "%s: too many columns", what);
-  const int64_t blocks = ceil_div(rows, shape.rows_per_block);
-  if (blocks > INT_MAX) return fail(XE_ERR_NOT_SUPPORTED, "%s: too many rows", what);
+  if (!norm_shape(columns, false, rows, shape)) return fail(XE_ERR_NOT_SUPPORTED, "%s: too many columns", what);
   xe::norm::Params p{};
   p.x = x, p.residual = residual, p.weight = weight, p.y = y, p.sum = sum, p.scale = scale;
   p.x_row = x_row, p.r_row = residual_row, p.rows = rows, p.columns = (int)columns, p.eps = eps;
@@ -517,9 +563,20 @@ xe_status xe_rms_norm(const void* x, int64_t x_row, const void* residual, int64_
                    columns % 8 == 0;
   by_types(dtype, residual_dtype, [&](auto t, auto r) {
     by_groups(shape.groups, [&](auto g) {
-      auto kernel = vec ? xe::norm::rms_norm_kernel<decltype(t), decltype(r), decltype(g)::value, true>
-                        : xe::norm::rms_norm_kernel<decltype(t), decltype(r), decltype(g)::value, false>;
-      kernel<<<(unsigned)blocks, shape.threads, 0, as_stream(stream)>>>(p, shape.warps_per_row);
+      auto go = [&](auto v) {
+        auto kernel = xe::norm::rms_norm_kernel<decltype(t), decltype(r), decltype(g)::value, decltype(v)::value>;
+        struct Tag {};
+        using T = decltype(t);
+        using R = decltype(r);
+        constexpr int kGroups = decltype(g)::value;
+        const int bytes = decltype(v)::value ? xe::norm::kForwardStages<T, R, kGroups> * shape.threads * xe::norm::kForwardBytes<T, R, kGroups> : 0;
+        const int64_t blocks = persistent_blocks<Tag>(kernel, shape.threads, bytes, ceil_div(rows, shape.rows_per_block));
+        kernel<<<(unsigned)blocks, shape.threads, bytes, as_stream(stream)>>>(p, shape.warps_per_row);
+      };
+      if (vec)
+        go(std::true_type{});
+      else
+        go(std::false_type{});
     });
   });
   return launched(what);
@@ -527,7 +584,7 @@ xe_status xe_rms_norm(const void* x, int64_t x_row, const void* residual, int64_
 
 size_t xe_rms_norm_backward_workspace_size(int64_t rows, int64_t columns) {
   NormShape shape;
-  if (rows <= 0 || columns < 1 || !norm_shape(columns, rows, true, shape)) return 0;
+  if (rows <= 0 || columns < 1 || !norm_shape(columns, true, rows, shape)) return 0;
   return padded((size_t)(norm_backward_blocks(rows, shape) * shape.rows_per_block * columns) * 4);
 }
 
@@ -542,8 +599,8 @@ xe_status xe_rms_norm_backward(const void* sum, int64_t sum_row, const void* add
   if (dweight && (!workspace || workspace_bytes < xe_rms_norm_backward_workspace_size(rows, columns)))
     return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
   NormShape shape;
-  if (!norm_shape(columns, rows, true, shape)) return fail(XE_ERR_NOT_SUPPORTED, "%s: too many columns", what);
-  const int64_t blocks = norm_backward_blocks(rows, shape);
+  if (!norm_shape(columns, true, rows, shape)) return fail(XE_ERR_NOT_SUPPORTED, "%s: too many columns", what);
+  int64_t blocks = norm_backward_blocks(rows, shape);
   xe::norm::BackwardParams p{};
   p.sum = sum, p.addend = addend, p.a_row = addend_row, p.weight = weight, p.dy = dy, p.dsum = dsum, p.dx = dx;
   p.partial = dweight ? static_cast<float*>(workspace) : nullptr;
@@ -554,9 +611,20 @@ xe_status xe_rms_norm_backward(const void* sum, int64_t sum_row, const void* add
                    vectors(dx, residual_dtype, {}) && columns % 8 == 0;
   by_types(dtype, residual_dtype, [&](auto t, auto r) {
     by_groups(shape.groups, [&](auto g) {
-      auto kernel = vec ? xe::norm::rms_norm_backward_kernel<decltype(t), decltype(r), decltype(g)::value, true>
-                        : xe::norm::rms_norm_backward_kernel<decltype(t), decltype(r), decltype(g)::value, false>;
-      kernel<<<(unsigned)blocks, shape.threads, 0, as_stream(stream)>>>(p, shape.warps_per_row);
+      auto go = [&](auto v) {
+        auto kernel = xe::norm::rms_norm_backward_kernel<decltype(t), decltype(r), decltype(g)::value, decltype(v)::value>;
+        struct Tag {};
+        using T = decltype(t);
+        using R = decltype(r);
+        constexpr int kGroups = decltype(g)::value;
+        const int bytes = decltype(v)::value ? xe::norm::kBackwardStages<T, R, kGroups> * shape.threads * xe::norm::kBackwardBytes<T, R, kGroups> : 0;
+        blocks = persistent_blocks<Tag>(kernel, shape.threads, bytes, blocks);
+        kernel<<<(unsigned)blocks, shape.threads, bytes, as_stream(stream)>>>(p, shape.warps_per_row);
+      };
+      if (vec)
+        go(std::true_type{});
+      else
+        go(std::false_type{});
     });
   });
   if (xe_status s = launched(what)) return s;

@@ -42,13 +42,13 @@ def _operand(what: str, name: str, t: torch.Tensor, like: torch.Tensor, shape: t
     """Checks one operand and makes its last axis contiguous."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: expected torch.Tensor for {name}, got {type(t).__name__}")
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise ValueError(f"{what}: tensors on different devices ({like.device} and {t.device})")
     if t.dtype != dtype:
         raise NotImplementedError(f"{what}: {name} must be {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.is_contiguous() or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _parameter(what: str, name: str, t: torch.Tensor, like: torch.Tensor, shape: tuple) -> torch.Tensor:
@@ -68,16 +68,28 @@ def _pointer(t: torch.Tensor | None) -> int | None:
 
 def _call(device: torch.device, name: str, *args) -> None:
     """Calls an entry point on the device's current stream (its last argument)."""
-    if device.index != torch.cuda.current_device():
+    index = device.index
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return _call(device, name, *args)
-    status = getattr(_lib.load(), name)(*args, torch.cuda.current_stream(device).cuda_stream)
+    status = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _lib.check(status, name)
 
 
+def _like(x: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """An empty contiguous tensor of x's shape (empty_like alone would keep the order of x's axes)."""
+    if x.is_contiguous():
+        return torch.empty_like(x, dtype=dtype) if dtype else torch.empty_like(x)
+    return torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def _needs_grad(*tensors: torch.Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _no_backward(what: str, *tensors: torch.Tensor | None) -> None:
@@ -119,7 +131,7 @@ def causal_conv1d(
     x, weight, bias, state, lengths, code = _conv_operands("causal_conv1d", x, weight, bias, state, lengths, activation)
     batch, length, channels = x.shape
     width = weight.shape[1]
-    y = torch.empty((batch, length, channels), device=x.device, dtype=x.dtype)
+    y = _like(x)
     new = torch.empty((batch, width - 1, channels), device=x.device, dtype=x.dtype) if return_state else None
     _call(
         x.device, "xe_causal_conv1d", x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _pointer(bias),
@@ -177,7 +189,7 @@ def causal_conv1d_step(
     _operand(what, "state", state, x, (batch, width - 1, channels), x.dtype)
     if not state.is_contiguous():
         raise ValueError(f"{what}: state is updated in place and must be contiguous")
-    y = torch.empty((batch, channels), device=x.device, dtype=x.dtype)
+    y = _like(x)
     _call(
         x.device, "xe_causal_conv1d_step", x.data_ptr(), x.stride(0), weight.data_ptr(), _pointer(bias), state.data_ptr(),
         y.data_ptr(), batch, channels, width, _ACTIVATIONS[activation], code,
@@ -191,14 +203,14 @@ def causal_conv1d_backward(x, weight, bias, state, activation, lengths, dy, dsta
     x, weight, bias, state, lengths, code = _conv_operands(what, x, weight, bias, state, lengths, activation)
     batch, length, channels = x.shape
     width = weight.shape[1]
-    dx = torch.empty((batch, length, channels), device=x.device, dtype=x.dtype)
+    dx = _like(x)
     dstate = torch.empty((batch, width - 1, channels), device=x.device, dtype=x.dtype) if need_dstate else None
     if batch == 0 or channels == 0:
         return dx, torch.zeros_like(weight), torch.zeros(channels, device=x.device), dstate
     dy = _operand(what, "dy", dy, x, x.shape, x.dtype)
     if dstate_out is not None:
         dstate_out = _operand(what, "the state's gradient", dstate_out, x, (batch, width - 1, channels), x.dtype).contiguous()
-    dweight = torch.empty((channels, width + 1), device=x.device, dtype=torch.float32)
+    dweight = torch.empty((width + 1, channels), device=x.device, dtype=torch.float32)
     size = _lib.load().xe_causal_conv1d_backward_workspace_size(batch, length, channels, width)
     workspace = _workspace(size, x.device)
     _call(
@@ -207,7 +219,7 @@ def causal_conv1d_backward(x, weight, bias, state, activation, lengths, dy, dsta
         dweight.data_ptr(), _pointer(lengths), int(lengths is not None and lengths.dtype == torch.int64), batch, length,
         channels, width, _ACTIVATIONS[activation], code, _pointer(workspace), size,
     )
-    return dx, dweight[:, :width], dweight[:, width], dstate
+    return dx, dweight[:width].t(), dweight[width], dstate
 
 
 # ---------------------------------------------------------------------------
@@ -301,7 +313,7 @@ def _scan_forward(x, delta, a, b, c, d, z, delta_bias, softplus, state, lengths,
     batch, length, channels = x.shape
     states = a.shape[1]
     lib = _lib.load()
-    y = torch.empty((batch, length, channels), device=x.device, dtype=x.dtype)
+    y = _like(x)
     args.y = y.data_ptr()
     new = checkpoints = None
     if return_state:
@@ -364,7 +376,7 @@ def selective_scan_step(
     _operand(what, "state", state, x, (batch, channels, states), torch.float32)
     if not state.is_contiguous():
         raise ValueError(f"{what}: state is updated in place and must be contiguous")
-    y = torch.empty((batch, channels), device=x.device, dtype=dtype)
+    y = _like(x)
     args = _lib.SelectiveScanArgs(
         x.data_ptr(), delta.data_ptr(), _pointer(z), b.data_ptr(), c.data_ptr(), y.data_ptr(), a.data_ptr(), _pointer(d),
         _pointer(delta_bias), None, state.data_ptr(), None, None,
@@ -385,10 +397,7 @@ def selective_scan_backward(x, delta, a, b, c, d, z, delta_bias, softplus, state
     states = a.shape[1]
     device, dtype = x.device, x.dtype
 
-    def like_x():
-        return torch.empty((batch, length, channels), device=device, dtype=dtype)
-
-    dx, ddelta, dz = like_x(), like_x(), like_x() if z is not None else None
+    dx, ddelta, dz = _like(x), _like(x), _like(x) if z is not None else None
     db, dc = (torch.empty((batch, length, groups, states), device=device, dtype=dtype) for _ in range(2))
     da = torch.empty((channels, states), device=device, dtype=torch.float32)
     dd = torch.empty((2, channels), device=device, dtype=torch.float32)
@@ -440,53 +449,57 @@ def rms_norm(
 
         y, total = RmsNorm.apply(x, weight, residual, eps)
         return y if residual is None else (y, total)
-    rows, weight, residual, code, weight_code, residual_code = _norm_operands(what, x, weight, residual)
-    columns = x.shape[-1]
-    device = x.device
-    scale = None
+    return _norm_forward(x, weight, residual, eps, quantize)
+
+
+def _norm_forward(x, weight, residual, eps, quantize):
+    what = "rms_norm"
+    device = _device_of(what, x)
+    code = _dtype_code(what, x)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"{what}: needs a last axis of at least one element")
+    rows = _as_rows(x)
+    count, columns = rows.shape
+    weight_ptr = residual_ptr = sum_ptr = scale_ptr = None
+    weight_code, residual_code, residual_row = _lib.XE_F32, code, 0
+    if weight is not None:
+        if weight.dtype != torch.float32:
+            weight_code = code
+        weight = _operand(what, "weight", weight, x, (columns,), torch.float32 if weight_code == _lib.XE_F32 else x.dtype)
+        weight = weight.contiguous()
+        weight_ptr = weight.data_ptr()
+    total = scale = None
+    if residual is not None:
+        if residual.dtype == torch.float32:
+            residual_code = _lib.XE_F32
+        residual = _as_rows(_operand(what, "residual", residual, x, x.shape, torch.float32 if residual_code == _lib.XE_F32 else x.dtype))
+        total = _like(x, residual.dtype)
+        residual_ptr, residual_row, sum_ptr = residual.data_ptr(), residual.stride(0), total.data_ptr()
     if quantize is None:
-        y = torch.empty(x.shape, device=device, dtype=x.dtype)
-        out_code = code
+        y, out_code = _like(x), code
     elif quantize in _QUANTIZE:
-        y = torch.empty(x.shape, device=device, dtype=_QUANTIZE[quantize])
-        scale = torch.empty(x.shape[:-1], device=device, dtype=torch.float32)
+        y = _like(x, _QUANTIZE[quantize])
         out_code = _QUANTIZED[y.dtype]
+        scale = torch.empty(x.shape[:-1], device=device, dtype=torch.float32)
+        scale_ptr = scale.data_ptr()
     else:
         raise ValueError(f"{what}: unknown quantize {quantize!r}; expected None, 'e4m3' or 'int8'")
-    total = None if residual is None else torch.empty(x.shape, device=device, dtype=residual.dtype)
     _call(
-        device, "xe_rms_norm", rows.data_ptr(), rows.stride(0), _pointer(residual),
-        0 if residual is None else residual.stride(0), _pointer(weight), y.data_ptr(), _pointer(total), _pointer(scale),
-        rows.shape[0], columns, eps, code, residual_code, weight_code, out_code,
+        device, "xe_rms_norm", rows.data_ptr(), rows.stride(0), residual_ptr, residual_row, weight_ptr, y.data_ptr(),
+        sum_ptr, scale_ptr, count, columns, eps, code, residual_code, weight_code, out_code,
     )
-    out = (y,) if scale is None else (y, scale)
-    if total is not None:
-        out += (total,)
-    return out[0] if len(out) == 1 else out
+    if scale is None:
+        return y if total is None else (y, total)
+    return (y, scale) if total is None else (y, scale, total)
 
 
 def _as_rows(t: torch.Tensor) -> torch.Tensor:
     """(rows, columns) with contiguous columns; a copy only where the rows have no common stride."""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     if t.stride(-1) != 1 and t.shape[-1] != 1:
         t = t.contiguous()
     return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-
-
-def _norm_operands(what, x, weight, residual):
-    _device_of(what, x)
-    code = _dtype_code(what, x)
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"{what}: needs a last axis of at least one element")
-    weight_code, residual_code = _lib.XE_F32, code
-    if weight is not None:
-        wide = weight.dtype == torch.float32
-        weight = _operand(what, "weight", weight, x, x.shape[-1:], torch.float32 if wide else x.dtype).contiguous()
-        weight_code = _lib.XE_F32 if wide else code
-    if residual is not None:
-        wide = residual.dtype == torch.float32
-        residual = _as_rows(_operand(what, "residual", residual, x, x.shape, torch.float32 if wide else x.dtype))
-        residual_code = _lib.XE_F32 if wide else code
-    return _as_rows(x), weight, residual, code, weight_code, residual_code
 
 
 def rms_norm_backward(total, addend, weight, dy, dtotal, eps, need_dweight):
@@ -501,7 +514,7 @@ def rms_norm_backward(total, addend, weight, dy, dtotal, eps, need_dweight):
     if addend is not None:
         addend = _as_rows(addend)
     dsum = None if dtotal is None else _as_rows(_operand(what, "the sum's gradient", dtotal, total, total.shape, total.dtype))
-    dx = torch.empty(total.shape, device=device, dtype=total.dtype)
+    dx = _like(total)
     columns = total.shape[-1]
     dweight = torch.empty(columns, device=device, dtype=torch.float32) if need_dweight else None
     if rows.shape[0] == 0:

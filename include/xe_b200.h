@@ -487,8 +487,8 @@ xe_status xe_causal_conv1d_step(const void* x, int64_t x_sb, const float* weight
                                 int64_t batch, int64_t channels, int64_t width, int32_t activation, int32_t dtype,
                                 void* stream);
 
-/* Gradients of xe_causal_conv1d: dx, dstate (or NULL) and dweight, float32 (channels,
- * width + 1) with the bias's gradient in the last column.  dstate_out (or NULL) is the
+/* Gradients of xe_causal_conv1d: dx, dstate (or NULL) and dweight, float32 (width + 1,
+ * channels): a row for each tap, then the bias's gradient.  dstate_out (or NULL) is the
  * gradient of the new state. */
 size_t xe_causal_conv1d_backward_workspace_size(int64_t batch, int64_t length, int64_t channels, int64_t width);
 xe_status xe_causal_conv1d_backward(const void* x, int64_t x_sb, int64_t x_st, const float* weight, const float* bias,
