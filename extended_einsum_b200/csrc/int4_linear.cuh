@@ -7,12 +7,17 @@
 // last bits of the significand), and subtracting 128 + z (1024 + z) leaves the exact integer q - z.  The
 // tensor core sums these integers against the 16-bit activations exactly into float32 (the weights as
 // the 16-row operand, the tokens as the 8 columns), and each group's sum is scaled in float32.
-// Activations of 8 bits convert to bf16 exactly; float32 ones enter as three bf16 parts (8 + 8 + 8
+// Activations of 8 bits convert to f16 exactly; float32 ones enter as three bf16 parts (8 + 8 + 8
 // bits of significand, also exact) in columns of their own.
 //
 // The order of k inside a group of eight is free as long as both operands agree: a 32-bit word of
 // codes gives the pairs (0, 4), (1, 5), (2, 6), (3, 7) by masking and shifting, so the activations
 // are staged in that order.
+//
+// A block holds a part of k of the activations in shared memory (the blocks of a cluster share the rows and
+// split k between them, so that a part fits), its warps take row tiles of sixteen and every so many stages of
+// 128 k, each with a ring of its own that cp.async fills.  Partial sums meet in shared memory, the warps' first
+// and then the cluster's, in a fixed order.
 #pragma once
 
 #include "seq_common.cuh"
@@ -37,9 +42,11 @@ struct Params {
   int64_t x_row, packed_row;  // strides of a row: elements, bytes
   int rows, inputs, outputs, group;
   int scale_dtype, y_dtype;
+  int x_vec;    // rows of x start on 16-byte boundaries (8 bytes for 8-bit types)
   int pieces;   // columns of the product per token: 3 for float32 activations, else 1
   int tokens;   // tokens of one block
-  int chunk;    // k staged at a time
+  int part;     // k of one block of the cluster, a multiple of kStageK
+  int chunk;    // k staged at a time, a multiple of kStageK
   int pitch;    // of the staged activations, elements
   int warps_k;  // warps along k; the others along rows
 };
@@ -83,60 +90,101 @@ struct Arithmetic<true> {
   }
 };
 
-// Eight activations as 16-bit floats in the order 0 4 1 5 2 6 3 7; piece p of float32 ones.
+// Eight activations as they lie in memory, and as 16-bit floats in the order 0 4 1 5 2 6 3 7.
 template <typename X>
-__device__ __forceinline__ uint4 staged8(const X* at, bool vec, int piece) {
-  uint32_t v[8];
-  if constexpr (sizeof(X) == 1) {
-    uint2 q;
+struct Eight {
+  uint32_t w[2 * sizeof(X)];
+
+  __device__ __forceinline__ void load(const X* at, bool vec) {
     if (vec) {
-      q = *reinterpret_cast<const uint2*>(at);
-    } else {
-      uint32_t w[2] = {0, 0};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i / 4] |= (uint32_t) reinterpret_cast<const uint8_t*>(at)[i] << (8 * (i % 4));
-      q = make_uint2(w[0], w[1]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint8_t code = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i % 4)));
-      float f;
-      if constexpr (__is_same(X, __nv_fp8_e4m3)) {
-        f = __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3)));
+      if constexpr (sizeof(X) == 1) {
+        asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(at));
       } else {
-        f = (float)(int8_t)code;
-      }
-      v[i] = __bfloat16_as_ushort(__float2bfloat16_rn(f));  // exact
-    }
-  } else if constexpr (sizeof(X) == 2) {
-    const Raw8<X> r = load8<X>(at, 8, vec);
-    const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (w[i / 2] >> (16 * (i % 2))) & 0xffffu;
-  } else {
-    float f[8];
-    load8f<X>(at, 8, vec, f);
+        for (int i = 0; i < (int)sizeof(X) / 2; ++i)
+          asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3])
+                       : "l"(reinterpret_cast<const uint4*>(at) + i));
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * (int)sizeof(X); ++i) w[i] = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      // the leading bits by truncation, so that no part overflows; the rests are exact
-      const bool finite = fabsf(f[i]) < __uint_as_float(0x7f800000u);
-      uint32_t bits = f[i] != f[i] ? 0x7fc00000u : __float_as_uint(f[i]) & 0xffff0000u;
-      if (piece > 0) {
-        const float rest = f[i] - __uint_as_float(bits);
-        bits = __float_as_uint(rest) & 0xffff0000u;
-        if (piece > 1) bits = __float_as_uint(rest - __uint_as_float(bits));
-        if (!finite) bits = 0;
-      }
-      v[i] = bits >> 16;
+      if constexpr (sizeof(X) == 1)
+        w[i / 4] |= (uint32_t) reinterpret_cast<const uint8_t*>(at)[i] << (8 * (i % 4));
+      else if constexpr (sizeof(X) == 2)
+        w[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(at)[i] << (16 * (i % 2));
+      else
+        w[i] = reinterpret_cast<const uint32_t*>(at)[i];
     }
   }
-  return make_uint4(v[0] | v[4] << 16, v[1] | v[5] << 16, v[2] | v[6] << 16, v[3] | v[7] << 16);
+
+  __device__ __forceinline__ uint4 staged(int piece) const {
+    uint32_t r[4];
+    if constexpr (sizeof(X) == 1) {
+      const uint32_t p[2] = {__byte_perm(w[0], w[1], 0x5140), __byte_perm(w[0], w[1], 0x7362)};  // 0 4 1 5, 2 6 3 7
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (__is_same(X, __nv_fp8_e4m3)) {
+          const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(p[i / 2] >> (16 * (i % 2)) & 0xffffu), __NV_E4M3);
+          r[i] = (uint32_t)h.x | (uint32_t)h.y << 16;
+        } else {
+          // 1024 + 128 + v by the bits of its significand, less 1152
+          const uint32_t u = __byte_perm(p[i / 2] ^ 0x80808080u, 0x64646464u, i % 2 ? 0x4342 : 0x4140);
+          r[i] = Arithmetic<true>::sub(u, 0x64806480u);
+        }
+      }
+    } else if constexpr (sizeof(X) == 2) {
+      r[0] = __byte_perm(w[0], w[2], 0x5410);
+      r[1] = __byte_perm(w[0], w[2], 0x7632);
+      r[2] = __byte_perm(w[1], w[3], 0x5410);
+      r[3] = __byte_perm(w[1], w[3], 0x7632);
+    } else {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // the leading bits by truncation, so that no part overflows; the rests are exact
+        const float f = __uint_as_float(w[i]);
+        const bool finite = fabsf(f) < __uint_as_float(0x7f800000u);
+        uint32_t bits = f != f ? 0x7fc00000u : w[i] & 0xffff0000u;
+        if (piece > 0) {
+          const float rest = f - __uint_as_float(bits);
+          bits = __float_as_uint(rest) & 0xffff0000u;
+          if (piece > 1) bits = __float_as_uint(rest - __uint_as_float(bits));
+          if (!finite) bits = 0;
+        }
+        v[i] = bits;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = __byte_perm(v[i], v[i + 4], 0x7632);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+  }
+};
+
+// A scale is loaded as its bits and converted where it is used: a conversion would wait for the load.
+__device__ __forceinline__ uint32_t load_scale(const void* p, int dtype, int64_t at) {
+  return dtype == XE_F32 ? static_cast<const uint32_t*>(p)[at] : static_cast<const uint16_t*>(p)[at];
+}
+__device__ __forceinline__ float scale_value(uint32_t bits, int dtype) {
+  return dtype == XE_F32   ? __uint_as_float(bits)
+         : dtype == XE_BF16 ? __uint_as_float(bits << 16)
+                            : __half2float(__ushort_as_half((unsigned short)bits));
 }
 
-__device__ __forceinline__ float load_scale(const void* p, int dtype, int64_t at) {
-  if (dtype == XE_F32) return static_cast<const float*>(p)[at];
-  if (dtype == XE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
-  return __half2float(static_cast<const __half*>(p)[at]);
+// All threads of the cluster, with what they have written to shared memory.
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A float of block `rank`'s shared memory, at the place of `at` in this block's.
+__device__ __forceinline__ float cluster_load(const float* at, int rank) {
+  uint32_t remote;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
 }
 
 __device__ __forceinline__ void store_as(void* y, int dtype, int64_t at, float v) {
@@ -148,34 +196,40 @@ __device__ __forceinline__ void store_as(void* y, int dtype, int64_t at, float v
     static_cast<__half*>(y)[at] = __float2half_rn(v);
 }
 
-// X: type of the activations; kTiles: columns / 8; kSplit: groups of 32 or 64 k, so
-// that the four 32s of a stage differ in scale.
+// X: type of the activations; kTiles: columns / 8; kSplit: groups that are no multiple of 128, so that the
+// four 32s of a stage may differ in scale.
 template <typename X, int kTiles, bool kSplit, int kStages>
-__global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(Params p) {
-  constexpr bool kHalf = __is_same(X, __half);
+__global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(const __grid_constant__ Params p) {
+  constexpr bool kHalf = __is_same(X, __half) || sizeof(X) == 1;
   using A = Arithmetic<kHalf>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int quad = lane % 4, row8 = lane / 4;
   const int warp_k = warp % p.warps_k, warp_m = warp / p.warps_k;
   const int rows_per_block = 16 * (kWarps / p.warps_k);
-  const int o0 = blockIdx.x * rows_per_block + warp_m * 16;
-  const int m0 = blockIdx.y * p.tokens;
+  const int o0 = blockIdx.y * rows_per_block + warp_m * 16;
+  const int m0 = blockIdx.z * p.tokens;
   const int tokens = min(p.tokens, p.rows - m0);
   const int columns = tokens * p.pieces;
   uint8_t* ring = smem + warp * (kStages * kStageBytes);
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-  uint16_t* xs = reinterpret_cast<uint16_t*>(smem + kWarps * kStages * kStageBytes);
+  uint8_t* xs = smem + kWarps * kStages * kStageBytes;  // 16 zero bytes, then the activations
   const int groups = p.inputs / p.group;
+  const int k_begin = blockIdx.x * p.part, k_end = min(k_begin + p.part, p.inputs);
 
-  // the two rows of this lane's fragments and of its scales, the row of its copies; past the last
-  // output all read the last one, and the results are dropped
+  // the two rows of this lane's fragments, copies and scales; past the last output all read the last one, and
+  // the results are dropped
   const int last_o = p.outputs - 1;
   const int oa = min(o0 + row8, last_o), ob = min(o0 + row8 + 8, last_o);
-  const uint8_t* copy_from[2];
+  const uint8_t* copy_a = p.packed + (int64_t)oa * p.packed_row + quad * 16;
+  const uint8_t* copy_b = p.packed + (int64_t)ob * p.packed_row + quad * 16;
+  const int64_t scales_a = (int64_t)oa * groups, scales_b = (int64_t)ob * groups;
+  // this lane's column of each tile of eight; those past the last read the zero bytes at every k
+  uint32_t column_at[kTiles];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    copy_from[i] = p.packed + (int64_t)min(o0 + row8 + 8 * i, last_o) * p.packed_row + quad * 16;
+  for (int n = 0; n < kTiles; ++n)
+    column_at[n] = n * 8 + row8 < columns ? 16 + ((n * 8 + row8) * p.pitch + quad * 8) * 2 : 0;
+  if (threadIdx.x < 4) reinterpret_cast<uint32_t*>(xs)[threadIdx.x] = 0;
 
   float acc[kTiles][4];
 #pragma unroll
@@ -183,49 +237,61 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(Params p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
 
-  for (int k0 = 0; k0 < p.inputs; k0 += p.chunk) {
-    const int kn = min(p.chunk, p.inputs - k0);
+  for (int k0 = k_begin; k0 < k_end; k0 += p.chunk) {
+    const int kn = min(p.chunk, k_end - k0);
     const int stages = (kn + kStageK - 1) / kStageK;
     // this warp's stages of the chunk: warp_k, warp_k + warps_k, ...
     const int own = warp_k < stages ? (stages - warp_k + p.warps_k - 1) / p.warps_k : 0;
-    float sa[kStages], sb[kStages], za[kStages], zb[kStages];
+    uint32_t sa[kStages], sb[kStages], za[kStages], zb[kStages];
     auto issue = [&](int i, int slot) {
       if (i < own) {
-        const int k = (warp_k + i * p.warps_k) * kStageK;  // inside the chunk
-        if (k + quad * 32 < kn) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            cp_async16(ring_at + slot * kStageBytes + (row8 + 8 * j) * kRowPitch + quad * 16, copy_from[j] + (k0 + k) / 2);
+        const int k = k0 + (warp_k + i * p.warps_k) * kStageK;
+        if (k + quad * 32 < k_end) {
+          const uint32_t at = ring_at + slot * kStageBytes + row8 * kRowPitch + quad * 16;
+          cp_async16(at, copy_a + k / 2);
+          cp_async16(at + 8 * kRowPitch, copy_b + k / 2);
         }
         // kSplit: lane `quad` holds the scales of the stage's 32s number `quad`
-        const int kk = k0 + k + (kSplit ? quad * 32 : 0);
-        if (kk < p.inputs) {
-          const int64_t ga = (int64_t)oa * groups + kk / p.group, gb = (int64_t)ob * groups + kk / p.group;
-          sa[slot] = load_scale(p.scales, p.scale_dtype, ga);
-          sb[slot] = load_scale(p.scales, p.scale_dtype, gb);
-          za[slot] = p.zeros ? (float)p.zeros[ga] : 8.0f;
-          zb[slot] = p.zeros ? (float)p.zeros[gb] : 8.0f;
+        const int kk = k + (kSplit ? quad * 32 : 0);
+        if (kk < k_end) {
+          const int g = kk / p.group;
+          sa[slot] = load_scale(p.scales, p.scale_dtype, scales_a + g);
+          sb[slot] = load_scale(p.scales, p.scale_dtype, scales_b + g);
+          if (p.zeros) {
+            za[slot] = p.zeros[scales_a + g];
+            zb[slot] = p.zeros[scales_b + g];
+          }
         }
       }
       cp_async_commit();
     };
 #pragma unroll
     for (int i = 0; i < kStages; ++i) {
-      sa[i] = sb[i] = za[i] = zb[i] = 0.0f;
+      sa[i] = sb[i] = 0;
+      za[i] = zb[i] = 8;
     }
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i, i);
-    // stage the activations: 8 k of one column at a time
-    if (k0 > 0) __syncthreads();
-    for (int i = threadIdx.x; i < kTiles * 8 * (kn / 8); i += kWarps * 32) {
-      const int col = i / (kn / 8), k = (i % (kn / 8)) * 8;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (col < columns) {
-        const X* at = static_cast<const X*>(p.x) + (int64_t)(m0 + col / p.pieces) * p.x_row + k0 + k;
-        v = staged8<X>(at, (reinterpret_cast<uintptr_t>(at) & 15) == 0 || (sizeof(X) == 1 && (reinterpret_cast<uintptr_t>(at) & 7) == 0),
-                       col % p.pieces);
+    // stage the activations, eight k at a time: the warps spread over the columns, and over k where there are
+    // fewer columns than warps
+    if (k0 > k_begin) __syncthreads();
+    {
+      const int across = columns > 4 ? 8 : columns > 2 ? 4 : columns > 1 ? 2 : 1;
+      const int along = kWarps / across;
+      for (int col = warp % across; col < columns; col += across) {
+        const X* from = static_cast<const X*>(p.x) + (int64_t)(m0 + col / p.pieces) * p.x_row + k0;
+        const int piece = p.pieces == 1 ? 0 : col % p.pieces;
+        uint8_t* to = xs + 16 + (int64_t)col * p.pitch * 2;
+        for (int k = (warp / across * 32 + lane) * 8; k < kn; k += along * 256 * 4) {
+          Eight<X> e[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (k + j * along * 256 < kn) e[j].load(from + k + j * along * 256, p.x_vec);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (k + j * along * 256 < kn) *reinterpret_cast<uint4*>(to + (k + j * along * 256) * 2) = e[j].staged(piece);
+        }
       }
-      *reinterpret_cast<uint4*>(xs + (int64_t)col * p.pitch + k) = v;
     }
     __syncthreads();
     for (int i0 = 0; i0 < own; i0 += kStages) {
@@ -236,18 +302,19 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(Params p) {
           issue(i + kStages - 1, (slot + kStages - 1) % kStages);
           cp_async_wait<kStages - 1>();
           __syncwarp();
-          const int k = (warp_k + i * p.warps_k) * kStageK;
-          const uint8_t* stage = ring + slot * kStageBytes;
+          const int k = (warp_k + i * p.warps_k) * kStageK;  // inside the chunk
+          const uint8_t* stage = ring + slot * kStageBytes + row8 * kRowPitch + quad * 4;
           float part[kTiles][4];
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
 #pragma unroll
             for (int j = 0; j < 4; ++j) part[n][j] = 0.0f;
-          uint32_t offset_a = A::offset(za[slot]), offset_b = A::offset(zb[slot]);
+          const float first_a = scale_value(sa[slot], p.scale_dtype), first_b = scale_value(sb[slot], p.scale_dtype);
+          const uint32_t offset_a = A::offset((float)za[slot]), offset_b = A::offset((float)zb[slot]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (k + j * 32 < kn) {
-              float scale_a = sa[slot], scale_b = sb[slot];
+              float scale_a = first_a, scale_b = first_b;
               uint32_t off_a = offset_a, off_b = offset_b;
               if (kSplit) {
                 scale_a = __shfl_sync(0xffffffffu, scale_a, j, 4);
@@ -255,8 +322,8 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(Params p) {
                 off_a = __shfl_sync(0xffffffffu, off_a, j, 4);
                 off_b = __shfl_sync(0xffffffffu, off_b, j, 4);
               }
-              const uint32_t wa = *reinterpret_cast<const uint32_t*>(stage + row8 * kRowPitch + j * 16 + quad * 4);
-              const uint32_t wb = *reinterpret_cast<const uint32_t*>(stage + (row8 + 8) * kRowPitch + j * 16 + quad * 4);
+              const uint32_t wa = *reinterpret_cast<const uint32_t*>(stage + j * 16);
+              const uint32_t wb = *reinterpret_cast<const uint32_t*>(stage + 8 * kRowPitch + j * 16);
               uint32_t f[2][4];
 #pragma unroll
               for (int h = 0; h < 4; ++h) {
@@ -267,7 +334,8 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(Params p) {
               }
 #pragma unroll
               for (int n = 0; n < kTiles; ++n) {
-                const uint4 b = *reinterpret_cast<const uint4*>(xs + (int64_t)(n * 8 + row8) * p.pitch + k + j * 32 + quad * 8);
+                const uint32_t at = column_at[n] ? column_at[n] + (k + j * 32) * 2 : 0;
+                const uint4 b = *reinterpret_cast<const uint4*>(xs + at);
                 A::mma(part[n], f[0], b.x, b.y);
                 A::mma(part[n], f[1], b.z, b.w);
               }
@@ -288,29 +356,43 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(Params p) {
         }
       }
     }
-    cp_async_wait<0>();
   }
+  cp_async_wait<0>();
 
-  // sums over the warps of a row tile, in order; one part per warp_k, [warp][16 rows][columns + 1]
+  // sums over the warps of a row tile and then over the blocks of the cluster, in order
   __syncthreads();
   constexpr int kCols = kTiles * 8 + 1;
-  float* red = reinterpret_cast<float*>(smem);
+  float* red = reinterpret_cast<float*>(smem);  // [warp][16 rows][columns + 1]
 #pragma unroll
   for (int n = 0; n < kTiles; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       red[(warp * 16 + row8 + (i / 2) * 8) * kCols + n * 8 + quad * 2 + (i % 2)] = acc[n][i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows_per_block * tokens; i += kWarps * 32) {
+  const int parts = gridDim.x;
+  __syncwarp();
+  if (parts > 1)
+    cluster_barrier();
+  else
+    __syncthreads();
+  for (int i = threadIdx.x + blockIdx.x * (kWarps * 32); i < rows_per_block * tokens; i += parts * (kWarps * 32)) {
     const int r = i % rows_per_block, m = i / rows_per_block;
-    const int o = blockIdx.x * rows_per_block + r;
+    const int o = blockIdx.y * rows_per_block + r;
     if (o >= p.outputs) continue;
     float sum = 0.0f;
-    for (int piece = p.pieces - 1; piece >= 0; --piece)
-      for (int w = 0; w < p.warps_k; ++w)
-        sum += red[(((r / 16) * p.warps_k + w) * 16 + r % 16) * kCols + m * p.pieces + piece];
+    for (int piece = p.pieces - 1; piece >= 0; --piece) {
+      for (int b = 0; b < parts; ++b) {
+        for (int w = 0; w < p.warps_k; ++w) {
+          const float* at = red + (((r / 16) * p.warps_k + w) * 16 + r % 16) * kCols + m * p.pieces + piece;
+          sum += parts > 1 ? cluster_load(at, b) : *at;
+        }
+      }
+    }
     if (p.x_scale) sum *= p.x_scale[m0 + m];
     store_as(p.y, p.y_dtype, (int64_t)(m0 + m) * p.outputs + o, sum);
+  }
+  if (parts > 1) {  // no block leaves while its sums are read
+    __syncwarp();
+    cluster_barrier();
   }
 }
 

@@ -8,10 +8,13 @@
 // channel for softplus and the gate); the 8 bytes of x, delta, z and y of a 16-bit type take a third of
 // that time.
 //
-// Layout: kLanes lanes share a channel and hold S states each, so kLanes * S >= states; states past
-// the real ones have A = B = C = 0.  A block stages a tile of tokens: (delta, delta x) pairs, B and
-// C as float32 in shared memory, the recurrence runs over the tile from registers, and v goes back
-// through shared memory to the threads that hold the tile's x and z.
+// Layout: a block is one warp (no barriers); four lanes share kC channels and hold S states of each,
+// 4 S >= states; states past the real ones have A = B = C = 0.  The warp stages a tile of tokens in shared
+// memory as float32, the recurrence runs over the tile from registers, and v goes back through shared
+// memory to the threads that hold the tile's x and z.  Two channels per thread because of the reads from
+// shared memory: B and C for one channel alone take the whole 128 bytes per clock at the rate of the
+// exponentials.  Tokens are staged and worked on in pairs, so that the packed instructions do two tokens
+// at a time with no copies of delta, u, B or C; only the chain h itself is scalar.
 //
 // Few channels: the length is split into segments.  A first pass runs each segment from a zero state
 // and keeps its last state and sum of delta (the product of its e is exp(A sum delta)), a second
@@ -25,7 +28,7 @@ namespace scan {
 
 using namespace seq;
 
-constexpr int kThreads = 128;
+constexpr int kBackwardThreads = 128;
 
 struct Params {
   const void *x, *delta, *z, *b, *c;
@@ -84,16 +87,16 @@ __device__ __forceinline__ Channels block_channels(const Params& p, int per_bloc
 }
 
 // B and C of a tile as float32, states padded with zeros; tokens at or past `live` read as zero.
-template <typename T, int kTile, int NP>
+template <typename T, int kTile, int NP, int kBlock>
 struct SharedStates {
   static constexpr int kVectors = 2 * kTile * (NP / 8);
-  static constexpr int kEach = (kVectors + kThreads - 1) / kThreads;
+  static constexpr int kEach = (kVectors + kBlock - 1) / kBlock;
   Raw8<T> raw[kEach];
 
   __device__ __forceinline__ void load(const Params& p, int batch, int group, int t0, int live, int wanted = 3) {
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-      const int i = k * kThreads + threadIdx.x;
+      const int i = k * kBlock + threadIdx.x;
       const int n0 = (i % (NP / 8)) * 8;
       const int which = (i / (NP / 8)) & 1;
       const int t = t0 + i / (NP / 8) / 2;
@@ -106,7 +109,7 @@ struct SharedStates {
   __device__ __forceinline__ void store(float* smem) {
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-      const int i = k * kThreads + threadIdx.x;
+      const int i = k * kBlock + threadIdx.x;
       if (i < kVectors) {
         float v[8];
         unpack8<T>(raw[k], v);
@@ -138,163 +141,255 @@ __device__ __forceinline__ float transpose_sum(float (&v)[kLanes], int lane) {
 // same of the reversed recurrence of the backward pass, c_{t-1} = e_t (c_t + C_t dv_t).
 enum Mode { kFull, kStates, kAdjoint };
 
-template <typename T, int S, int kLanes, Mode kMode>
-__global__ void __launch_bounds__(kThreads) selective_scan_kernel(Params p) {
+template <typename T, int S, int kC, Mode kMode>
+__global__ void __launch_bounds__(32) selective_scan_kernel(const __grid_constant__ Params p) {
   constexpr bool kStateOnly = kMode != kFull;
-  constexpr int kChannels = kThreads / kLanes;
-  constexpr int kTile = 8 * kLanes;  // tokens: one group of eight channels per thread
-  constexpr int NP = S * kLanes;
-  constexpr int kPitch = kChannels + 4;
-  __shared__ __align__(16) float2 s_dd[kTile][kChannels + 2];
-  __shared__ __align__(16) float s_bc[kTile * 2 * NP];
-  __shared__ __align__(16) float s_v[kStateOnly ? 1 : kTile][kPitch];
+  constexpr int kLanes = 4;                     // lanes on a channel
+  constexpr int kChannels = 32 / kLanes * kC;   // of the warp
+  constexpr int kQuads = kChannels / 4;         // threads that stage a pair of tokens, four channels each
+  constexpr int kPairs = 32 / kQuads;           // pairs of tokens in a tile
+  constexpr int kTile = 2 * kPairs;
+  constexpr int kRun = kTile < kCheckpoint ? kTile : kCheckpoint;
+  constexpr int NP = kLanes * S;                // states, padded
+  constexpr int kParts = kMode == kFull ? 2 : 1;               // B and C, or the one that is needed
+  constexpr int kEach = kPairs * kParts * (NP / 4) / 32;       // their quads of states per thread
+  static_assert(kPairs * kParts * (NP / 4) % 32 == 0 && kTile % kRun == 0 && kCheckpoint % kRun == 0, "whole turns");
+  // per pair of tokens t, t + 1 and channel: delta_t, delta_{t+1}, u_t, u_{t+1}; u = delta x, or the adjoint's dv
+  __shared__ __align__(16) float4 s_du[kPairs][kChannels + 1];
+  __shared__ __align__(16) float2 s_bc[kPairs * kParts * NP];          // (t, t + 1) of each state
+  __shared__ __align__(16) float2 s_v[kStateOnly ? 1 : kPairs][kChannels + 2];
   const Channels ch = block_channels(p, kChannels);
   // the first segment needs no adjoint from zero, the last one no state
   const int batch = blockIdx.y, segment = blockIdx.z + (kMode == kAdjoint ? 1 : 0);
   const int begin = segment * p.segment_length;
   const int end = min(begin + p.segment_length, p.length);
   const int live = min(end, sequence_length(p.lengths, p.lengths64, batch, p.length));
-
-  // staging: this thread's token and eight channels of every tile
-  const int row = threadIdx.x / (kChannels / 8);
-  const int col = (threadIdx.x % (kChannels / 8)) * 8;
-  const int count = max(0, min(8, ch.count - col));
-  float bias[8], skip[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    bias[i] = p.bias && i < count ? p.bias[ch.first + col + i] : 0.0f;
-    skip[i] = p.d && i < count ? p.d[ch.first + col + i] : 0.0f;
-  }
-  const T* x = kMode == kAdjoint ? static_cast<const T*>(p.dy) + batch * p.dy_sb + ch.first + col
-                                 : static_cast<const T*>(p.x) + batch * p.x_sb + ch.first + col;
-  const int64_t x_st = kMode == kAdjoint ? p.dy_st : p.x_st;
-  const int x_vec = p.vec & (kMode == kAdjoint ? 64 : 1);
-  const T* delta = static_cast<const T*>(p.delta) + batch * p.delta_sb + ch.first + col;
-  const T* z = static_cast<const T*>(p.z) + batch * p.z_sb + ch.first + col;
-  T* y = static_cast<T*>(p.y) + (int64_t)batch * p.length * p.channels + ch.first + col;
-
-  // recurrence: this thread's channel and states
-  const int c = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
-  const bool mine = c < ch.count;
-  const int64_t state_at = ((int64_t)batch * p.channels + ch.first + c) * p.states + lane * S;
-  float a[S], h[S];
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    const bool in = mine && lane * S + s < p.states;
-    a[s] = in ? p.a[(int64_t)(ch.first + c) * p.states + lane * S + s] * kLog2e : 0.0f;
-    h[s] = 0.0f;
-    if (!kStateOnly && in) {
-      if (p.segments > 1)
-        h[s] = p.segment_state[(int64_t)segment * p.batch * p.channels * p.states + state_at + s];
-      else if (p.state)
-        h[s] = p.state[state_at + s];
-    }
-  }
-  float delta_sum = 0.0f;
-
-  Raw8<T> raw_x, raw_d, raw_z, next_z;
-  SharedStates<T, kTile, NP> bc;
-  auto fetch = [&](int t0) {
-    const int t = t0 + row;
-    const int n = t < live ? count : 0;
-    raw_x = load8<T>(x + t * x_st, n, x_vec);
-    raw_d = load8<T>(delta + t * p.delta_st, n, p.vec & 2);
-    if (kMode != kStates && p.z) next_z = load8<T>(z + t * p.z_st, n, p.vec & 4);
-    bc.load(p, batch, ch.group, t0, live, kMode == kFull ? 3 : kMode == kStates ? 1 : 2);
-  };
   const int tiles = (end - begin + kTile - 1) / kTile;
   const int step = kMode == kAdjoint ? -kTile : kTile;
   int t0 = kMode == kAdjoint ? begin + (tiles - 1) * kTile : begin;
-  fetch(t0);
-  for (int tile = 0; tile < tiles; ++tile, t0 += step) {
-    const bool in = t0 + row < live;
-    float xv[8], dv[8];
-    unpack8<T>(raw_x, xv);
-    unpack8<T>(raw_d, dv);
+
+  // staging: this thread's pair of tokens and four channels; the places of the next loads move by a tile at a time
+  const int row = threadIdx.x / kQuads * 2;
+  const int col = threadIdx.x % kQuads * 4;
+  const int count = max(0, min(4, ch.count - col));
+  const int64_t x_st = kMode == kAdjoint ? p.dy_st : p.x_st;
+  const T* x = kMode == kAdjoint ? static_cast<const T*>(p.dy) + batch * p.dy_sb : static_cast<const T*>(p.x) + batch * p.x_sb;
+  x += ch.first + col + (t0 + row) * x_st;
+  const T* delta = static_cast<const T*>(p.delta) + batch * p.delta_sb + ch.first + col + (t0 + row) * p.delta_st;
+  const T* z = static_cast<const T*>(p.z) + batch * p.z_sb + ch.first + col + (t0 + row) * p.z_st;
+  T* y = static_cast<T*>(p.y) + ((int64_t)batch * p.length + t0 + row) * p.channels + ch.first + col;
+  const bool whole_x = (p.vec & (kMode == kAdjoint ? 64 : 1)) && count == 4, whole_d = (p.vec & 2) && count == 4;
+  const bool whole_z = (p.vec & 4) && count == 4, whole_y = (p.vec & 8) && count == 4;
+  const T* shared_at[kEach];  // B and C: pair of tokens, which of the two, four states
+  int shared_t[kEach], shared_n[kEach];
+  bool whole_s[kEach];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v = dv[i] + bias[i];
-      if (p.softplus) v = softplus(v);
-      if (kMode != kAdjoint) {
-        s_dd[row][col + i] = in ? make_float2(v, v * xv[i]) : make_float2(0.0f, 0.0f);
-      } else {
-        float dv_t = xv[i];
-        if (p.z) {
-          float zv[8];
-          unpack8<T>(next_z, zv);
-          dv_t *= zv[i] * sigmoid(zv[i]);
-        }
-        s_dd[row][col + i] = in ? make_float2(v, dv_t) : make_float2(0.0f, 0.0f);
-      }
-    }
-    bc.store(s_bc);
-    raw_z = next_z;
-    __syncthreads();
-    if (tile + 1 < tiles) fetch(t0 + step);
-    if (t0 < live || p.checkpoints) {
-#pragma unroll 2
-      for (int t = 0; t < kTile; t += kLanes) {
-        float v[kLanes];
-#pragma unroll
-        for (int k = 0; k < kLanes; ++k) {
-          if (!kStateOnly && p.checkpoints && mine && (t0 + t + k) % kCheckpoint == 0 && t0 + t + k < p.length) {
-            const int64_t rows = (p.length + kCheckpoint - 1) / kCheckpoint;
-            float* at = p.checkpoints +
-                        (((int64_t)batch * rows + (t0 + t + k) / kCheckpoint) * p.channels + ch.first + c) * NP + lane * S;
-#pragma unroll
-            for (int s = 0; s < S; ++s) at[s] = h[s];
-          }
-          const int at = kMode == kAdjoint ? kTile - 1 - (t + k) : t + k;
-          const float2 dd = s_dd[at][c];
-          float bv[S], cv[S];
-          // B, or C in the adjoint recurrence
-          load_f32<S>(s_bc + (at * 2 + (kMode == kAdjoint ? 1 : 0)) * NP + lane * S, bv);
-          if (!kStateOnly) load_f32<S>(s_bc + ((t + k) * 2 + 1) * NP + lane * S, cv);
-          v[k] = 0.0f;
-          delta_sum += dd.x;
-#pragma unroll
-          for (int s = 0; s < S; ++s) {
-            if (kMode == kAdjoint)
-              h[s] = exp2_fast(dd.x * a[s]) * fmaf(dd.y, bv[s], h[s]);
-            else
-              h[s] = fmaf(exp2_fast(dd.x * a[s]), h[s], dd.y * bv[s]);
-            if (!kStateOnly) v[k] = fmaf(cv[s], h[s], v[k]);
-          }
-        }
-        if (!kStateOnly) {
-          const float sum = transpose_sum<kLanes>(v, lane);
-          s_v[t + lane][c] = sum;
-        }
-      }
-    }
-    if (!kStateOnly) {
-      __syncthreads();
-      if (t0 + row < end && count > 0) {
-        float o[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = in ? fmaf(skip[i], xv[i], s_v[row][col + i]) : 0.0f;
-        if (p.z && in) {
-          float zv[8];
-          unpack8<T>(raw_z, zv);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] *= zv[i] * sigmoid(zv[i]);
-        }
-        store8<T>(y + (int64_t)(t0 + row) * p.channels, count, p.vec & 8, o);
-      }
-    }
-    __syncthreads();
+  for (int k = 0; k < kEach; ++k) {
+    const int i = k * 32 + threadIdx.x;
+    const int n0 = i % (NP / 4) * 4;
+    const bool second = kMode == kAdjoint || (kParts == 2 && i / (NP / 4) % 2);
+    shared_t[k] = i / (NP / 4 * kParts) * 2;
+    shared_n[k] = max(0, min(4, p.states - n0));
+    whole_s[k] = (p.vec & (second ? 32 : 16)) && (shared_n[k] == 4 || shared_n[k] == 0);
+    shared_at[k] = second ? static_cast<const T*>(p.c) + batch * p.c_sb + ch.group * p.c_sg + n0 + (t0 + shared_t[k]) * p.c_st
+                          : static_cast<const T*>(p.b) + batch * p.b_sb + ch.group * p.b_sg + n0 + (t0 + shared_t[k]) * p.b_st;
   }
-  if (!mine) return;
-  if (kStateOnly) {
-    float* out = p.segment_state + (int64_t)segment * p.batch * p.channels * p.states + state_at;
+  float bias[4], skip[4];
 #pragma unroll
-    for (int s = 0; s < S; ++s)
-      if (lane * S + s < p.states) out[s] = h[s];
-    if (lane == 0) p.segment_delta[((int64_t)segment * p.batch + batch) * p.channels + ch.first + c] = delta_sum;
-  } else if (p.state_out && segment == p.segments - 1) {
+  for (int i = 0; i < 4; ++i) {
+    bias[i] = p.bias && i < count ? p.bias[ch.first + col + i] : 0.0f;
+    skip[i] = !kStateOnly && p.d && i < count ? p.d[ch.first + col + i] : 0.0f;
+  }
+
+  // recurrence: this thread's kC channels and S states of each
+  const int mine = threadIdx.x / kLanes * kC, lane = threadIdx.x % kLanes;
+  F2 a[kC][S];  // twice, for two tokens at a time
+  float h[kC][S];
+  const int64_t state_at = ((int64_t)batch * p.channels + ch.first + mine) * p.states + lane * S;
 #pragma unroll
-    for (int s = 0; s < S; ++s)
-      if (lane * S + s < p.states) p.state_out[state_at + s] = h[s];
+  for (int j = 0; j < kC; ++j) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const bool in = mine + j < ch.count && lane * S + s < p.states;
+      a[j][s] = both(in ? p.a[(int64_t)(ch.first + mine + j) * p.states + lane * S + s] * kLog2e : 0.0f);
+      h[j][s] = 0.0f;
+      if (!kStateOnly && in) {
+        if (p.segments > 1)
+          h[j][s] = p.segment_state[(int64_t)segment * p.batch * p.channels * p.states + state_at + j * p.states + s];
+        else if (p.state)
+          h[j][s] = p.state[state_at + j * p.states + s];
+      }
+    }
+  }
+  F2 delta_sum[kC] = {};
+  const int64_t checkpoint_rows = (p.length + kCheckpoint - 1) / kCheckpoint;
+  float* checkpoints = p.checkpoints + ((int64_t)batch * checkpoint_rows * p.channels + ch.first + mine) * NP + lane * S;
+
+  struct {
+    Raw4<T> x, d, z;
+  } next[2];
+  Raw4<T> next_s[kEach][2];
+  auto fetch = [&](int at) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const bool in = at + row + q < live;
+      next[q].x = load4_if<T>(x + q * x_st, in, count, whole_x);
+      next[q].d = load4_if<T>(delta + q * p.delta_st, in, count, whole_d);
+      if (kMode != kStates && p.z) next[q].z = load4_if<T>(z + q * p.z_st, in, count, whole_z);
+    }
+    x += step * x_st;
+    delta += step * p.delta_st;
+    z += step * p.z_st;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const bool second = kMode == kAdjoint || (kParts == 2 && (k * 32 + threadIdx.x) / (NP / 4) % 2);
+      const int64_t st = second ? p.c_st : p.b_st;
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        next_s[k][q] = load4_if<T>(shared_at[k] + q * st, shared_n[k] > 0 && at + shared_t[k] + q < live, shared_n[k], whole_s[k]);
+      shared_at[k] += step * st;
+    }
+  };
+  if (tiles > 0) fetch(t0);
+  for (int tile = 0; tile < tiles; ++tile, t0 += step) {
+    const bool in[2] = {t0 + row < live, t0 + row + 1 < live};
+    F2 xv[4];
+    Raw4<T> z_raw[2] = {next[0].z, next[1].z};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      xv[i] = pack2(value4<T>(next[0].x, i), value4<T>(next[1].x, i));
+      F2 d = add2(pack2(value4<T>(next[0].d, i), value4<T>(next[1].d, i)), both(bias[i]));
+      if (p.softplus) d = softplus2(d);
+      float2 dd = unpack2(d);
+      if (!in[0]) dd.x = 0.0f;  // x, z, B and C have been read as zero
+      if (!in[1]) dd.y = 0.0f;
+      F2 u;
+      if (kMode == kAdjoint)
+        u = p.z ? gate2(xv[i], pack2(value4<T>(z_raw[0], i), value4<T>(z_raw[1], i))) : xv[i];
+      else
+        u = mul2(pack2(dd.x, dd.y), xv[i]);
+      const float2 uu = unpack2(u);
+      s_du[row / 2][col + i] = make_float4(dd.x, dd.y, uu.x, uu.y);
+    }
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      float4* at = reinterpret_cast<float4*>(s_bc + (k * 32 + threadIdx.x) * 4);
+#pragma unroll
+      for (int i = 0; i < 4; i += 2)
+        at[i / 2] = make_float4(value4<T>(next_s[k][0], i), value4<T>(next_s[k][1], i), value4<T>(next_s[k][0], i + 1),
+                                value4<T>(next_s[k][1], i + 1));
+    }
+    __syncwarp();
+    if (tile + 1 < tiles) fetch(t0 + step);
+    if (t0 < live || (!kStateOnly && p.checkpoints)) {
+#pragma unroll 1
+      for (int t1 = 0; t1 < kTile; t1 += kRun) {
+        if (!kStateOnly && p.checkpoints && (t0 + t1) % kCheckpoint == 0 && t0 + t1 < p.length) {
+#pragma unroll
+          for (int j = 0; j < kC; ++j) {
+            float* at = checkpoints + ((int64_t)((t0 + t1) / kCheckpoint) * p.channels + j) * NP;
+            if (mine + j < ch.count) {
+#pragma unroll
+              for (int s = 0; s < S; s += 4)
+                *reinterpret_cast<float4*>(at + s) = make_float4(h[j][s], h[j][s + 1], h[j][s + 2], h[j][s + 3]);
+            }
+          }
+        }
+#pragma unroll
+        for (int t2 = 0; t2 < kRun; t2 += 4) {
+          float v[kC][4];
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {
+            const int pair = (kMode == kAdjoint ? kTile - 2 - (t1 + t2 + k) : t1 + t2 + k) / 2;
+            // B, or C in the adjoint recurrence
+            const ulonglong2* bv = reinterpret_cast<const ulonglong2*>(s_bc + (pair * kParts) * NP + lane * S);
+            const ulonglong2* cv = bv + NP / 2;
+            ulonglong2 du[kC];
+            F2 sum[kC];
+#pragma unroll
+            for (int j = 0; j < kC; ++j) {
+              du[j] = *reinterpret_cast<const ulonglong2*>(&s_du[pair][mine + j]);
+              if (kStateOnly) delta_sum[j] = add2(delta_sum[j], du[j].x);
+            }
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+              const F2 b2 = s % 2 ? bv[s / 2].y : bv[s / 2].x;
+#pragma unroll
+              for (int j = 0; j < kC; ++j) {
+                const float2 e = unpack2(exp2_fast2(mul2(du[j].x, a[j][s])));
+                const float2 u = unpack2(mul2(du[j].y, b2));
+                if (kMode == kAdjoint) {
+                  h[j][s] = e.y * (h[j][s] + u.y);
+                  h[j][s] = e.x * (h[j][s] + u.x);
+                } else {
+                  const float first = fmaf(e.x, h[j][s], u.x);
+                  h[j][s] = fmaf(e.y, first, u.y);
+                  if (!kStateOnly) {
+                    const F2 c2 = s % 2 ? cv[s / 2].y : cv[s / 2].x;
+                    const F2 hh = pack2(first, h[j][s]);
+                    sum[j] = s == 0 ? mul2(c2, hh) : fma2(c2, hh, sum[j]);
+                  }
+                }
+              }
+            }
+            if (!kStateOnly) {
+#pragma unroll
+              for (int j = 0; j < kC; ++j) {
+                const float2 q = unpack2(sum[j]);
+                v[j][k] = q.x, v[j][k + 1] = q.y;
+              }
+            }
+          }
+          if (!kStateOnly) {
+            float* at = reinterpret_cast<float*>(&s_v[(t1 + t2 + lane) / 2][mine]) + lane % 2;
+#pragma unroll
+            for (int j = 0; j < kC; ++j) at[2 * j] = transpose_sum<4>(v[j], lane);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (!kStateOnly) {
+      float o[2][4];
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(&s_v[row / 2][col + i]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          F2 v = fma2(both(skip[i + k]), xv[i + k], k ? q.y : q.x);
+          if (p.z) v = gate2(v, pack2(value4<T>(z_raw[0], i + k), value4<T>(z_raw[1], i + k)));
+          const float2 f = unpack2(v);
+          o[0][i + k] = f.x, o[1][i + k] = f.y;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (t0 + row + q < end && count > 0) {
+          if (!in[q]) o[q][0] = o[q][1] = o[q][2] = o[q][3] = 0.0f;
+          store4<T>(y + q * (int64_t)p.channels, count, whole_y, o[q]);
+        }
+      }
+      y += (int64_t)kTile * p.channels;
+      __syncwarp();
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kC; ++j) {
+    if (mine + j >= ch.count) continue;
+    float* out = nullptr;
+    if (kStateOnly)
+      out = p.segment_state + (int64_t)segment * p.batch * p.channels * p.states + state_at + j * p.states;
+    else if (p.state_out && segment == p.segments - 1)
+      out = p.state_out + state_at + j * p.states;
+    if (out) {
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (lane * S + s < p.states) out[s] = h[j][s];
+    }
+    if (kStateOnly && lane == 0) {
+      const float2 q = unpack2(delta_sum[j]);
+      p.segment_delta[((int64_t)segment * p.batch + batch) * p.channels + ch.first + mine + j] = q.x + q.y;
+    }
   }
 }
 
@@ -349,8 +444,8 @@ __device__ __forceinline__ float channel_sum(float (&v)[8], int lane_in_warp) {
 // transposed butterflies; the warps' parts of dB and dC go through shared memory, the blocks' through
 // global memory, all in a fixed order.
 template <typename T, int kBlocks>
-__global__ void __launch_bounds__(kThreads, 2) selective_scan_backward_kernel(Params p) {
-  constexpr int S = 4, kLanes = 4, kChannels = kThreads / kLanes, kTile = 32, kWarps = kThreads / 32;
+__global__ void __launch_bounds__(kBackwardThreads, 2) selective_scan_backward_kernel(Params p) {
+  constexpr int S = 4, kLanes = 4, kChannels = kBackwardThreads / kLanes, kTile = 32, kWarps = kBackwardThreads / 32;
   constexpr int NP = 16 * kBlocks;
   constexpr int kHalf = kCheckpoint;
   extern __shared__ __align__(16) float smem[];
@@ -408,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 2) selective_scan_backward_kernel(Pa
   const int64_t checkpoint_rows = (p.length + kCheckpoint - 1) / kCheckpoint;
 
   Raw8<T> raw_x, raw_d, raw_z, raw_g;
-  SharedStates<T, kTile, NP> bc;
+  SharedStates<T, kTile, NP, kBackwardThreads> bc;
   auto fetch = [&](int t0) {
     const int t = t0 + row;
     const int n = t < live ? count : 0;
@@ -541,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 2) selective_scan_backward_kernel(Pa
       }
       __syncthreads();
       // the warps' parts of dB and dC of these sixteen states
-      for (int i = threadIdx.x; i < kTile * 2 * 16; i += kThreads) {
+      for (int i = threadIdx.x; i < kTile * 2 * 16; i += kBackwardThreads) {
         const int t = t0 + i / 32;
         if (t < end) {
           float sum = s_red[i];

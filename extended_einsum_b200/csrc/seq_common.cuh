@@ -141,6 +141,68 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Four consecutive elements: 8 bytes of a 16-bit type, 16 of float.  `whole`: one aligned load.
+template <typename T>
+struct Raw4 {
+  uint32_t w[sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ Raw4<T> load4_if(const T* p, bool in, int count, bool whole) {
+  Raw4<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T); ++i) r.w[i] = 0u;
+  if (whole) {
+    if (in) {
+      if constexpr (sizeof(T) == 2)
+        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "l"(p));
+      else
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3])
+                     : "l"(p));
+    }
+  } else if (in) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i < count) {
+        if constexpr (sizeof(T) == 2)
+          r.w[i / 2] |= (uint32_t) reinterpret_cast<const unsigned short*>(p)[i] << (16 * (i % 2));
+        else
+          r.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+      }
+    }
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float value4(const Raw4<T>& r, int i) {
+  if constexpr (__is_same(T, float))
+    return __uint_as_float(r.w[i]);
+  else if constexpr (__is_same(T, __nv_bfloat16))
+    return __uint_as_float(i % 2 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
+  else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i / 2]));
+    return i % 2 ? f.y : f.x;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int count, bool whole, const float (&v)[4]) {
+  if (whole) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if constexpr (__is_same(T, __nv_bfloat16)) {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+      *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+      const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+      *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < count) p[i] = from_f32<T>(v[i]);
+}
+
 // 2^x and 1/x of the special function unit: relative errors of 2^-22 and 2^-23.
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -155,18 +217,62 @@ __device__ __forceinline__ float rcp_fast(float x) {
 
 __device__ __forceinline__ float sigmoid(float v) { return rcp_fast(1.0f + exp2_fast(-kLog2e * v)); }
 
-// softplus(v) = max(v, 0) + log1p(u), u = exp(-|v|) in (0, 1].  log1p(u) = 2 artanh(s) with
-// s = u / (2 + u) <= 1/3, and artanh(s) / s is a polynomial of degree 4 in s^2 <= 1/9 (minimax,
-// relative error 4e-9): the logarithm instruction would lose the small results of negative v.
-__device__ __forceinline__ float softplus(float v) {
-  const float u = exp2_fast(-kLog2e * fabsf(v));
-  const float s = u * rcp_fast(2.0f + u);
-  const float q = s * s;
-  float p = fmaf(0.28178335f, q, 0.27960603f);
-  p = fmaf(p, q, 0.40024910f);
-  p = fmaf(p, q, 0.66666315f);
-  p = fmaf(p, q, 2.0f);
-  return (v > 0.0f || v != v ? v : 0.0f) + s * p;  // a NaN stays
+// Two float32 values in one register pair, for the packed arithmetic instructions.
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 pack2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(F2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 both(float v) { return pack2(v, v); }
+__device__ __forceinline__ F2 exp2_fast2(F2 v) {
+  const float2 f = unpack2(v);
+  return pack2(exp2_fast(f.x), exp2_fast(f.y));
+}
+
+// softplus(v) = max(v, 0) + log1p(u), u = exp(-|v|) in (0, 1].  log1p(u) / u is a polynomial of degree 8
+// (minimax on [0, 1], relative error 3e-8): the logarithm instruction would lose the small results of
+// negative v, and a reciprocal would cost the special function unit another turn.
+__device__ __forceinline__ F2 softplus2(F2 x) {
+  const float2 vw = unpack2(x);
+  const float v = vw.x, w = vw.y;
+  const F2 u = pack2(exp2_fast(-kLog2e * fabsf(v)), exp2_fast(-kLog2e * fabsf(w)));
+  F2 p = fma2(both(5.2326941e-3f), u, both(-2.9505240e-2f));
+  p = fma2(p, u, both(7.8225940e-2f));
+  p = fma2(p, u, both(-0.13663246f));
+  p = fma2(p, u, both(0.19106007f));
+  p = fma2(p, u, both(-0.24842982f));
+  p = fma2(p, u, both(0.33319098f));
+  p = fma2(p, u, both(-0.49999493f));
+  p = fma2(p, u, both(0.99999994f));
+  return fma2(p, u, pack2(fmaxf(v, 0.0f), fmaxf(w, 0.0f)));  // a NaN stays, in u
+}
+__device__ __forceinline__ float softplus(float v) { return unpack2(softplus2(both(v))).x; }
+
+// The gate v silu(z) of a pair.
+__device__ __forceinline__ F2 gate2(F2 v, F2 z) {
+  const float2 d = unpack2(add2(exp2_fast2(mul2(z, both(-kLog2e))), both(1.0f)));
+  return mul2(v, mul2(z, pack2(rcp_fast(d.x), rcp_fast(d.y))));
 }
 
 // Length of sequence i of a ragged batch, clamped to [0, most]; `lengths` may be null (all whole).

@@ -228,7 +228,7 @@ int scan_blocks(int64_t states) { return states <= 16 ? 1 : states <= 32 ? 2 : 4
 
 struct ScanPlan {
   int segments, segment_length;
-  int64_t channel_blocks;
+  int64_t channel_blocks;  // of the backward kernel: 32 channels
 };
 
 // How many segments the length is split into.  A split costs a pass of its own over x, delta and B, so
@@ -269,7 +269,8 @@ xe_status check_scan(const char* what, const xe_selective_scan_args* q, bool ste
   return XE_OK;
 }
 
-ScanParams scan_params(const xe_selective_scan_args* q) {
+// `bytes`: what a kernel's vector loads need rows to be aligned to.
+ScanParams scan_params(const xe_selective_scan_args* q, int64_t bytes) {
   ScanParams p{};
   p.x = q->x, p.delta = q->delta, p.z = q->z, p.b = q->b, p.c = q->c, p.y = q->y;
   p.a = q->a, p.d = q->d, p.bias = q->delta_bias;
@@ -283,12 +284,12 @@ ScanParams scan_params(const xe_selective_scan_args* q) {
   p.states = (int)q->states, p.groups = (int)q->groups;
   p.softplus = q->softplus;
   const int64_t each = q->channels / q->groups;  // a group's first channel starts a vector
-  p.vec = (vectors(q->x, q->dtype, {q->x_sb, q->x_st, each}) ? 1 : 0) |
-          (vectors(q->delta, q->dtype, {q->delta_sb, q->delta_st, each}) ? 2 : 0) |
-          (vectors(q->z, q->dtype, {q->z_sb, q->z_st, each}) ? 4 : 0) |
-          (vectors(q->y, q->dtype, {q->channels, each}) ? 8 : 0) |
-          (vectors(q->b, q->dtype, {q->b_sb, q->b_st, q->b_sg}) ? 16 : 0) |
-          (vectors(q->c, q->dtype, {q->c_sb, q->c_st, q->c_sg}) ? 32 : 0);
+  p.vec = (aligned(bytes, q->x, q->dtype, {q->x_sb, q->x_st, each}) ? 1 : 0) |
+          (aligned(bytes, q->delta, q->dtype, {q->delta_sb, q->delta_st, each}) ? 2 : 0) |
+          (aligned(bytes, q->z, q->dtype, {q->z_sb, q->z_st, each}) ? 4 : 0) |
+          (aligned(bytes, q->y, q->dtype, {q->channels, each}) ? 8 : 0) |
+          (aligned(bytes, q->b, q->dtype, {q->b_sb, q->b_st, q->b_sg}) ? 16 : 0) |
+          (aligned(bytes, q->c, q->dtype, {q->c_sb, q->c_st, q->c_sg}) ? 32 : 0);
   return p;
 }
 
@@ -303,15 +304,17 @@ void scan_segments(ScanParams& p, const ScanPlan& plan, void* workspace) {
 template <xe::scan::Mode kMode>
 xe_status launch_scan(const ScanParams& p, const ScanPlan& plan, int32_t dtype, cudaStream_t stream) {
   using namespace xe::scan;
-  const dim3 grid((unsigned)plan.channel_blocks, (unsigned)p.batch, (unsigned)(kMode == kFull ? p.segments : p.segments - 1));
+  const int kC = p.states <= 32 ? 2 : 1;
+  const int64_t blocks = (int64_t)p.groups * ceil_div(p.channels / p.groups, 8 * kC);
+  const dim3 grid((unsigned)blocks, (unsigned)p.batch, (unsigned)(kMode == kFull ? p.segments : p.segments - 1));
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
     if (p.states <= 16)
-      selective_scan_kernel<T, 4, 4, kMode><<<grid, kThreads, 0, stream>>>(p);
+      selective_scan_kernel<T, 4, 2, kMode><<<grid, 32, 0, stream>>>(p);
     else if (p.states <= 32)
-      selective_scan_kernel<T, 8, 4, kMode><<<grid, kThreads, 0, stream>>>(p);
+      selective_scan_kernel<T, 8, 2, kMode><<<grid, 32, 0, stream>>>(p);
     else
-      selective_scan_kernel<T, 16, 4, kMode><<<grid, kThreads, 0, stream>>>(p);
+      selective_scan_kernel<T, 16, 1, kMode><<<grid, 32, 0, stream>>>(p);
   });
   return launched("selective scan");
 }
@@ -337,7 +340,7 @@ xe_status launch_scan_backward(const ScanParams& p, const ScanPlan& plan, cudaSt
     done.fetch_or(1u << (dev & 31));
   }
   const dim3 grid((unsigned)plan.channel_blocks, (unsigned)p.batch, (unsigned)p.segments);
-  selective_scan_backward_kernel<T, kBlocks><<<grid, kThreads, kBytes, stream>>>(p);
+  selective_scan_backward_kernel<T, kBlocks><<<grid, kBackwardThreads, kBytes, stream>>>(p);
   return launched("selective scan backward");
 }
 
@@ -363,7 +366,7 @@ xe_status xe_selective_scan(const xe_selective_scan_args* q, void* workspace, si
   const ScanPlan plan = scan_plan(q->batch, q->length, q->channels, q->groups);
   if (workspace_bytes < scan_segment_bytes(plan, q->batch, q->channels, q->states) || (plan.segments > 1 && !workspace))
     return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
-  ScanParams p = scan_params(q);
+  ScanParams p = scan_params(q, 4 * size_of(q->dtype));  // four elements
   scan_segments(p, plan, workspace);
   if (p.segments > 1) {
     if (xe_status s = launch_scan<xe::scan::kStates>(p, plan, q->dtype, as_stream(stream))) return s;
@@ -377,7 +380,7 @@ xe_status xe_selective_scan_step(const xe_selective_scan_args* q, void* stream) 
   if (xe_status s = check_scan(what, q, true)) return s;
   if (q->batch == 0 || q->channels == 0) return XE_OK;
   if (!q->y || !q->state_out) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
-  ScanParams p = scan_params(q);
+  ScanParams p = scan_params(q, 4 * size_of(q->dtype));  // four elements
   // bit 3: states and A in groups of four
   p.vec = reinterpret_cast<uintptr_t>(q->state_out) % 16 == 0 && reinterpret_cast<uintptr_t>(q->a) % 16 == 0 ? 8 : 0;
   constexpr int kLanes = 4;
@@ -411,7 +414,7 @@ xe_status xe_selective_scan_backward(const xe_selective_scan_args* q, const xe_s
   if (!workspace || workspace_bytes < xe_selective_scan_backward_workspace_size(q->batch, q->length, q->channels, q->states, q->groups))
     return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
   const ScanPlan plan = scan_plan(q->batch, q->length, q->channels, q->groups);
-  ScanParams p = scan_params(q);
+  ScanParams p = scan_params(q, 16);  // eight elements in loads of 16 bytes
   scan_segments(p, plan, workspace);
   p.dy = g->dy, p.dy_sb = g->dy_sb, p.dy_st = g->dy_st, p.dstate_out = g->dstate_out, p.dstate = g->dstate;
   p.dx = g->dx, p.ddelta = g->ddelta, p.dz = g->dz;
@@ -644,25 +647,47 @@ template <typename X, int kTiles, bool kSplit>
 xe_status launch_int4(xe::int4::Params& p, int64_t rows, cudaStream_t stream) {
   using namespace xe::int4;
   constexpr int kRing = kWarps * kStages * kStageBytes;
-  constexpr int kBudget = 65536;
-  const int64_t whole = ceil_div(p.inputs, kStageK) * kStageK;
-  p.chunk = (int)std::min<int64_t>(whole, kBudget / (kTiles * 8 * 2) / kStageK * kStageK);
+  constexpr int kBudget = 72 * 1024;  // of the staged activations: two blocks to an SM
+  const int64_t columns = (int64_t)p.tokens * p.pieces;
+  const int64_t whole = ceil_div(p.inputs, kStageK);  // stages
+  const int64_t fit = std::max<int64_t>(1, (kBudget / (columns * 2) - 32) / kStageK);
+  // the smallest cluster whose blocks hold their part of k at once
+  int64_t parts = 1;
+  while (parts < 8 && ceil_div(whole, parts) > fit) parts *= 2;
+  const int64_t part = ceil_div(whole, parts);  // the last blocks may have less, or none
+  p.part = (int)(part * kStageK);
+  p.chunk = (int)(std::min(part, fit) * kStageK);
   p.pitch = p.chunk + 32;  // bytes: 64 past a multiple of 128, two columns' reads in different banks
-  p.warps_k = kTiles == 1 ? 8 : kTiles == 2 ? 4 : 2;
-  const int bytes = kRing + kTiles * 8 * p.pitch * 2;
-  constexpr int kMost = kRing + kBudget + kTiles * 8 * 32 * 2;
+  // rows of a block: enough that staging the activations stays small beside reading their weights, fewer where the
+  // device would have blocks for half its multiprocessors only
+  int rows_m = 1;
+  while (rows_m < 8 && 16 * rows_m < 4 * columns && ceil_div(p.outputs, 32 * rows_m) * parts >= 148) rows_m *= 2;
+  p.warps_k = kWarps / rows_m;
+  const int bytes = kRing + 16 + (int)columns * p.pitch * 2;
+  constexpr int kMost = kRing + kBudget + 16 * 1024;
   static std::atomic<uint32_t> done{0};
+  auto kernel = int4_linear_kernel<X, kTiles, kSplit, kStages>;
   int dev = 0;
   cudaGetDevice(&dev);
   if (!(done.load() >> (dev & 31) & 1u)) {
-    const cudaError_t e = cudaFuncSetAttribute(int4_linear_kernel<X, kTiles, kSplit, kStages>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
     if (e != cudaSuccess) return fail(XE_ERR_CUDA, "xe_int4_linear: %s", cudaGetErrorString(e));
     done.fetch_or(1u << (dev & 31));
   }
   const int per_block = 16 * (kWarps / p.warps_k);
-  const dim3 grid((unsigned)ceil_div(p.outputs, per_block), (unsigned)ceil_div(rows, p.tokens));
-  int4_linear_kernel<X, kTiles, kSplit, kStages><<<grid, kWarps * 32, bytes, stream>>>(p);
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)parts, (unsigned)ceil_div(p.outputs, per_block), (unsigned)ceil_div(rows, p.tokens));
+  config.blockDim = dim3(kWarps * 32);
+  config.dynamicSmemBytes = bytes;
+  config.stream = stream;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = (unsigned)parts;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = parts > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, p);
+  if (e != cudaSuccess) return fail(XE_ERR_CUDA, "xe_int4_linear: %s", cudaGetErrorString(e));
   return launched("xe_int4_linear");
 }
 
@@ -701,7 +726,7 @@ xe_status xe_int4_linear(const void* x, int64_t x_row, const float* x_scale, con
   if (group % 32) return fail(XE_ERR_NOT_SUPPORTED, "%s: groups of %lld, not a multiple of 32", what, (long long)group);
   if (reinterpret_cast<uintptr_t>(packed) % 16 || packed_row % 16)
     return fail(XE_ERR_INVALID_ARGUMENT, "%s: rows of codes must start on 16-byte boundaries", what);
-  if (rows > INT_MAX / 4 || inputs > INT_MAX / 4 || outputs > INT_MAX / 4 || ceil_div(rows, 21) > 65535)
+  if (rows > INT_MAX / 4 || inputs > INT_MAX / 4 || outputs > 65535 * 16 || ceil_div(rows, 21) > 65535)
     return fail(XE_ERR_NOT_SUPPORTED, "%s: a size is above its limit", what);
   if (rows == 0 || outputs == 0) return XE_OK;
   xe::int4::Params p{};
@@ -711,6 +736,7 @@ xe_status xe_int4_linear(const void* x, int64_t x_row, const float* x_scale, con
   p.rows = (int)rows, p.inputs = (int)inputs, p.outputs = (int)outputs, p.group = (int)group;
   p.scale_dtype = scale_dtype, p.y_dtype = y_dtype;
   p.pieces = x_dtype == XE_F32 ? 3 : 1;
+  p.x_vec = aligned(size_of(x_dtype) == 1 ? 8 : 16, x, x_dtype, {x_row});
   cudaStream_t st = as_stream(stream);
   switch (x_dtype) {
     case XE_F32: return run_int4<float>(p, st);
