@@ -285,9 +285,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _c_i32,
         [
             _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr,  # x, row, x_scale, packed, row, scales, zeros, y
-            _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_ptr,  # rows, inputs, outputs, group, types, stream
+            _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32,  # rows, inputs, outputs, group, types
+            _c_ptr, _c_size, _c_ptr,  # workspace, bytes, stream
         ],
     ),
+    "xe_int4_linear_workspace_size": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i32]),
 }
 
 _lock = threading.Lock()

@@ -14,10 +14,11 @@
 // codes gives the pairs (0, 4), (1, 5), (2, 6), (3, 7) by masking and shifting, so the activations
 // are staged in that order.
 //
-// A block holds a part of k of the activations in shared memory (the blocks of a cluster share the rows and
-// split k between them, so that a part fits), its warps take row tiles of sixteen and every so many stages of
-// 128 k, each with a ring of its own that cp.async fills.  Partial sums meet in shared memory, the warps' first
-// and then the cluster's, in a fixed order.
+// Warps work alone: a unit of work is a tile of sixteen rows over a run of k, and a warp takes every so many
+// units, its ring of stages (128 k of sixteen rows, filled by cp.async) running on from one unit to the next, so
+// that the reads never pause for a barrier.  A block only shares the staged activations: all of k, or, where that
+// does not fit, one part of it.  With more than one run of k, sums go to a workspace and a second kernel adds
+// them in order.
 #pragma once
 
 #include "seq_common.cuh"
@@ -30,7 +31,9 @@ using namespace seq;
 constexpr int kStageK = 128;                       // k of one ring stage: 64 bytes of each row
 constexpr int kRowPitch = 80;                      // bytes in the ring: 8 rows x 4 words in 32 banks
 constexpr int kStageBytes = 16 * kRowPitch;
+constexpr int kStages = 4;
 constexpr int kWarps = 8;
+constexpr int kZeroBytes = 4 * kStageK / 2;
 
 struct Params {
   const void* x;
@@ -39,16 +42,19 @@ struct Params {
   const void* scales;
   const uint8_t* zeros;  // or null
   void* y;
+  float* sums;  // (runs, columns of all tokens, outputs), or null where one run is all of k
   int64_t x_row, packed_row;  // strides of a row: elements, bytes
   int rows, inputs, outputs, group;
+  uint32_t group_magic;  // floor(2^32 / (group / 32)) + 1, or 0 for groups of 32
   int scale_dtype, y_dtype;
   int x_vec;    // rows of x start on 16-byte boundaries (8 bytes for 8-bit types)
   int pieces;   // columns of the product per token: 3 for float32 activations, else 1
   int tokens;   // tokens of one block
-  int part;     // k of one block of the cluster, a multiple of kStageK
-  int chunk;    // k staged at a time, a multiple of kStageK
+  int parts;    // parts of k that blocks hold, blockIdx.x % parts
+  int part;     // their stages
+  int runs;     // runs of a part
+  int run;      // their stages
   int pitch;    // of the staged activations, elements
-  int warps_k;  // warps along k; the others along rows
 };
 
 template <bool kHalf>
@@ -64,11 +70,17 @@ struct Arithmetic<false> {
     const __nv_bfloat162 v = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  // d = a b + c
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                             float c0, float c1, float c2, float c3) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+  }
+  // The four pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word, less the offset.
+  static __device__ __forceinline__ void expand(uint32_t w, uint32_t offset, uint32_t (&f)[4]) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) f[h] = sub(((w >> (4 * h)) & 0x000f000fu) | kMagic, offset);
   }
 };
 template <>
@@ -82,11 +94,27 @@ struct Arithmetic<true> {
     const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                             float c0, float c1, float c2, float c3) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+  }
+  // As above; the odd nibbles stay where they are and stand for sixteen times themselves, which a multiplication by
+  // 1/16 takes back exactly (64 + q, less 64 + z): two shifts fewer.
+  static __device__ __forceinline__ void expand(uint32_t w, uint32_t offset, uint32_t (&f)[4]) {
+    const uint32_t v = w >> 8;
+    const uint32_t offset16 = sub(0x63806380u, offset);  // 960 - (1024 + z) = -64 - z
+    f[0] = sub((w & 0x000f000fu) | kMagic, offset);
+    f[1] = fma16((w & 0x00f000f0u) | kMagic, offset16);
+    f[2] = sub((v & 0x000f000fu) | kMagic, offset);
+    f[3] = fma16((v & 0x00f000f0u) | kMagic, offset16);
+  }
+  // v / 16 + c
+  static __device__ __forceinline__ uint32_t fma16(uint32_t v, uint32_t c) {
+    const uint32_t k = 0x2c002c00u;  // 1/16
+    const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&v), *reinterpret_cast<const __half2*>(&k), *reinterpret_cast<__half2*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&r);
   }
 };
 
@@ -164,7 +192,6 @@ struct Eight {
   }
 };
 
-// A scale is loaded as its bits and converted where it is used: a conversion would wait for the load.
 __device__ __forceinline__ uint32_t load_scale(const void* p, int dtype, int64_t at) {
   return dtype == XE_F32 ? static_cast<const uint32_t*>(p)[at] : static_cast<const uint16_t*>(p)[at];
 }
@@ -174,16 +201,22 @@ __device__ __forceinline__ float scale_value(uint32_t bits, int dtype) {
                             : __half2float(__ushort_as_half((unsigned short)bits));
 }
 
-// All threads of the cluster, with what they have written to shared memory.
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+// The group of k = 32 u.  The product's high word is the exact quotient as long as u * (group / 32) < 2^32.
+__device__ __forceinline__ int group_of(const Params& p, int u) {
+  return p.group_magic ? (int)__umulhi((uint32_t)u, p.group_magic) : u;
 }
-// A float of block `rank`'s shared memory, at the place of `at` in this block's.
-__device__ __forceinline__ float cluster_load(const float* at, int rank) {
-  uint32_t remote;
-  float v;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void lds64(uint32_t at, float& v, uint32_t& w) {
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=f"(v), "=r"(w) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
   return v;
 }
 
@@ -196,204 +229,239 @@ __device__ __forceinline__ void store_as(void* y, int dtype, int64_t at, float v
     static_cast<__half*>(y)[at] = __float2half_rn(v);
 }
 
-// X: type of the activations; kTiles: columns / 8; kSplit: groups that are no multiple of 128, so that the
-// four 32s of a stage may differ in scale.
-template <typename X, int kTiles, bool kSplit, int kStages>
+// X: type of the activations; kTiles: columns / 8; kRun: how many 32s of a stage are sure to share a scale (1, 2
+// or 4, the largest that divides group / 32).
+template <typename X, int kTiles, int kRun>
 __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(const __grid_constant__ Params p) {
   constexpr bool kHalf = __is_same(X, __half) || sizeof(X) == 1;
   using A = Arithmetic<kHalf>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int quad = lane % 4, row8 = lane / 4;
-  const int warp_k = warp % p.warps_k, warp_m = warp / p.warps_k;
-  const int rows_per_block = 16 * (kWarps / p.warps_k);
-  const int o0 = blockIdx.y * rows_per_block + warp_m * 16;
-  const int m0 = blockIdx.z * p.tokens;
+  const int m0 = blockIdx.y * p.tokens;
   const int tokens = min(p.tokens, p.rows - m0);
   const int columns = tokens * p.pieces;
-  uint8_t* ring = smem + warp * (kStages * kStageBytes);
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-  uint8_t* xs = smem + kWarps * kStages * kStageBytes;  // 16 zero bytes, then the activations
+  const int part = blockIdx.x % p.parts;
+  const int stage0 = part * p.part;                                               // of this block's part
+  const int stage1 = min(stage0 + p.part, (p.inputs + kStageK - 1) / kStageK);
+  uint8_t* xs = smem + kWarps * kStages * kStageBytes;  // zero bytes for a stage of a column, then the activations
+  const uint32_t xs_at = (uint32_t)__cvta_generic_to_shared(xs);
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kStages * kStageBytes);
+  const uint32_t copy_to = ring_at + row8 * kRowPitch + quad * 16;
+  const uint32_t read_at = ring_at + row8 * kRowPitch + quad * 4;
   const int groups = p.inputs / p.group;
-  const int k_begin = blockIdx.x * p.part, k_end = min(k_begin + p.part, p.inputs);
-
-  // the two rows of this lane's fragments, copies and scales; past the last output all read the last one, and
-  // the results are dropped
   const int last_o = p.outputs - 1;
-  const int oa = min(o0 + row8, last_o), ob = min(o0 + row8 + 8, last_o);
-  const uint8_t* copy_a = p.packed + (int64_t)oa * p.packed_row + quad * 16;
-  const uint8_t* copy_b = p.packed + (int64_t)ob * p.packed_row + quad * 16;
-  const int64_t scales_a = (int64_t)oa * groups, scales_b = (int64_t)ob * groups;
-  // this lane's column of each tile of eight; those past the last read the zero bytes at every k
-  uint32_t column_at[kTiles];
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n)
-    column_at[n] = n * 8 + row8 < columns ? 16 + ((n * 8 + row8) * p.pitch + quad * 8) * 2 : 0;
-  if (threadIdx.x < 4) reinterpret_cast<uint32_t*>(xs)[threadIdx.x] = 0;
 
+  // this warp's units: (row tile, run of the part), every `stride`th
+  const int units = (p.outputs + 15) / 16 * p.runs;
+  const int stride = gridDim.x / p.parts * kWarps;
+  const int first = blockIdx.x / p.parts * kWarps + warp;
+
+  // the copying side: the next stage and where its rows and scales lie.  Rows past the last output read the last one.
+  int copy_unit = first, copy_stage = 0, copy_end = 0;
+  const uint8_t *from_a = nullptr, *from_b = nullptr;
+  int64_t scale_a = 0, scale_b = 0;
+  // The last part may have fewer stages than the others, and runs of none: they are passed over here, and
+  // their sums are zeros.
+  auto open_copy = [&] {
+    for (; copy_unit < units; copy_unit += stride) {
+      const int tile = copy_unit / p.runs, run = copy_unit - tile * p.runs;
+      copy_stage = stage0 + run * p.run;
+      copy_end = min(copy_stage + p.run, stage1);
+      if (copy_stage >= copy_end) continue;
+      const int oa = min(tile * 16 + row8, last_o), ob = min(tile * 16 + row8 + 8, last_o);
+      from_a = p.packed + oa * p.packed_row + (int64_t)copy_stage * (kStageK / 2) + quad * 16;
+      from_b = p.packed + ob * p.packed_row + (int64_t)copy_stage * (kStageK / 2) + quad * 16;
+      scale_a = (int64_t)oa * groups;
+      scale_b = (int64_t)ob * groups;
+      return;
+    }
+  };
+  // a stage's scales, loaded as bits: a conversion would wait for the load.  kRun < 4: lane `quad` holds those of
+  // the stage's 32s number `quad`.
+  uint32_t sa[kStages], sb[kStages], za[kStages], zb[kStages];
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) {
+    sa[i] = sb[i] = 0;
+    za[i] = zb[i] = 8;
+  }
+  auto issue = [&](int slot) {
+    if (copy_unit < units) {
+      if (copy_stage * kStageK + quad * 32 < p.inputs) {
+        cp_async16(copy_to + slot * kStageBytes, from_a);
+        cp_async16(copy_to + slot * kStageBytes + 8 * kRowPitch, from_b);
+        const int g = group_of(p, copy_stage * 4 + (kRun < 4 ? quad : 0));
+        sa[slot] = load_scale(p.scales, p.scale_dtype, scale_a + g);
+        sb[slot] = load_scale(p.scales, p.scale_dtype, scale_b + g);
+        if (p.zeros) {
+          za[slot] = p.zeros[scale_a + g];
+          zb[slot] = p.zeros[scale_b + g];
+        }
+      }
+      from_a += kStageK / 2;
+      from_b += kStageK / 2;
+      if (++copy_stage == copy_end) {
+        copy_unit += stride;
+        open_copy();
+      }
+    }
+    cp_async_commit();
+  };
+  open_copy();
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(i);
+
+  // stage the activations of the part, eight k at a time: the warps spread over the columns, and over k where
+  // there are fewer columns than warps
+  if (threadIdx.x < kZeroBytes / 4) reinterpret_cast<uint32_t*>(xs)[threadIdx.x] = 0;
+  {
+    const int k0 = stage0 * kStageK, kn = min(stage1 * kStageK, p.inputs) - k0;
+    const int across = columns > 4 ? 8 : columns > 2 ? 4 : columns > 1 ? 2 : 1;
+    const int along = kWarps / across;
+    for (int col = warp % across; col < columns; col += across) {
+      const X* from = static_cast<const X*>(p.x) + (int64_t)(m0 + col / p.pieces) * p.x_row + k0;
+      const int piece = p.pieces == 1 ? 0 : col % p.pieces;
+      uint8_t* to = xs + kZeroBytes + (int64_t)col * p.pitch * 2;
+      for (int k = (warp / across * 32 + lane) * 8; k < kn; k += along * 256 * 4) {
+        Eight<X> e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (k + j * along * 256 < kn) e[j].load(from + k + j * along * 256, p.x_vec);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (k + j * along * 256 < kn) *reinterpret_cast<uint4*>(to + (k + j * along * 256) * 2) = e[j].staged(piece);
+      }
+    }
+  }
+  __syncthreads();
+
+  // this lane's activations by tile of eight columns; lanes past the last column stay on the zeros
+  uint32_t x_base[kTiles], x_step[kTiles];
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+    const bool in = n * 8 + row8 < columns;
+    x_base[n] = xs_at + (in ? kZeroBytes + ((n * 8 + row8) * p.pitch + quad * 8) * 2 : 0);
+    x_step[n] = in ? kStageK * 2 : 0;
+  }
   float acc[kTiles][4];
+  int unit = first, stage = 0, end = 0, tile = 0, run = 0;
+  uint32_t x_at[kTiles];
+  auto close_unit = [&] {
 #pragma unroll
-  for (int n = 0; n < kTiles; ++n)
+    for (int n = 0; n < kTiles; ++n) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
-
-  for (int k0 = k_begin; k0 < k_end; k0 += p.chunk) {
-    const int kn = min(p.chunk, k_end - k0);
-    const int stages = (kn + kStageK - 1) / kStageK;
-    // this warp's stages of the chunk: warp_k, warp_k + warps_k, ...
-    const int own = warp_k < stages ? (stages - warp_k + p.warps_k - 1) / p.warps_k : 0;
-    uint32_t sa[kStages], sb[kStages], za[kStages], zb[kStages];
-    auto issue = [&](int i, int slot) {
-      if (i < own) {
-        const int k = k0 + (warp_k + i * p.warps_k) * kStageK;
-        if (k + quad * 32 < k_end) {
-          const uint32_t at = ring_at + slot * kStageBytes + row8 * kRowPitch + quad * 16;
-          cp_async16(at, copy_a + k / 2);
-          cp_async16(at + 8 * kRowPitch, copy_b + k / 2);
-        }
-        // kSplit: lane `quad` holds the scales of the stage's 32s number `quad`
-        const int kk = k + (kSplit ? quad * 32 : 0);
-        if (kk < k_end) {
-          const int g = kk / p.group;
-          sa[slot] = load_scale(p.scales, p.scale_dtype, scales_a + g);
-          sb[slot] = load_scale(p.scales, p.scale_dtype, scales_b + g);
-          if (p.zeros) {
-            za[slot] = p.zeros[scales_a + g];
-            zb[slot] = p.zeros[scales_b + g];
+      for (int i = 0; i < 4; ++i) {
+        const int col = n * 8 + quad * 2 + i % 2, o = tile * 16 + row8 + i / 2 * 8;
+        if (col < columns && o <= last_o) {
+          if (p.sums) {
+            const int64_t all = (int64_t)p.rows * p.pieces;
+            p.sums[((int64_t)(part * p.runs + run) * all + (int64_t)m0 * p.pieces + col) * p.outputs + o] = acc[n][i];
+          } else {
+            const float v = p.x_scale ? acc[n][i] * p.x_scale[m0 + col] : acc[n][i];
+            store_as(p.y, p.y_dtype, (int64_t)(m0 + col) * p.outputs + o, v);
           }
         }
       }
-      cp_async_commit();
+    }
+  };
+  auto open_unit = [&] {
+    for (; unit < units; unit += stride) {
+      tile = unit / p.runs, run = unit - tile * p.runs;
+      stage = stage0 + run * p.run;
+      end = min(stage + p.run, stage1);
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        x_at[n] = x_base[n] + (stage - stage0) * x_step[n];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+      }
+      if (stage < end) return;
+      close_unit();
+    }
+  };
+  auto work = [&](int slot) {
+    float sum[kTiles][4];
+    const float first_a = scale_value(sa[slot], p.scale_dtype), first_b = scale_value(sb[slot], p.scale_dtype);
+    const uint32_t offset_a = A::offset((float)za[slot]), offset_b = A::offset((float)zb[slot]);
+    float scale_a = first_a, scale_b = first_b;
+    uint32_t off_a = offset_a, off_b = offset_b;
+    auto group32 = [&](int j, bool start, bool last) {
+      if (kRun < 4 && start) {
+        scale_a = __shfl_sync(0xffffffffu, first_a, j, 4);
+        scale_b = __shfl_sync(0xffffffffu, first_b, j, 4);
+        if (p.zeros) {
+          off_a = __shfl_sync(0xffffffffu, offset_a, j, 4);
+          off_b = __shfl_sync(0xffffffffu, offset_b, j, 4);
+        }
+      }
+      const uint32_t at = read_at + slot * kStageBytes + j * 16;
+      uint32_t fa[4], fb[4];
+      A::expand(lds32(at), off_a, fa);
+      A::expand(lds32(at + 8 * kRowPitch), off_b, fb);
+      const uint32_t f0[4] = {fa[0], fb[0], fa[1], fb[1]}, f1[4] = {fa[2], fb[2], fa[3], fb[3]};
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        const uint4 b = lds128(x_at[n] + j * 64);
+        if (start)
+          A::mma(sum[n], f0, b.x, b.y, 0.0f, 0.0f, 0.0f, 0.0f);
+        else
+          A::mma(sum[n], f0, b.x, b.y, sum[n][0], sum[n][1], sum[n][2], sum[n][3]);
+        A::mma(sum[n], f1, b.z, b.w, sum[n][0], sum[n][1], sum[n][2], sum[n][3]);
+        if (last) {
+          acc[n][0] = fmaf(scale_a, sum[n][0], acc[n][0]);
+          acc[n][1] = fmaf(scale_a, sum[n][1], acc[n][1]);
+          acc[n][2] = fmaf(scale_b, sum[n][2], acc[n][2]);
+          acc[n][3] = fmaf(scale_b, sum[n][3], acc[n][3]);
+        }
+      }
     };
+    const int left = p.inputs - stage * kStageK;
+    if (left >= kStageK) {
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) {
-      sa[i] = sb[i] = 0;
-      za[i] = zb[i] = 8;
+      for (int j = 0; j < 4; ++j) group32(j, j % kRun == 0, j % kRun == kRun - 1);
+    } else {
+#pragma unroll 1
+      for (int j = 0; j * 32 < left; ++j) group32(j, true, true);
     }
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(i, i);
-    // stage the activations, eight k at a time: the warps spread over the columns, and over k where there are
-    // fewer columns than warps
-    if (k0 > k_begin) __syncthreads();
-    {
-      const int across = columns > 4 ? 8 : columns > 2 ? 4 : columns > 1 ? 2 : 1;
-      const int along = kWarps / across;
-      for (int col = warp % across; col < columns; col += across) {
-        const X* from = static_cast<const X*>(p.x) + (int64_t)(m0 + col / p.pieces) * p.x_row + k0;
-        const int piece = p.pieces == 1 ? 0 : col % p.pieces;
-        uint8_t* to = xs + 16 + (int64_t)col * p.pitch * 2;
-        for (int k = (warp / across * 32 + lane) * 8; k < kn; k += along * 256 * 4) {
-          Eight<X> e[4];
+    for (int n = 0; n < kTiles; ++n) x_at[n] += x_step[n];
+  };
+  open_unit();
+  while (unit < units) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (k + j * along * 256 < kn) e[j].load(from + k + j * along * 256, p.x_vec);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (k + j * along * 256 < kn) *reinterpret_cast<uint4*>(to + (k + j * along * 256) * 2) = e[j].staged(piece);
-        }
-      }
-    }
-    __syncthreads();
-    for (int i0 = 0; i0 < own; i0 += kStages) {
-#pragma unroll
-      for (int slot = 0; slot < kStages; ++slot) {
-        const int i = i0 + slot;
-        if (i < own) {
-          issue(i + kStages - 1, (slot + kStages - 1) % kStages);
-          cp_async_wait<kStages - 1>();
-          __syncwarp();
-          const int k = (warp_k + i * p.warps_k) * kStageK;  // inside the chunk
-          const uint8_t* stage = ring + slot * kStageBytes + row8 * kRowPitch + quad * 4;
-          float part[kTiles][4];
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) part[n][j] = 0.0f;
-          const float first_a = scale_value(sa[slot], p.scale_dtype), first_b = scale_value(sb[slot], p.scale_dtype);
-          const uint32_t offset_a = A::offset((float)za[slot]), offset_b = A::offset((float)zb[slot]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (k + j * 32 < kn) {
-              float scale_a = first_a, scale_b = first_b;
-              uint32_t off_a = offset_a, off_b = offset_b;
-              if (kSplit) {
-                scale_a = __shfl_sync(0xffffffffu, scale_a, j, 4);
-                scale_b = __shfl_sync(0xffffffffu, scale_b, j, 4);
-                off_a = __shfl_sync(0xffffffffu, off_a, j, 4);
-                off_b = __shfl_sync(0xffffffffu, off_b, j, 4);
-              }
-              const uint32_t wa = *reinterpret_cast<const uint32_t*>(stage + j * 16);
-              const uint32_t wb = *reinterpret_cast<const uint32_t*>(stage + 8 * kRowPitch + j * 16);
-              uint32_t f[2][4];
-#pragma unroll
-              for (int h = 0; h < 4; ++h) {
-                const uint32_t qa = ((wa >> (4 * h)) & 0x000f000fu) | A::kMagic;
-                const uint32_t qb = ((wb >> (4 * h)) & 0x000f000fu) | A::kMagic;
-                f[h / 2][(h % 2) * 2] = A::sub(qa, off_a);
-                f[h / 2][(h % 2) * 2 + 1] = A::sub(qb, off_b);
-              }
-#pragma unroll
-              for (int n = 0; n < kTiles; ++n) {
-                const uint32_t at = column_at[n] ? column_at[n] + (k + j * 32) * 2 : 0;
-                const uint4 b = *reinterpret_cast<const uint4*>(xs + at);
-                A::mma(part[n], f[0], b.x, b.y);
-                A::mma(part[n], f[1], b.z, b.w);
-              }
-              if (kSplit || j == 3 || k + (j + 1) * 32 >= kn) {
-#pragma unroll
-                for (int n = 0; n < kTiles; ++n) {
-                  acc[n][0] = fmaf(scale_a, part[n][0], acc[n][0]);
-                  acc[n][1] = fmaf(scale_a, part[n][1], acc[n][1]);
-                  acc[n][2] = fmaf(scale_b, part[n][2], acc[n][2]);
-                  acc[n][3] = fmaf(scale_b, part[n][3], acc[n][3]);
-#pragma unroll
-                  for (int q = 0; q < 4; ++q) part[n][q] = 0.0f;
-                }
-              }
-            }
-          }
-          __syncwarp();  // the slot is free for the next copies
+    for (int slot = 0; slot < kStages; ++slot) {
+      if (unit < units) {
+        issue((slot + kStages - 1) % kStages);
+        cp_async_wait<kStages - 1>();
+        __syncwarp();
+        work(slot);
+        __syncwarp();  // the slot is free for the next copies
+        if (++stage == end) {
+          close_unit();
+          unit += stride;
+          open_unit();
         }
       }
     }
   }
   cp_async_wait<0>();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
-  // sums over the warps of a row tile and then over the blocks of the cluster, in order
-  __syncthreads();
-  constexpr int kCols = kTiles * 8 + 1;
-  float* red = reinterpret_cast<float*>(smem);  // [warp][16 rows][columns + 1]
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      red[(warp * 16 + row8 + (i / 2) * 8) * kCols + n * 8 + quad * 2 + (i % 2)] = acc[n][i];
-  const int parts = gridDim.x;
-  __syncwarp();
-  if (parts > 1)
-    cluster_barrier();
-  else
-    __syncthreads();
-  for (int i = threadIdx.x + blockIdx.x * (kWarps * 32); i < rows_per_block * tokens; i += parts * (kWarps * 32)) {
-    const int r = i % rows_per_block, m = i / rows_per_block;
-    const int o = blockIdx.y * rows_per_block + r;
-    if (o >= p.outputs) continue;
-    float sum = 0.0f;
-    for (int piece = p.pieces - 1; piece >= 0; --piece) {
-      for (int b = 0; b < parts; ++b) {
-        for (int w = 0; w < p.warps_k; ++w) {
-          const float* at = red + (((r / 16) * p.warps_k + w) * 16 + r % 16) * kCols + m * p.pieces + piece;
-          sum += parts > 1 ? cluster_load(at, b) : *at;
-        }
-      }
-    }
-    if (p.x_scale) sum *= p.x_scale[m0 + m];
-    store_as(p.y, p.y_dtype, (int64_t)(m0 + m) * p.outputs + o, sum);
+// y from the runs' sums, in order; the parts of a float32 activation from the smallest on.
+__global__ void __launch_bounds__(256) int4_sum_kernel(const __grid_constant__ Params p, int runs) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int o = blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
+  if (o >= p.outputs) return;
+  const int64_t all = (int64_t)p.rows * p.pieces;
+  float sum = 0.0f;
+  for (int piece = p.pieces - 1; piece >= 0; --piece) {
+    const float* at = p.sums + ((int64_t)m * p.pieces + piece) * p.outputs + o;
+#pragma unroll 4
+    for (int r = 0; r < runs; ++r) sum += at[r * all * p.outputs];
   }
-  if (parts > 1) {  // no block leaves while its sums are read
-    __syncwarp();
-    cluster_barrier();
-  }
+  if (p.x_scale) sum *= p.x_scale[m];
+  store_as(p.y, p.y_dtype, (int64_t)m * p.outputs + o, sum);
 }
 
 }  // namespace int4

@@ -641,79 +641,113 @@ xe_status xe_rms_norm_backward(const void* sum, int64_t sum_row, const void* add
 
 namespace {
 
-constexpr int kStages = 4;
+struct Int4Plan {
+  int tokens, tiles;  // tokens of a block, and their columns in eights
+  int parts, part, runs, run, pitch;
+  int bytes, blocks;  // shared memory; blocks in x
+};
 
-template <typename X, int kTiles, bool kSplit>
-xe_status launch_int4(xe::int4::Params& p, int64_t rows, cudaStream_t stream) {
+// How the work is cut: k into the parts that fit a block's shared memory, and these into runs, so that the
+// device's warps get equally many stages each.  A unit of work costs its stages and about four more for its
+// start and its sums, a warp alone needs about three times the issue slots of its instructions, and the device
+// takes 592 warps' instructions at a time.
+Int4Plan int4_plan(int64_t rows, int64_t inputs, int64_t outputs, int pieces) {
   using namespace xe::int4;
+  Int4Plan q;
+  q.tokens = (int)std::min<int64_t>(rows, 64 / pieces);
+  const int columns = q.tokens * pieces;
+  q.tiles = columns <= 8 ? 1 : columns <= 16 ? 2 : columns <= 32 ? 4 : 8;
   constexpr int kRing = kWarps * kStages * kStageBytes;
-  constexpr int kBudget = 72 * 1024;  // of the staged activations: two blocks to an SM
-  const int64_t columns = (int64_t)p.tokens * p.pieces;
-  const int64_t whole = ceil_div(p.inputs, kStageK);  // stages
-  const int64_t fit = std::max<int64_t>(1, (kBudget / (columns * 2) - 32) / kStageK);
-  // the smallest cluster whose blocks hold their part of k at once
-  int64_t parts = 1;
-  while (parts < 8 && ceil_div(whole, parts) > fit) parts *= 2;
-  const int64_t part = ceil_div(whole, parts);  // the last blocks may have less, or none
-  p.part = (int)(part * kStageK);
-  p.chunk = (int)(std::min(part, fit) * kStageK);
-  p.pitch = p.chunk + 32;  // bytes: 64 past a multiple of 128, two columns' reads in different banks
-  // rows of a block: enough that staging the activations stays small beside reading their weights, fewer where the
-  // device would have blocks for half its multiprocessors only
-  int rows_m = 1;
-  while (rows_m < 8 && 16 * rows_m < 4 * columns && ceil_div(p.outputs, 32 * rows_m) * parts >= 148) rows_m *= 2;
-  p.warps_k = kWarps / rows_m;
-  const int bytes = kRing + 16 + (int)columns * p.pitch * 2;
-  constexpr int kMost = kRing + kBudget + 16 * 1024;
+  // three blocks to a multiprocessor, two, or one, as the columns (and with them the registers) grow
+  const int each = q.tiles <= 2 ? 3 : q.tiles == 4 ? 2 : 1;
+  const int budget = 225 * 1024 / each - 1024 - kRing - kZeroBytes;
+  const int64_t stages = ceil_div(inputs, kStageK);
+  const int64_t fit = std::max<int64_t>(1, (budget / (columns * 2) - 32) / kStageK);
+  q.parts = (int)ceil_div(stages, fit);
+  q.part = (int)ceil_div(stages, q.parts);
+  q.parts = (int)ceil_div(stages, q.part);
+  q.pitch = q.part * kStageK + 32;  // bytes: 64 past a multiple of 128, two columns' reads in different banks
+  q.bytes = kRing + kZeroBytes + columns * q.pitch * 2;
+  const int64_t blocks = ceil_div(rows, q.tokens);  // in y
+  const int64_t workers = std::max<int64_t>(1, 148 * each / (q.parts * blocks));
+  const int64_t rows16 = ceil_div(outputs, 16);
+  int64_t best = INT64_MAX;
+  q.runs = 1, q.run = q.part;
+  for (int64_t runs = 1; runs <= 16 && runs <= q.part; ++runs) {
+    const int64_t run = ceil_div(q.part, runs);
+    if (ceil_div(q.part, run) != runs) continue;
+    const int64_t units = rows16 * runs;
+    const int64_t cost = (run + 4) * std::max(3 * ceil_div(units, workers * kWarps), ceil_div(units * q.parts * blocks, 592));
+    if (cost < best) best = cost, q.runs = (int)runs, q.run = (int)run;
+  }
+  q.blocks = (int)(q.parts * std::min<int64_t>(workers, ceil_div(rows16 * q.runs, kWarps)));
+  return q;
+}
+
+template <typename X, int kTiles, int kRun>
+xe_status launch_int4(const xe::int4::Params& p, const Int4Plan& plan, cudaStream_t stream) {
+  using namespace xe::int4;
   static std::atomic<uint32_t> done{0};
-  auto kernel = int4_linear_kernel<X, kTiles, kSplit, kStages>;
+  auto kernel = int4_linear_kernel<X, kTiles, kRun>;
   int dev = 0;
   cudaGetDevice(&dev);
   if (!(done.load() >> (dev & 31) & 1u)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     if (e != cudaSuccess) return fail(XE_ERR_CUDA, "xe_int4_linear: %s", cudaGetErrorString(e));
     done.fetch_or(1u << (dev & 31));
   }
-  const int per_block = 16 * (kWarps / p.warps_k);
+  const dim3 grid((unsigned)plan.blocks, (unsigned)ceil_div(p.rows, p.tokens));
+  kernel<<<grid, kWarps * 32, plan.bytes, stream>>>(p);
+  if (xe_status s = launched("xe_int4_linear")) return s;
+  if (!p.sums) return XE_OK;
+  // the second kernel's blocks may start while the first one ends; they wait for its results themselves
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3((unsigned)parts, (unsigned)ceil_div(p.outputs, per_block), (unsigned)ceil_div(rows, p.tokens));
-  config.blockDim = dim3(kWarps * 32);
-  config.dynamicSmemBytes = bytes;
+  config.gridDim = dim3((unsigned)ceil_div(p.outputs, 256), (unsigned)p.rows);
+  config.blockDim = dim3(256);
   config.stream = stream;
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = (unsigned)parts;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  config.attrs = &cluster;
-  config.numAttrs = parts > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, p);
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, int4_sum_kernel, p, plan.parts * plan.runs);
   if (e != cudaSuccess) return fail(XE_ERR_CUDA, "xe_int4_linear: %s", cudaGetErrorString(e));
   return launched("xe_int4_linear");
 }
 
 template <typename X>
-xe_status run_int4(xe::int4::Params& p, cudaStream_t stream) {
-  const int most = 64 / p.pieces;  // tokens of a block
-  p.tokens = std::min(p.rows, most);
-  const int columns = p.tokens * p.pieces;
-  const bool split = p.group % xe::int4::kStageK != 0;
+xe_status run_int4(const xe::int4::Params& p, const Int4Plan& plan, cudaStream_t stream) {
+  const int units = p.group / 32;
   auto go = [&](auto tiles) {
     constexpr int n = decltype(tiles)::value;
-    return split ? launch_int4<X, n, true>(p, p.rows, stream) : launch_int4<X, n, false>(p, p.rows, stream);
+    return units % 4 == 0   ? launch_int4<X, n, 4>(p, plan, stream)
+           : units % 2 == 0 ? launch_int4<X, n, 2>(p, plan, stream)
+                            : launch_int4<X, n, 1>(p, plan, stream);
   };
-  if (columns <= 8) return go(std::integral_constant<int, 1>{});
-  if (columns <= 16) return go(std::integral_constant<int, 2>{});
-  if (columns <= 32) return go(std::integral_constant<int, 4>{});
-  return go(std::integral_constant<int, 8>{});
+  switch (plan.tiles) {
+    case 1: return go(std::integral_constant<int, 1>{});
+    case 2: return go(std::integral_constant<int, 2>{});
+    case 4: return go(std::integral_constant<int, 4>{});
+    default: return go(std::integral_constant<int, 8>{});
+  }
 }
 
 }  // namespace
 
 extern "C" {
 
+size_t xe_int4_linear_workspace_size(int64_t rows, int64_t inputs, int64_t outputs, int32_t x_dtype) {
+  if (rows <= 0 || inputs < 1 || outputs <= 0 || inputs > 1 << 20) return 0;
+  const int pieces = x_dtype == XE_F32 ? 3 : 1;
+  const Int4Plan plan = int4_plan(rows, inputs, outputs, pieces);
+  const int64_t runs = (int64_t)plan.parts * plan.runs;
+  return runs == 1 && pieces == 1 ? 0 : padded((size_t)(runs * rows * pieces * outputs) * 4);
+}
+
 xe_status xe_int4_linear(const void* x, int64_t x_row, const float* x_scale, const void* packed, int64_t packed_row,
                          const void* scales, const void* zeros, void* y, int64_t rows, int64_t inputs, int64_t outputs,
-                         int64_t group, int32_t x_dtype, int32_t scale_dtype, int32_t y_dtype, void* stream) {
+                         int64_t group, int32_t x_dtype, int32_t scale_dtype, int32_t y_dtype, void* workspace,
+                         size_t workspace_bytes, void* stream) {
   const char* what = "xe_int4_linear";
   if (rows * outputs != 0 && (!x || !packed || !scales || !y))
     return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
@@ -726,7 +760,7 @@ xe_status xe_int4_linear(const void* x, int64_t x_row, const float* x_scale, con
   if (group % 32) return fail(XE_ERR_NOT_SUPPORTED, "%s: groups of %lld, not a multiple of 32", what, (long long)group);
   if (reinterpret_cast<uintptr_t>(packed) % 16 || packed_row % 16)
     return fail(XE_ERR_INVALID_ARGUMENT, "%s: rows of codes must start on 16-byte boundaries", what);
-  if (rows > INT_MAX / 4 || inputs > INT_MAX / 4 || outputs > 65535 * 16 || ceil_div(rows, 21) > 65535)
+  if (rows > INT_MAX / 4 || inputs > 1 << 20 || outputs > INT_MAX / 64 || rows > 65535)
     return fail(XE_ERR_NOT_SUPPORTED, "%s: a size is above its limit", what);
   if (rows == 0 || outputs == 0) return XE_OK;
   xe::int4::Params p{};
@@ -736,14 +770,20 @@ xe_status xe_int4_linear(const void* x, int64_t x_row, const float* x_scale, con
   p.rows = (int)rows, p.inputs = (int)inputs, p.outputs = (int)outputs, p.group = (int)group;
   p.scale_dtype = scale_dtype, p.y_dtype = y_dtype;
   p.pieces = x_dtype == XE_F32 ? 3 : 1;
+  p.group_magic = group == 32 ? 0u : (uint32_t)((1ull << 32) / (uint64_t)(group / 32)) + 1u;
   p.x_vec = aligned(size_of(x_dtype) == 1 ? 8 : 16, x, x_dtype, {x_row});
+  const size_t need = xe_int4_linear_workspace_size(rows, inputs, outputs, x_dtype);
+  if (need && (!workspace || workspace_bytes < need)) return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+  const Int4Plan plan = int4_plan(rows, inputs, outputs, p.pieces);
+  p.sums = need ? static_cast<float*>(workspace) : nullptr;
+  p.tokens = plan.tokens, p.parts = plan.parts, p.part = plan.part, p.runs = plan.runs, p.run = plan.run, p.pitch = plan.pitch;
   cudaStream_t st = as_stream(stream);
   switch (x_dtype) {
-    case XE_F32: return run_int4<float>(p, st);
-    case XE_BF16: return run_int4<__nv_bfloat16>(p, st);
-    case XE_F16: return run_int4<__half>(p, st);
-    case XE_E4M3: return run_int4<__nv_fp8_e4m3>(p, st);
-    default: return run_int4<int8_t>(p, st);
+    case XE_F32: return run_int4<float>(p, plan, st);
+    case XE_BF16: return run_int4<__nv_bfloat16>(p, plan, st);
+    case XE_F16: return run_int4<__half>(p, plan, st);
+    case XE_E4M3: return run_int4<__nv_fp8_e4m3>(p, plan, st);
+    default: return run_int4<int8_t>(p, plan, st);
   }
 }
 

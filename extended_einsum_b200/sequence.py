@@ -588,10 +588,12 @@ def int4_linear(
     if x_scale is not None:
         x_scale = _operand(what, "x_scale", x_scale, x, x.shape[:-1], torch.float32).contiguous() if x.dim() > 1 else x_scale
     y = torch.empty((*x.shape[:-1], outputs), device=device, dtype=dtype)
+    size = _lib.load().xe_int4_linear_workspace_size(rows.shape[0], inputs, outputs, code)
+    workspace = _workspace(size, device)
     _call(
         device, "xe_int4_linear", rows.data_ptr(), rows.stride(0), _pointer(x_scale), packed.data_ptr(), packed.stride(0),
         scales.data_ptr(), _pointer(zeros), y.data_ptr(), rows.shape[0], inputs, outputs, inputs // groups, code, scale_code,
-        y_code,
+        y_code, _pointer(workspace), size,
     )
     return y
 

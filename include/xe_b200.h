@@ -573,9 +573,11 @@ xe_status xe_rms_norm_backward(const void* sum, int64_t sum_row, const void* add
  * XE_F16; zeros one byte each, 0 to 15, or NULL for 8.  x: XE_F32, XE_BF16, XE_F16, or XE_E4M3 /
  * XE_I8 with x_scale per row (or NULL: 1).  `group` is a multiple of 32 that divides `inputs`.
  * Made for few rows (the weights are read again for every 64 of them, 21 with XE_F32). */
+size_t xe_int4_linear_workspace_size(int64_t rows, int64_t inputs, int64_t outputs, int32_t x_dtype);
 xe_status xe_int4_linear(const void* x, int64_t x_row, const float* x_scale, const void* packed, int64_t packed_row,
                          const void* scales, const void* zeros, void* y, int64_t rows, int64_t inputs, int64_t outputs,
-                         int64_t group, int32_t x_dtype, int32_t scale_dtype, int32_t y_dtype, void* stream);
+                         int64_t group, int32_t x_dtype, int32_t scale_dtype, int32_t y_dtype, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
