@@ -17,8 +17,8 @@
 // Warps work alone: a unit of work is a tile of sixteen rows over a run of k, and a warp takes every so many
 // units, its ring of stages (128 k of sixteen rows, filled by cp.async) running on from one unit to the next, so
 // that the reads never pause for a barrier.  A block only shares the staged activations: all of k, or, where that
-// does not fit, one part of it.  With more than one run of k, sums go to a workspace and a second kernel adds
-// them in order.
+// does not fit, one part of it.  Where blocks hold all of k, a tile's runs go to neighbouring warps, whose sums
+// meet in shared memory; sums of several parts go to a workspace and a second kernel adds them in order.
 #pragma once
 
 #include "seq_common.cuh"
@@ -42,7 +42,7 @@ struct Params {
   const void* scales;
   const uint8_t* zeros;  // or null
   void* y;
-  float* sums;  // (runs, columns of all tokens, outputs), or null where one run is all of k
+  float* sums;  // (parts * runs, columns of all tokens, outputs), or null where blocks hold all of k
   int64_t x_row, packed_row;  // strides of a row: elements, bytes
   int rows, inputs, outputs, group;
   uint32_t group_magic;  // floor(2^32 / (group / 32)) + 1, or 0 for groups of 32
@@ -52,7 +52,7 @@ struct Params {
   int tokens;   // tokens of one block
   int parts;    // parts of k that blocks hold, blockIdx.x % parts
   int part;     // their stages
-  int runs;     // runs of a part
+  int runs;     // runs of a part; 1, 2, 4 or 8 without `sums`
   int run;      // their stages
   int pitch;    // of the staged activations, elements
 };
@@ -192,13 +192,12 @@ struct Eight {
   }
 };
 
-__device__ __forceinline__ uint32_t load_scale(const void* p, int dtype, int64_t at) {
-  return dtype == XE_F32 ? static_cast<const uint32_t*>(p)[at] : static_cast<const uint16_t*>(p)[at];
+__device__ __forceinline__ uint32_t load_scale(const void* at, int dtype) {
+  return dtype == XE_F32 ? *static_cast<const uint32_t*>(at) : *static_cast<const uint16_t*>(at);
 }
 __device__ __forceinline__ float scale_value(uint32_t bits, int dtype) {
-  return dtype == XE_F32   ? __uint_as_float(bits)
-         : dtype == XE_BF16 ? __uint_as_float(bits << 16)
-                            : __half2float(__ushort_as_half((unsigned short)bits));
+  const float wide = __uint_as_float(dtype == XE_F32 ? bits : bits << 16);
+  return dtype == XE_F16 ? __half2float(__ushort_as_half((unsigned short)bits)) : wide;
 }
 
 // The group of k = 32 u.  The product's high word is the exact quotient as long as u * (group / 32) < 2^32.
@@ -260,7 +259,8 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(const __grid_c
   // the copying side: the next stage and where its rows and scales lie.  Rows past the last output read the last one.
   int copy_unit = first, copy_stage = 0, copy_end = 0;
   const uint8_t *from_a = nullptr, *from_b = nullptr;
-  int64_t scale_a = 0, scale_b = 0;
+  const uint8_t *scale_a = nullptr, *scale_b = nullptr, *zero_a = nullptr, *zero_b = nullptr;
+  const int scale_shift = p.scale_dtype == XE_F32 ? 2 : 1;
   // The last part may have fewer stages than the others, and runs of none: they are passed over here, and
   // their sums are zeros.
   auto open_copy = [&] {
@@ -272,8 +272,10 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(const __grid_c
       const int oa = min(tile * 16 + row8, last_o), ob = min(tile * 16 + row8 + 8, last_o);
       from_a = p.packed + oa * p.packed_row + (int64_t)copy_stage * (kStageK / 2) + quad * 16;
       from_b = p.packed + ob * p.packed_row + (int64_t)copy_stage * (kStageK / 2) + quad * 16;
-      scale_a = (int64_t)oa * groups;
-      scale_b = (int64_t)ob * groups;
+      scale_a = static_cast<const uint8_t*>(p.scales) + (((int64_t)oa * groups) << scale_shift);
+      scale_b = static_cast<const uint8_t*>(p.scales) + (((int64_t)ob * groups) << scale_shift);
+      zero_a = p.zeros + (int64_t)oa * groups;
+      zero_b = p.zeros + (int64_t)ob * groups;
       return;
     }
   };
@@ -287,16 +289,19 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(const __grid_c
   }
   auto issue = [&](int slot) {
     if (copy_unit < units) {
-      if (copy_stage * kStageK + quad * 32 < p.inputs) {
+      const int k32 = copy_stage * 4 + quad;
+      if (k32 * 32 < p.inputs) {
         cp_async16(copy_to + slot * kStageBytes, from_a);
         cp_async16(copy_to + slot * kStageBytes + 8 * kRowPitch, from_b);
-        const int g = group_of(p, copy_stage * 4 + (kRun < 4 ? quad : 0));
-        sa[slot] = load_scale(p.scales, p.scale_dtype, scale_a + g);
-        sb[slot] = load_scale(p.scales, p.scale_dtype, scale_b + g);
+        const int g = group_of(p, kRun < 4 ? k32 : copy_stage * 4);
+        sa[slot] = load_scale(scale_a + (g << scale_shift), p.scale_dtype);
+        sb[slot] = load_scale(scale_b + (g << scale_shift), p.scale_dtype);
         if (p.zeros) {
-          za[slot] = p.zeros[scale_a + g];
-          zb[slot] = p.zeros[scale_b + g];
+          za[slot] = zero_a[g];
+          zb[slot] = zero_b[g];
         }
+      } else if (kRun < 4) {
+        sa[slot] = sb[slot] = 0;  // not another stage's: it might not be finite
       }
       from_a += kStageK / 2;
       from_b += kStageK / 2;
@@ -315,21 +320,23 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(const __grid_c
   // there are fewer columns than warps
   if (threadIdx.x < kZeroBytes / 4) reinterpret_cast<uint32_t*>(xs)[threadIdx.x] = 0;
   {
-    const int k0 = stage0 * kStageK, kn = min(stage1 * kStageK, p.inputs) - k0;
+    const int k0 = stage0 * kStageK, kn = min(stage1 * kStageK, p.inputs) - k0, ke = (stage1 - stage0) * kStageK;
     const int across = columns > 4 ? 8 : columns > 2 ? 4 : columns > 1 ? 2 : 1;
     const int along = kWarps / across;
     for (int col = warp % across; col < columns; col += across) {
       const X* from = static_cast<const X*>(p.x) + (int64_t)(m0 + col / p.pieces) * p.x_row + k0;
       const int piece = p.pieces == 1 ? 0 : col % p.pieces;
       uint8_t* to = xs + kZeroBytes + (int64_t)col * p.pitch * 2;
-      for (int k = (warp / across * 32 + lane) * 8; k < kn; k += along * 256 * 4) {
+      for (int k = (warp / across * 32 + lane) * 8; k < ke; k += along * 256 * 4) {
         Eight<X> e[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (k + j * along * 256 < kn) e[j].load(from + k + j * along * 256, p.x_vec);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (k + j * along * 256 < kn) *reinterpret_cast<uint4*>(to + (k + j * along * 256) * 2) = e[j].staged(piece);
+        for (int j = 0; j < 4; ++j) {
+          const int at = k + j * along * 256;
+          if (at < ke) *reinterpret_cast<uint4*>(to + at * 2) = at < kn ? e[j].staged(piece) : make_uint4(0, 0, 0, 0);
+        }
       }
     }
   }
@@ -346,23 +353,44 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(const __grid_c
   float acc[kTiles][4];
   int unit = first, stage = 0, end = 0, tile = 0, run = 0;
   uint32_t x_at[kTiles];
+  constexpr int kCols = kTiles * 8 + 1;
+  float* red = reinterpret_cast<float*>(xs + kZeroBytes + columns * p.pitch * 2);  // [warp][16 rows][columns + 1]
   auto close_unit = [&] {
+    if (p.sums) {
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
+      for (int n = 0; n < kTiles; ++n) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int col = n * 8 + quad * 2 + i % 2, o = tile * 16 + row8 + i / 2 * 8;
-        if (col < columns && o <= last_o) {
-          if (p.sums) {
+        for (int i = 0; i < 4; ++i) {
+          const int col = n * 8 + quad * 2 + i % 2, o = tile * 16 + row8 + i / 2 * 8;
+          if (col < columns && o <= last_o) {
             const int64_t all = (int64_t)p.rows * p.pieces;
             p.sums[((int64_t)(part * p.runs + run) * all + (int64_t)m0 * p.pieces + col) * p.outputs + o] = acc[n][i];
-          } else {
-            const float v = p.x_scale ? acc[n][i] * p.x_scale[m0 + col] : acc[n][i];
-            store_as(p.y, p.y_dtype, (int64_t)(m0 + col) * p.outputs + o, v);
           }
         }
       }
+      return;
     }
+    // every warp of the block comes here once for each of the block's turns
+    const uint32_t red_at = (uint32_t)__cvta_generic_to_shared(red + (warp * 16 + row8) * kCols + quad * 2);
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(red_at + (i / 2 * 8 * kCols + n * 8 + i % 2) * 4), "f"(acc[n][i]) : "memory");
+    }
+    __syncthreads();
+    const int rows = 16 * kWarps / p.runs;
+    const int o0 = (unit - warp) / p.runs * 16;
+    for (int i = threadIdx.x; i < rows * tokens; i += kWarps * 32) {
+      const int r = i % rows, m = i / rows;
+      if (o0 + r > last_o) continue;
+      float v = 0.0f;
+      for (int piece = p.pieces - 1; piece >= 0; --piece)
+        for (int w = 0; w < p.runs; ++w) v += red[((r / 16 * p.runs + w) * 16 + r % 16) * kCols + m * p.pieces + piece];
+      if (p.x_scale) v *= p.x_scale[m0 + m];
+      store_as(p.y, p.y_dtype, (int64_t)(m0 + m) * p.outputs + o0 + r, v);
+    }
+    __syncthreads();
   };
   auto open_unit = [&] {
     for (; unit < units; unit += stride) {
@@ -415,14 +443,9 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(const __grid_c
         }
       }
     };
-    const int left = p.inputs - stage * kStageK;
-    if (left >= kStageK) {
+    // past the last k the activations are zeros, and the codes whatever the slot held
 #pragma unroll
-      for (int j = 0; j < 4; ++j) group32(j, j % kRun == 0, j % kRun == kRun - 1);
-    } else {
-#pragma unroll 1
-      for (int j = 0; j * 32 < left; ++j) group32(j, true, true);
-    }
+    for (int j = 0; j < 4; ++j) group32(j, j % kRun == 0, j % kRun == kRun - 1);
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) x_at[n] += x_step[n];
   };
@@ -445,6 +468,15 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(const __grid_c
     }
   }
   cp_async_wait<0>();
+  if (!p.sums) {
+    // the last turn's units may end inside the block
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+    if (unit - warp < units) close_unit();
+    return;
+  }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 

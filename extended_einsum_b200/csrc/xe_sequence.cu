@@ -648,9 +648,8 @@ struct Int4Plan {
 };
 
 // How the work is cut: k into the parts that fit a block's shared memory, and these into runs, so that the
-// device's warps get equally many stages each.  A unit of work costs its stages and about four more for its
-// start and its sums, a warp alone needs about three times the issue slots of its instructions, and the device
-// takes 592 warps' instructions at a time.
+// device's warps get equally many stages each.  A unit of work costs its stages and about two more for its
+// start and its sums.
 Int4Plan int4_plan(int64_t rows, int64_t inputs, int64_t outputs, int pieces) {
   using namespace xe::int4;
   Int4Plan q;
@@ -658,26 +657,30 @@ Int4Plan int4_plan(int64_t rows, int64_t inputs, int64_t outputs, int pieces) {
   const int columns = q.tokens * pieces;
   q.tiles = columns <= 8 ? 1 : columns <= 16 ? 2 : columns <= 32 ? 4 : 8;
   constexpr int kRing = kWarps * kStages * kStageBytes;
-  // three blocks to a multiprocessor, two, or one, as the columns (and with them the registers) grow
-  const int each = q.tiles <= 2 ? 3 : q.tiles == 4 ? 2 : 1;
-  const int budget = 225 * 1024 / each - 1024 - kRing - kZeroBytes;
-  const int64_t stages = ceil_div(inputs, kStageK);
-  const int64_t fit = std::max<int64_t>(1, (budget / (columns * 2) - 32) / kStageK);
-  q.parts = (int)ceil_div(stages, fit);
+  const int64_t stages = ceil_div(inputs, kStageK), rows16 = ceil_div(outputs, 16);
+  // three blocks to a multiprocessor, two, or one, as the columns (and with them the registers) grow; fewer too
+  // where there is little work and their larger share of the memory holds all of k
+  int each = q.tiles <= 2 ? 3 : q.tiles == 4 ? 2 : 1;
+  const int sums = kWarps * 16 * (q.tiles * 8 + 1) * 4;
+  auto fit = [&](int blocks, int beside) {
+    const int budget = 225 * 1024 / blocks - 1024 - kRing - kZeroBytes - beside;
+    return std::max<int64_t>(1, (budget / (columns * 2) - 32) / kStageK);
+  };
+  if (rows16 * stages <= 148 * kWarps * 4)
+    while (each > 1 && fit(each, sums) < stages) --each;
+  q.parts = fit(each, sums) >= stages ? 1 : (int)std::max<int64_t>(2, ceil_div(stages, fit(each, 0)));
   q.part = (int)ceil_div(stages, q.parts);
   q.parts = (int)ceil_div(stages, q.part);
   q.pitch = q.part * kStageK + 32;  // bytes: 64 past a multiple of 128, two columns' reads in different banks
-  q.bytes = kRing + kZeroBytes + columns * q.pitch * 2;
+  q.bytes = kRing + kZeroBytes + columns * q.pitch * 2 + (q.parts == 1 ? sums : 0);
   const int64_t blocks = ceil_div(rows, q.tokens);  // in y
   const int64_t workers = std::max<int64_t>(1, 148 * each / (q.parts * blocks));
-  const int64_t rows16 = ceil_div(outputs, 16);
   int64_t best = INT64_MAX;
   q.runs = 1, q.run = q.part;
-  for (int64_t runs = 1; runs <= 16 && runs <= q.part; ++runs) {
+  for (int64_t runs = 1; runs <= 16 && runs <= std::max(q.part, kWarps); ++runs) {
     const int64_t run = ceil_div(q.part, runs);
-    if (ceil_div(q.part, run) != runs) continue;
-    const int64_t units = rows16 * runs;
-    const int64_t cost = (run + 4) * std::max(3 * ceil_div(units, workers * kWarps), ceil_div(units * q.parts * blocks, 592));
+    if (q.parts == 1 ? (runs & (runs - 1)) != 0 || runs > kWarps : ceil_div(q.part, run) != runs) continue;
+    const int64_t cost = ceil_div(rows16 * runs, workers * kWarps) * (run + 2);
     if (cost < best) best = cost, q.runs = (int)runs, q.run = (int)run;
   }
   q.blocks = (int)(q.parts * std::min<int64_t>(workers, ceil_div(rows16 * q.runs, kWarps)));
@@ -740,8 +743,7 @@ size_t xe_int4_linear_workspace_size(int64_t rows, int64_t inputs, int64_t outpu
   if (rows <= 0 || inputs < 1 || outputs <= 0 || inputs > 1 << 20) return 0;
   const int pieces = x_dtype == XE_F32 ? 3 : 1;
   const Int4Plan plan = int4_plan(rows, inputs, outputs, pieces);
-  const int64_t runs = (int64_t)plan.parts * plan.runs;
-  return runs == 1 && pieces == 1 ? 0 : padded((size_t)(runs * rows * pieces * outputs) * 4);
+  return plan.parts == 1 ? 0 : padded((size_t)((int64_t)plan.parts * plan.runs * rows * pieces * outputs) * 4);
 }
 
 xe_status xe_int4_linear(const void* x, int64_t x_row, const float* x_scale, const void* packed, int64_t packed_row,
