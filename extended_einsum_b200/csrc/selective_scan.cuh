@@ -28,7 +28,8 @@ namespace scan {
 
 using namespace seq;
 
-constexpr int kBackwardThreads = 128;
+constexpr int kBackwardThreads = 64;
+constexpr int kBackwardChannels = 32;
 
 struct Params {
   const void *x, *delta, *z, *b, *c;
@@ -58,21 +59,7 @@ struct Params {
 };
 
 // Tokens between two stored states (training): the backward pass runs forward again from them.
-constexpr int kCheckpoint = 16;
-
-template <int N>
-__device__ __forceinline__ void load_f32(const float* smem, float (&v)[N]) {
-  if constexpr (N % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const float4 q = *reinterpret_cast<const float4*>(smem + i);
-      v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = smem[i];
-  }
-}
+constexpr int kCheckpoint = 8;
 
 // A block's channels lie in one group: blocks [g * per_group, (g + 1) * per_group) are group g's.
 struct Channels {
@@ -85,41 +72,6 @@ __device__ __forceinline__ Channels block_channels(const Params& p, int per_bloc
   const int at = (blockIdx.x % per_group) * per_block;
   return {group, group * each + at, min(per_block, each - at)};
 }
-
-// B and C of a tile as float32, states padded with zeros; tokens at or past `live` read as zero.
-template <typename T, int kTile, int NP, int kBlock>
-struct SharedStates {
-  static constexpr int kVectors = 2 * kTile * (NP / 8);
-  static constexpr int kEach = (kVectors + kBlock - 1) / kBlock;
-  Raw8<T> raw[kEach];
-
-  __device__ __forceinline__ void load(const Params& p, int batch, int group, int t0, int live, int wanted = 3) {
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      const int i = k * kBlock + threadIdx.x;
-      const int n0 = (i % (NP / 8)) * 8;
-      const int which = (i / (NP / 8)) & 1;
-      const int t = t0 + i / (NP / 8) / 2;
-      const int count = i < kVectors && t < live && (wanted >> which & 1) ? min(8, p.states - n0) : 0;
-      const T* at = which ? static_cast<const T*>(p.c) + batch * p.c_sb + t * p.c_st + group * p.c_sg + n0
-                          : static_cast<const T*>(p.b) + batch * p.b_sb + t * p.b_st + group * p.b_sg + n0;
-      raw[k] = load8<T>(at, count, p.vec & (which ? 32 : 16));
-    }
-  }
-  __device__ __forceinline__ void store(float* smem) {
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      const int i = k * kBlock + threadIdx.x;
-      if (i < kVectors) {
-        float v[8];
-        unpack8<T>(raw[k], v);
-        float4* at = reinterpret_cast<float4*>(smem + (int64_t)i * 8);
-        at[0] = make_float4(v[0], v[1], v[2], v[3]);
-        at[1] = make_float4(v[4], v[5], v[6], v[7]);
-      }
-    }
-  }
-};
 
 // Sums v[k] over the kLanes lanes of a channel; lane l returns the sum of v[l].
 template <int kLanes>
@@ -437,39 +389,43 @@ __device__ __forceinline__ float channel_sum(float (&v)[8], int lane_in_warp) {
 //   dx = D dv + delta sum_n g B,  ddelta = x sum_n g B + sum_n A w,  dA = sum_t delta w,
 //   dB = sum_d g delta x,  dC = sum_d dv h,  dD = sum dv x,  dz = dy v silu'(z).
 //
-// Tiles of 32 tokens are taken from the last to the first, in halves of kCheckpoint tokens: the states
+// Tiles of sixteen tokens are taken from the last to the first, in halves of kCheckpoint tokens: the states
 // of a half are run again from its stored first state and stay in registers, with their e, for the
-// way back.  Sixteen states at a time (four lanes of four); more states take further turns over
-// the staged tile.  Sums over the states of a channel and over the channels of a warp are
-// transposed butterflies; the warps' parts of dB and dC go through shared memory, the blocks' through
-// global memory, all in a fixed order.
+// way back.  A thread holds four states of two channels, so that their terms of dB and dC add up before any
+// exchange; sixteen states at a time, and more take further turns over the staged tile.  Sums over the
+// states of a channel and over the channels of a warp are transposed butterflies; the block's two warps'
+// parts of dB and dC meet in shared memory, the blocks' in global memory, all in a fixed order.  The next tile is
+// only called into the L2 cache: registers go to the states.
 template <typename T, int kBlocks>
-__global__ void __launch_bounds__(kBackwardThreads, 2) selective_scan_backward_kernel(Params p) {
-  constexpr int S = 4, kLanes = 4, kChannels = kBackwardThreads / kLanes, kTile = 32, kWarps = kBackwardThreads / 32;
+__global__ void __launch_bounds__(kBackwardThreads) selective_scan_backward_kernel(const __grid_constant__ Params p) {
+  constexpr int kTile = 16, kHalf = kCheckpoint, kWarps = kBackwardThreads / 32, kChannels = kBackwardChannels;
   constexpr int NP = 16 * kBlocks;
-  constexpr int kHalf = kCheckpoint;
+  constexpr int kEach = 8 * 2 * (NP / 4) / kBackwardThreads;  // quads of B and C states per thread
   extern __shared__ __align__(16) float smem[];
   constexpr int kPitch = kChannels + 4;
-  float2(*s_dx)[kChannels + 2] = reinterpret_cast<float2(*)[kChannels + 2]>(smem);  // (delta, x)
+  float2(*s_du)[kChannels + 2] = reinterpret_cast<float2(*)[kChannels + 2]>(smem);  // (delta, delta x)
   float* at_smem = smem + kTile * (kChannels + 2) * 2;
   float(*s_dv)[kPitch] = reinterpret_cast<float(*)[kPitch]>(at_smem);
   float(*s_v)[kPitch] = s_dv + kTile;   // sum C h
   float(*s_gb)[kPitch] = s_v + kTile;   // sum g B
   float(*s_ga)[kPitch] = s_gb + kTile;  // sum A w / ln 2
-  float* s_bc = at_smem + 4 * kTile * kPitch;
-  float* s_red = s_bc + kTile * 2 * NP;  // [kWarps][kTile][2][16]
+  float* s_bc = at_smem + 4 * kTile * kPitch;  // [kTile][2][NP]
+  float* s_red = s_bc + kTile * 2 * NP;        // [kBlocks][kWarps][kTile][2][16]
 
   const Channels ch = block_channels(p, kChannels);
   const int batch = blockIdx.y, segment = blockIdx.z;
   const int begin = segment * p.segment_length;
   const int end = min(begin + p.segment_length, p.length);
   const int live = min(end, sequence_length(p.lengths, p.lengths64, batch, p.length));
-  const int row = threadIdx.x / (kChannels / 8);
-  const int col = (threadIdx.x % (kChannels / 8)) * 8;
-  const int count = max(0, min(8, ch.count - col));
-  float bias[8], skip[8], dd[8], dbias[8];
+
+  // staging: this thread's pair of tokens and four channels
+  const int row = threadIdx.x / (kChannels / 4) * 2;
+  const int col = threadIdx.x % (kChannels / 4) * 4;
+  const int count = max(0, min(4, ch.count - col));
+  const bool whole = count == 4;
+  float bias[4], skip[4], dd[4], dbias[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     bias[i] = p.bias && i < count ? p.bias[ch.first + col + i] : 0.0f;
     skip[i] = p.d && i < count ? p.d[ch.first + col + i] : 0.0f;
     dd[i] = dbias[i] = 0.0f;
@@ -479,226 +435,263 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) selective_scan_backward_k
   const T* z = static_cast<const T*>(p.z) + batch * p.z_sb + ch.first + col;
   const T* dy = static_cast<const T*>(p.dy) + batch * p.dy_sb + ch.first + col;
   const int64_t out_at = (int64_t)batch * p.length * p.channels + ch.first + col;
+  const T* b = static_cast<const T*>(p.b) + batch * p.b_sb + ch.group * p.b_sg;
+  const T* c = static_cast<const T*>(p.c) + batch * p.c_sb + ch.group * p.c_sg;
 
-  const int c = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
-  const int warp = threadIdx.x / 32, warp_lane = threadIdx.x % 32;
-  const bool mine = c < ch.count;
-  const int64_t state_at = ((int64_t)batch * p.channels + ch.first + c) * p.states;
-  float a[kBlocks][S], carry[kBlocks][S], da[kBlocks][S];
+  // recurrence: this thread's two channels and four states of each sixteen
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, quad = lane % 4;
+  const int mine = warp * 16 + lane / 4 * 2;
+  const int64_t state_at = ((int64_t)batch * p.channels + ch.first + mine) * p.states;
+  F2 a[kBlocks][2][2], carry[kBlocks][2][2], da[kBlocks][2][2];
   for (int nb = 0; nb < kBlocks; ++nb) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int n = nb * 16 + lane * S + s;
-      const bool in = mine && n < p.states;
-      a[nb][s] = in ? p.a[(int64_t)(ch.first + c) * p.states + n] * kLog2e : 0.0f;
-      carry[nb][s] = da[nb][s] = 0.0f;
-      if (in) {
-        if (p.segments > 1)
-          carry[nb][s] = p.segment_state[(int64_t)segment * p.batch * p.channels * p.states + state_at + n];
-        else if (p.dstate_out)
-          carry[nb][s] = p.dstate_out[state_at + n];
+    for (int j = 0; j < 2; ++j) {
+      float a1[4], c1[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int n = nb * 16 + quad * 4 + s;
+        const bool in = mine + j < ch.count && n < p.states;
+        a1[s] = in ? p.a[(int64_t)(ch.first + mine + j) * p.states + n] * kLog2e : 0.0f;
+        c1[s] = 0.0f;
+        if (in) {
+          if (p.segments > 1)
+            c1[s] = p.segment_state[(int64_t)segment * p.batch * p.channels * p.states + state_at + j * p.states + n];
+          else if (p.dstate_out)
+            c1[s] = p.dstate_out[state_at + j * p.states + n];
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        a[nb][j][s] = pack2(a1[2 * s], a1[2 * s + 1]);
+        carry[nb][j][s] = pack2(c1[2 * s], c1[2 * s + 1]);
+        da[nb][j][s] = 0;
       }
     }
   }
   const int64_t checkpoint_rows = (p.length + kCheckpoint - 1) / kCheckpoint;
+  const float* checkpoints = p.checkpoints + ((int64_t)batch * checkpoint_rows * p.channels + ch.first + mine) * NP + quad * 4;
 
-  Raw8<T> raw_x, raw_d, raw_z, raw_g;
-  SharedStates<T, kTile, NP, kBackwardThreads> bc;
-  auto fetch = [&](int t0) {
-    const int t = t0 + row;
-    const int n = t < live ? count : 0;
-    raw_x = load8<T>(x + t * p.x_st, n, p.vec & 1);
-    raw_d = load8<T>(delta + t * p.delta_st, n, p.vec & 2);
-    raw_g = load8<T>(dy + t * p.dy_st, n, p.vec & 64);
-    if (p.z) raw_z = load8<T>(z + t * p.z_st, n, p.vec & 4);
-    bc.load(p, batch, ch.group, t0, live);
-  };
   const int tiles = (end - begin + kTile - 1) / kTile;
-  if (tiles > 0) fetch(begin + (tiles - 1) * kTile);
   for (int t0 = begin + (tiles - 1) * kTile; t0 >= begin; t0 -= kTile) {
-    const bool in = t0 + row < live;
-    float slope[8], dgate[8];  // softplus'(raw), dy silu'(z)
-    {
-      float xv[8], rv[8], gv[8], zv[8];
-      unpack8<T>(raw_x, xv);
-      unpack8<T>(raw_d, rv);
-      unpack8<T>(raw_g, gv);
-      if (p.z) unpack8<T>(raw_z, zv);
+    struct {
+      Raw4<T> x, d, g, z;
+    } raw[2];
+    const bool in[2] = {t0 + row < live, t0 + row + 1 < live};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float r = rv[i] + bias[i];
-        slope[i] = p.softplus ? sigmoid(r) : 1.0f;
-        const float dl = p.softplus ? softplus(r) : r;
-        float dv = gv[i];
-        dgate[i] = 0.0f;
-        if (p.z) {
-          const float s = sigmoid(zv[i]);
-          dv *= zv[i] * s;
-          dgate[i] = gv[i] * s * (1.0f + zv[i] * (1.0f - s));
-        }
-        s_dx[row][col + i] = in ? make_float2(dl, xv[i]) : make_float2(0.0f, 0.0f);
-        s_dv[row][col + i] = in ? dv : 0.0f;
+    for (int q = 0; q < 2; ++q) {
+      const int64_t t = t0 + row + q;
+      raw[q].x = load4_if<T>(x + t * p.x_st, in[q], count, whole && (p.vec & 1));
+      raw[q].d = load4_if<T>(delta + t * p.delta_st, in[q], count, whole && (p.vec & 2));
+      raw[q].g = load4_if<T>(dy + t * p.dy_st, in[q], count, whole && (p.vec & 64));
+      if (p.z) raw[q].z = load4_if<T>(z + t * p.z_st, in[q], count, whole && (p.vec & 4));
+      if (t0 > begin && count > 0) {
+        prefetch_l2(x + (t - kTile) * p.x_st);
+        prefetch_l2(delta + (t - kTile) * p.delta_st);
+        prefetch_l2(dy + (t - kTile) * p.dy_st);
+        if (p.z) prefetch_l2(z + (t - kTile) * p.z_st);
       }
     }
-    bc.store(s_bc);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int i = k * kBackwardThreads + threadIdx.x;
+      const int n0 = i % (NP / 4) * 4, which = i / (NP / 4) % 2, t = i / (NP / 4) / 2 * 2;
+      const int n1 = max(0, min(4, p.states - n0));
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const T* at = which ? c + (int64_t)(t0 + t + q) * p.c_st + n0 : b + (int64_t)(t0 + t + q) * p.b_st + n0;
+        const Raw4<T> r = load4_if<T>(at, n1 > 0 && t0 + t + q < live, n1, n1 == 4 && (p.vec & (which ? 32 : 16)));
+        *reinterpret_cast<float4*>(s_bc + ((t + q) * 2 + which) * NP + n0) =
+            make_float4(value4<T>(r, 0), value4<T>(r, 1), value4<T>(r, 2), value4<T>(r, 3));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      F2 d = add2(pack2(value4<T>(raw[0].d, i), value4<T>(raw[1].d, i)), both(bias[i]));
+      if (p.softplus) d = softplus2(d);
+      const F2 g = pack2(value4<T>(raw[0].g, i), value4<T>(raw[1].g, i));
+      const float2 dv = unpack2(p.z ? gate2(g, pack2(value4<T>(raw[0].z, i), value4<T>(raw[1].z, i))) : g);
+      const float2 dl = unpack2(d);
+      // past a sequence's end delta is a constant zero, though the adjoint still passes through; x, z, dy, B and C
+      // have been read as zero
+      const float d0 = in[0] ? dl.x : 0.0f, d1 = in[1] ? dl.y : 0.0f;
+      s_du[row][col + i] = make_float2(d0, d0 * value4<T>(raw[0].x, i));
+      s_du[row + 1][col + i] = make_float2(d1, d1 * value4<T>(raw[1].x, i));
+      s_dv[row][col + i] = dv.x;
+      s_dv[row + 1][col + i] = dv.y;
+    }
     __syncthreads();
-    if (t0 > begin) fetch(t0 - kTile);
+#pragma unroll 1
     for (int nb = 0; nb < kBlocks; ++nb) {
+#pragma unroll 1
       for (int half = kTile / kHalf - 1; half >= 0; --half) {
         const int u0 = half * kHalf;
-        if (t0 + u0 >= p.length) {
-          // past the end: nothing comes from these tokens
-          for (int t = lane; t < kHalf; t += kLanes) {
-            if (nb == 0) s_v[u0 + t][c] = s_gb[u0 + t][c] = s_ga[u0 + t][c] = 0.0f;
-          }
-          if (warp_lane < 16)
-            for (int t = 0; t < kHalf; ++t)
-              s_red[((warp * kTile + u0 + t) * 2 + 0) * 16 + warp_lane] =
-                  s_red[((warp * kTile + u0 + t) * 2 + 1) * 16 + warp_lane] = 0.0f;
-          continue;
-        }
-        float h0[S], h[kHalf][S], e[kHalf][S], da_half[S] = {};
-        {
-          float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (mine)
-            q = *reinterpret_cast<const float4*>(
-                p.checkpoints +
-                (((int64_t)batch * checkpoint_rows + (t0 + u0) / kCheckpoint) * p.channels + ch.first + c) * NP + nb * 16 +
-                lane * S);
-          h0[0] = q.x, h0[1] = q.y, h0[2] = q.z, h0[3] = q.w;
+        F2 h0[2][2], h[kHalf][2][2], e[kHalf][2][2], da_half[2][2] = {};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          ulonglong2 q = make_ulonglong2(0, 0);
+          if (mine + j < ch.count && t0 + u0 < p.length)
+            q = *reinterpret_cast<const ulonglong2*>(
+                checkpoints + ((int64_t)((t0 + u0) / kCheckpoint) * p.channels + j) * NP + nb * 16);
+          h0[j][0] = q.x, h0[j][1] = q.y;
         }
 #pragma unroll
         for (int t4 = 0; t4 < kHalf; t4 += 4) {
-          float v[4];
+          float v[2][4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int t = t4 + k;
-            const float2 q = s_dx[u0 + t][c];
-            float bv[S], cv[S];
-            load_f32<S>(s_bc + ((u0 + t) * 2) * NP + nb * 16 + lane * S, bv);
-            load_f32<S>(s_bc + ((u0 + t) * 2 + 1) * NP + nb * 16 + lane * S, cv);
-            v[k] = 0.0f;
+            const float4 du = *reinterpret_cast<const float4*>(&s_du[u0 + t][mine]);
+            const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(s_bc + (u0 + t) * 2 * NP + nb * 16 + quad * 4);
+            const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(s_bc + ((u0 + t) * 2 + 1) * NP + nb * 16 + quad * 4);
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-              e[t][s] = exp2_fast(q.x * a[nb][s]);
-              h[t][s] = fmaf(e[t][s], t == 0 ? h0[s] : h[t - 1][s], q.x * q.y * bv[s]);
-              v[k] = fmaf(cv[s], h[t][s], v[k]);
+            for (int j = 0; j < 2; ++j) {
+              const F2 d2 = both(j ? du.z : du.x), u2 = both(j ? du.w : du.y);
+#pragma unroll
+              for (int s = 0; s < 2; ++s) {
+                e[t][j][s] = exp2_fast2(mul2(d2, a[nb][j][s]));
+                h[t][j][s] = fma2(e[t][j][s], t == 0 ? h0[j][s] : h[t > 0 ? t - 1 : 0][j][s], mul2(u2, s ? bv.y : bv.x));
+              }
+              const float2 q = unpack2(fma2(cv.y, h[t][j][1], mul2(cv.x, h[t][j][0])));
+              v[j][k] = q.x + q.y;
             }
           }
-          const float sum = transpose_sum<4>(v, lane);
-          float& out = s_v[u0 + t4 + lane][c];
-          out = nb == 0 ? sum : out + sum;
+          if (p.z) {  // only the gate's gradient asks for it
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float sum = transpose_sum<4>(v[j], quad);
+              float& out = s_v[u0 + t4 + quad][mine + j];
+              out = nb == 0 ? sum : out + sum;
+            }
+          }
         }
 #pragma unroll
         for (int t4 = kHalf - 4; t4 >= 0; t4 -= 4) {
-          float gb[4], ga[4];
+          float gb[2][4], ga[2][4];
 #pragma unroll
-          for (int k2 = 2; k2 >= 0; k2 -= 2) {
-            float db[8], dc[8];
+          for (int k = 3; k >= 0; --k) {
+            const int t = t4 + k;
+            const float4 du = *reinterpret_cast<const float4*>(&s_du[u0 + t][mine]);
+            const float2 dv = *reinterpret_cast<const float2*>(&s_dv[u0 + t][mine]);
+            const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(s_bc + (u0 + t) * 2 * NP + nb * 16 + quad * 4);
+            const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(s_bc + ((u0 + t) * 2 + 1) * NP + nb * 16 + quad * 4);
+            F2 db[2], dc[2];
 #pragma unroll
-            for (int k1 = 1; k1 >= 0; --k1) {
-              const int k = k2 + k1, t = t4 + k;
-              const float2 q = s_dx[u0 + t][c];
-              const float dv = s_dv[u0 + t][c];
-              float bv[S], cv[S];
-              load_f32<S>(s_bc + ((u0 + t) * 2) * NP + nb * 16 + lane * S, bv);
-              load_f32<S>(s_bc + ((u0 + t) * 2 + 1) * NP + nb * 16 + lane * S, cv);
-              gb[k] = ga[k] = 0.0f;
+            for (int j = 0; j < 2; ++j) {
+              const F2 d2 = both(j ? du.z : du.x), u2 = both(j ? du.w : du.y), dv2 = both(j ? dv.y : dv.x);
+              F2 gb2 = 0, ga2 = 0;
 #pragma unroll
-              for (int s = 0; s < S; ++s) {
-                const float g = fmaf(cv[s], dv, carry[nb][s]);
-                gb[k] = fmaf(g, bv[s], gb[k]);
-                db[k1 * 4 + s] = g * q.x * q.y;
-                dc[k1 * 4 + s] = dv * h[t][s];
-                carry[nb][s] = g * e[t][s];
-                const float w = carry[nb][s] * (t == 0 ? h0[s] : h[t - 1][s]);
-                ga[k] = fmaf(a[nb][s], w, ga[k]);
-                da_half[s] = fmaf(q.x, w, da_half[s]);
+              for (int s = 0; s < 2; ++s) {
+                const F2 g = fma2(s ? cv.y : cv.x, dv2, carry[nb][j][s]);
+                db[s] = j == 0 ? mul2(g, u2) : fma2(g, u2, db[s]);
+                dc[s] = j == 0 ? mul2(dv2, h[t][j][s]) : fma2(dv2, h[t][j][s], dc[s]);
+                gb2 = s == 0 ? mul2(g, bv.x) : fma2(g, bv.y, gb2);
+                carry[nb][j][s] = mul2(g, e[t][j][s]);
+                const F2 w = mul2(carry[nb][j][s], t == 0 ? h0[j][s] : h[t > 0 ? t - 1 : 0][j][s]);
+                ga2 = s == 0 ? mul2(a[nb][j][s], w) : fma2(a[nb][j][s], w, ga2);
+                da_half[j][s] = fma2(d2, w, da_half[j][s]);
               }
+              const float2 q = unpack2(gb2), r = unpack2(ga2);
+              gb[j][k] = q.x + q.y;
+              ga[j][k] = r.x + r.y;
             }
-            const float rb = channel_sum(db, warp_lane);
-            const float rc = channel_sum(dc, warp_lane);
-            const int index = ((warp_lane >> 4 & 1) << 2) | ((warp_lane >> 3 & 1) << 1) | (warp_lane >> 2 & 1);
-            float* out = s_red + ((warp * kTile + u0 + t4 + k2 + (index >> 2)) * 2) * 16 + lane * S + (index & 3);
-            out[0] = rb;
-            out[16] = rc;
+            const float2 q0 = unpack2(db[0]), q1 = unpack2(db[1]), r0 = unpack2(dc[0]), r1 = unpack2(dc[1]);
+            float both_sums[8] = {q0.x, q0.y, q1.x, q1.y, r0.x, r0.y, r1.x, r1.y};
+            const float sum = channel_sum(both_sums, lane);
+            const int index = lane >> 2;  // dB or dC, state of the quad
+            s_red[((nb * kWarps + warp) * kTile + u0 + t) * 32 + (index >> 2) * 16 + quad * 4 + (index & 3)] = sum;
           }
-          const float sb = transpose_sum<4>(gb, lane);
-          const float sa = transpose_sum<4>(ga, lane);
-          float& ob = s_gb[u0 + t4 + lane][c];
-          float& oa = s_ga[u0 + t4 + lane][c];
-          ob = nb == 0 ? sb : ob + sb;
-          oa = nb == 0 ? sa : oa + sa;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float sb = transpose_sum<4>(gb[j], quad), sa = transpose_sum<4>(ga[j], quad);
+            float& ob = s_gb[u0 + t4 + quad][mine + j];
+            float& oa = s_ga[u0 + t4 + quad][mine + j];
+            ob = nb == 0 ? sb : ob + sb;
+            oa = nb == 0 ? sa : oa + sa;
+          }
         }
         // sums of sums: one running sum over thousands of tokens would lose its last bits
 #pragma unroll
-        for (int s = 0; s < S; ++s) da[nb][s] += da_half[s];
-      }
-      __syncthreads();
-      // the warps' parts of dB and dC of these sixteen states
-      for (int i = threadIdx.x; i < kTile * 2 * 16; i += kBackwardThreads) {
-        const int t = t0 + i / 32;
-        if (t < end) {
-          float sum = s_red[i];
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int k = 1; k < kWarps; ++k) sum += s_red[k * kTile * 32 + i];
-          p.dbc[(((int64_t)blockIdx.x * p.batch + batch) * p.length + t) * 2 * NP + (i / 16 % 2) * NP + nb * 16 + i % 16] = sum;
-        }
+          for (int s = 0; s < 2; ++s) da[nb][j][s] = add2(da[nb][j][s], da_half[j][s]);
       }
-      if (kBlocks > 1 && nb + 1 < kBlocks) __syncthreads();
     }
-    if (t0 + row < end && count > 0) {
-      float o_x[8], o_d[8], o_z[8];
+    __syncthreads();
+    // the warps' parts of dB and dC
+    for (int i = threadIdx.x; i < kBlocks * kTile * 32; i += kBackwardThreads) {
+      const int nb = i / (kTile * 32), t = i / 32 % kTile;
+      if (t0 + t < end) {
+        float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 q = s_dx[row][col + i];
-        const float dv = s_dv[row][col + i], gb = s_gb[row][col + i];
-        o_x[i] = fmaf(dv, skip[i], q.x * gb);
-        // past a sequence's end delta is a constant zero, though the adjoint still passes through
-        o_d[i] = in ? fmaf(q.y, gb, kLn2 * s_ga[row][col + i]) * slope[i] : 0.0f;
-        o_z[i] = in ? dgate[i] * fmaf(skip[i], q.y, s_v[row][col + i]) : 0.0f;
-        dd[i] = fmaf(dv, q.y, dd[i]);
-        dbias[i] += o_d[i];
+        for (int k = 0; k < kWarps; ++k) sum += s_red[((nb * kWarps + k) * kTile) * 32 + i % (kTile * 32)];
+        p.dbc[(((int64_t)blockIdx.x * p.batch + batch) * p.length + t0 + t) * 2 * NP + (i / 16 % 2) * NP + nb * 16 + i % 16] = sum;
       }
-      const int64_t at = out_at + (int64_t)(t0 + row) * p.channels;
-      store8<T>(static_cast<T*>(p.dx) + at, count, p.vec & 8, o_x);
-      store8<T>(static_cast<T*>(p.ddelta) + at, count, p.vec & 8, o_d);
-      if (p.z) store8<T>(static_cast<T*>(p.dz) + at, count, p.vec & 8, o_z);
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if (t0 + row + q < end && count > 0) {
+        float o_x[4], o_d[4], o_z[4];
+        const float4 gb = *reinterpret_cast<const float4*>(&s_gb[row + q][col]);
+        const float4 ga = *reinterpret_cast<const float4*>(&s_ga[row + q][col]);
+        const float4 v4 = *reinterpret_cast<const float4*>(&s_v[row + q][col]);
+        const float4 dv4 = *reinterpret_cast<const float4*>(&s_dv[row + q][col]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float xv = value4<T>(raw[q].x, i), gbi = (&gb.x)[i], dv = (&dv4.x)[i];
+          o_x[i] = fmaf(dv, skip[i], s_du[row + q][col + i].x * gbi);
+          o_d[i] = fmaf(xv, gbi, kLn2 * (&ga.x)[i]);
+          if (p.softplus) o_d[i] *= sigmoid(value4<T>(raw[q].d, i) + bias[i]);
+          if (!in[q]) o_d[i] = 0.0f;
+          if (p.z) {
+            const float zv = value4<T>(raw[q].z, i), sg = sigmoid(zv);
+            o_z[i] = value4<T>(raw[q].g, i) * sg * (1.0f + zv * (1.0f - sg)) * fmaf(skip[i], xv, (&v4.x)[i]);
+            if (!in[q]) o_z[i] = 0.0f;
+          }
+          dd[i] = fmaf(dv, xv, dd[i]);
+          dbias[i] += o_d[i];
+        }
+        const int64_t at = out_at + (int64_t)(t0 + row + q) * p.channels;
+        store4<T>(static_cast<T*>(p.dx) + at, count, whole && (p.vec & 8), o_x);
+        store4<T>(static_cast<T*>(p.ddelta) + at, count, whole && (p.vec & 8), o_d);
+        if (p.z) store4<T>(static_cast<T*>(p.dz) + at, count, whole && (p.vec & 8), o_z);
+      }
     }
     __syncthreads();
   }
   const int64_t part = (int64_t)segment * p.batch + batch;
-  if (mine) {
-    for (int nb = 0; nb < kBlocks; ++nb) {
+  for (int nb = 0; nb < kBlocks; ++nb) {
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const int n = nb * 16 + lane * S + s;
-        if (n < p.states) {
-          p.da[(part * p.channels + ch.first + c) * p.states + n] = da[nb][s];
-          if (p.dstate && segment == 0) p.dstate[state_at + n] = carry[nb][s];
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int n = nb * 16 + quad * 4 + s;
+        if (mine + j < ch.count && n < p.states) {
+          const float2 q = unpack2(da[nb][j][s / 2]), r = unpack2(carry[nb][j][s / 2]);
+          p.da[(part * p.channels + ch.first + mine + j) * p.states + n] = s % 2 ? q.y : q.x;
+          if (p.dstate && segment == 0) p.dstate[state_at + j * p.states + n] = s % 2 ? r.y : r.x;
         }
       }
     }
   }
-  // d(D) and d(bias): the 32 tokens' threads of each channel, in a fixed order
-  float* s_sum = smem;  // [kTile][2][kChannels]
+  // d(D) and d(bias): the eight pairs' threads of each channel, in a fixed order
+  float* s_sum = smem;  // [8][2][kChannels]
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    s_sum[(row * 2 + 0) * kChannels + col + i] = dd[i];
-    s_sum[(row * 2 + 1) * kChannels + col + i] = dbias[i];
+  for (int i = 0; i < 4; ++i) {
+    s_sum[(row / 2 * 2 + 0) * kChannels + col + i] = dd[i];
+    s_sum[(row / 2 * 2 + 1) * kChannels + col + i] = dbias[i];
   }
   __syncthreads();
-  if (threadIdx.x < 2 * kChannels) {
+  {
     const int which = threadIdx.x / kChannels, k = threadIdx.x % kChannels;
     float sum = 0.0f;
-    for (int t = 0; t < kTile; ++t) sum += s_sum[(t * 2 + which) * kChannels + k];
+    for (int t = 0; t < kTile / 2; ++t) sum += s_sum[(t * 2 + which) * kChannels + k];
     if (k < ch.count) p.dd[(part * 2 + which) * p.channels + ch.first + k] = sum;
   }
 }
 
 template <int kBlocks>
 constexpr int backward_smem_bytes() {
-  return (32 * (32 + 2) * 2 + 4 * 32 * 36 + 32 * 2 * 16 * kBlocks + 4 * 32 * 2 * 16) * 4;
+  return (16 * (32 + 2) * 2 + 4 * 16 * 36 + 16 * 2 * 16 * kBlocks + kBlocks * 2 * 16 * 32) * 4;
 }
 
 // dB and dC from the channel blocks' parts, in the order of the blocks.

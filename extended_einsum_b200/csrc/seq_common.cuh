@@ -173,6 +173,8 @@ __device__ __forceinline__ Raw4<T> load4_if(const T* p, bool in, int count, bool
   }
   return r;
 }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 template <typename T>
 __device__ __forceinline__ float value4(const Raw4<T>& r, int i) {
   if constexpr (__is_same(T, float))

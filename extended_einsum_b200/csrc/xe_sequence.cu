@@ -238,7 +238,7 @@ ScanPlan scan_plan(int64_t batch, int64_t length, int64_t channels, int64_t grou
   plan.channel_blocks = groups * ceil_div(channels / groups, 32);
   const int64_t blocks = plan.channel_blocks * batch;
   int64_t segments = 1;
-  if (blocks < 296) segments = std::max<int64_t>(1, std::min<int64_t>(ceil_div(592, blocks), length / 128));
+  if (blocks < 296) segments = std::max<int64_t>(1, std::min<int64_t>(592 / blocks, length / 128));
   plan.segment_length = (int)std::max<int64_t>(32, ceil_div(ceil_div(length, segments), 32) * 32);
   plan.segments = (int)std::max<int64_t>(1, ceil_div(length, plan.segment_length));
   return plan;
@@ -269,8 +269,7 @@ xe_status check_scan(const char* what, const xe_selective_scan_args* q, bool ste
   return XE_OK;
 }
 
-// `bytes`: what a kernel's vector loads need rows to be aligned to.
-ScanParams scan_params(const xe_selective_scan_args* q, int64_t bytes) {
+ScanParams scan_params(const xe_selective_scan_args* q) {
   ScanParams p{};
   p.x = q->x, p.delta = q->delta, p.z = q->z, p.b = q->b, p.c = q->c, p.y = q->y;
   p.a = q->a, p.d = q->d, p.bias = q->delta_bias;
@@ -284,12 +283,12 @@ ScanParams scan_params(const xe_selective_scan_args* q, int64_t bytes) {
   p.states = (int)q->states, p.groups = (int)q->groups;
   p.softplus = q->softplus;
   const int64_t each = q->channels / q->groups;  // a group's first channel starts a vector
-  p.vec = (aligned(bytes, q->x, q->dtype, {q->x_sb, q->x_st, each}) ? 1 : 0) |
-          (aligned(bytes, q->delta, q->dtype, {q->delta_sb, q->delta_st, each}) ? 2 : 0) |
-          (aligned(bytes, q->z, q->dtype, {q->z_sb, q->z_st, each}) ? 4 : 0) |
-          (aligned(bytes, q->y, q->dtype, {q->channels, each}) ? 8 : 0) |
-          (aligned(bytes, q->b, q->dtype, {q->b_sb, q->b_st, q->b_sg}) ? 16 : 0) |
-          (aligned(bytes, q->c, q->dtype, {q->c_sb, q->c_st, q->c_sg}) ? 32 : 0);
+  p.vec = (fours(q->x, q->dtype, {q->x_sb, q->x_st, each}) ? 1 : 0) |
+          (fours(q->delta, q->dtype, {q->delta_sb, q->delta_st, each}) ? 2 : 0) |
+          (fours(q->z, q->dtype, {q->z_sb, q->z_st, each}) ? 4 : 0) |
+          (fours(q->y, q->dtype, {q->channels, each}) ? 8 : 0) |
+          (fours(q->b, q->dtype, {q->b_sb, q->b_st, q->b_sg}) ? 16 : 0) |
+          (fours(q->c, q->dtype, {q->c_sb, q->c_st, q->c_sg}) ? 32 : 0);
   return p;
 }
 
@@ -366,7 +365,7 @@ xe_status xe_selective_scan(const xe_selective_scan_args* q, void* workspace, si
   const ScanPlan plan = scan_plan(q->batch, q->length, q->channels, q->groups);
   if (workspace_bytes < scan_segment_bytes(plan, q->batch, q->channels, q->states) || (plan.segments > 1 && !workspace))
     return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
-  ScanParams p = scan_params(q, 4 * size_of(q->dtype));  // four elements
+  ScanParams p = scan_params(q);
   scan_segments(p, plan, workspace);
   if (p.segments > 1) {
     if (xe_status s = launch_scan<xe::scan::kStates>(p, plan, q->dtype, as_stream(stream))) return s;
@@ -380,7 +379,7 @@ xe_status xe_selective_scan_step(const xe_selective_scan_args* q, void* stream) 
   if (xe_status s = check_scan(what, q, true)) return s;
   if (q->batch == 0 || q->channels == 0) return XE_OK;
   if (!q->y || !q->state_out) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
-  ScanParams p = scan_params(q, 4 * size_of(q->dtype));  // four elements
+  ScanParams p = scan_params(q);
   // bit 3: states and A in groups of four
   p.vec = reinterpret_cast<uintptr_t>(q->state_out) % 16 == 0 && reinterpret_cast<uintptr_t>(q->a) % 16 == 0 ? 8 : 0;
   constexpr int kLanes = 4;
@@ -414,13 +413,13 @@ xe_status xe_selective_scan_backward(const xe_selective_scan_args* q, const xe_s
   if (!workspace || workspace_bytes < xe_selective_scan_backward_workspace_size(q->batch, q->length, q->channels, q->states, q->groups))
     return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
   const ScanPlan plan = scan_plan(q->batch, q->length, q->channels, q->groups);
-  ScanParams p = scan_params(q, 16);  // eight elements in loads of 16 bytes
+  ScanParams p = scan_params(q);
   scan_segments(p, plan, workspace);
   p.dy = g->dy, p.dy_sb = g->dy_sb, p.dy_st = g->dy_st, p.dstate_out = g->dstate_out, p.dstate = g->dstate;
   p.dx = g->dx, p.ddelta = g->ddelta, p.dz = g->dz;
   const int64_t each = q->channels / q->groups;
-  p.vec = (p.vec & ~8) | (vectors(g->dy, q->dtype, {g->dy_sb, g->dy_st, each}) ? 64 : 0) |
-          (vectors(g->dx, q->dtype, {q->channels, each}) && vectors(g->ddelta, q->dtype, {}) && vectors(g->dz, q->dtype, {}) ? 8 : 0);
+  p.vec = (p.vec & ~8) | (fours(g->dy, q->dtype, {g->dy_sb, g->dy_st, each}) ? 64 : 0) |
+          (fours(g->dx, q->dtype, {q->channels, each}) && fours(g->ddelta, q->dtype, {}) && fours(g->dz, q->dtype, {}) ? 8 : 0);
   const int blocks = scan_blocks(q->states);
   char* at = static_cast<char*>(workspace) + scan_segment_bytes(plan, q->batch, q->channels, q->states);
   p.dbc = reinterpret_cast<float*>(at);
