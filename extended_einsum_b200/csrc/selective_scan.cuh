@@ -8,13 +8,13 @@
 // channel for softplus and the gate); the 8 bytes of x, delta, z and y of a 16-bit type take a third of
 // that time.
 //
-// Layout: a block is one warp (no barriers); four lanes share kC channels and hold S states of each,
-// 4 S >= states; states past the real ones have A = B = C = 0.  The warp stages a tile of tokens in shared
-// memory as float32, the recurrence runs over the tile from registers, and v goes back through shared
-// memory to the threads that hold the tile's x and z.  Two channels per thread because of the reads from
-// shared memory: B and C for one channel alone take the whole 128 bytes per clock at the rate of the
-// exponentials.  Tokens are staged and worked on in pairs, so that the packed instructions do two tokens
-// at a time with no copies of delta, u, B or C; only the chain h itself is scalar.
+// Layout: one warp runs the recurrence of 8 kC channels; four lanes share kC channels and hold S states of each,
+// 4 S >= states; states past the real ones have A = B = C = 0.  A second warp stages tiles of tokens in
+// shared memory as float32 and puts out the tiles that are done, so that its chains of dependent instructions
+// and its loads lie beside the recurrence's and not between its tiles: there are only one or two
+// recurrences to a scheduler to hide them.  Two channels per thread because of the reads from shared
+// memory: B and C for one channel alone take the whole 128 bytes per clock at the rate of the
+// exponentials.  The packed instructions take two states at a time.
 //
 // Few channels: the length is split into segments.  A first pass runs each segment from a zero state
 // and keeps its last state and sum of delta (the product of its e is exp(A sum delta)), a second
@@ -94,7 +94,7 @@ __device__ __forceinline__ float transpose_sum(float (&v)[kLanes], int lane) {
 enum Mode { kFull, kStates, kAdjoint };
 
 template <typename T, int S, int kC, Mode kMode>
-__global__ void __launch_bounds__(32) selective_scan_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(64) selective_scan_kernel(const __grid_constant__ Params p) {
   constexpr bool kStateOnly = kMode != kFull;
   constexpr int kLanes = 4;                     // lanes on a channel
   constexpr int kChannels = 32 / kLanes * kC;   // of the warp
@@ -106,10 +106,10 @@ __global__ void __launch_bounds__(32) selective_scan_kernel(const __grid_constan
   constexpr int kParts = kMode == kFull ? 2 : 1;               // B and C, or the one that is needed
   constexpr int kEach = kPairs * kParts * (NP / 4) / 32;       // their quads of states per thread
   static_assert(kPairs * kParts * (NP / 4) % 32 == 0 && kTile % kRun == 0 && kCheckpoint % kRun == 0, "whole turns");
-  // per pair of tokens t, t + 1 and channel: delta_t, delta_{t+1}, u_t, u_{t+1}; u = delta x, or the adjoint's dv
-  __shared__ __align__(16) float4 s_du[kPairs][kChannels + 1];
-  __shared__ __align__(16) float2 s_bc[kPairs * kParts * NP];          // (t, t + 1) of each state
-  __shared__ __align__(16) float2 s_v[kStateOnly ? 1 : kPairs][kChannels + 2];
+  // two tiles: (delta, u) of each channel, u = delta x, or the adjoint's dv; B and C; v
+  __shared__ __align__(16) float2 s_du[2][kTile][kChannels + 2];
+  __shared__ __align__(16) float s_bc[2][kTile * kParts * NP];
+  __shared__ __align__(16) float s_v[2][kStateOnly ? 1 : kTile][kChannels + 4];
   const Channels ch = block_channels(p, kChannels);
   // the first segment needs no adjoint from zero, the last one no state
   const int batch = blockIdx.y, segment = blockIdx.z + (kMode == kAdjoint ? 1 : 0);
@@ -118,18 +118,31 @@ __global__ void __launch_bounds__(32) selective_scan_kernel(const __grid_constan
   const int live = min(end, sequence_length(p.lengths, p.lengths64, batch, p.length));
   const int tiles = (end - begin + kTile - 1) / kTile;
   const int step = kMode == kAdjoint ? -kTile : kTile;
-  int t0 = kMode == kAdjoint ? begin + (tiles - 1) * kTile : begin;
+  const int t_first = kMode == kAdjoint ? begin + (tiles - 1) * kTile : begin;
+  // One warp runs the recurrence, the other one stages.  Which of the two is a matter of speed alone: a block's
+  // warps go to neighbouring schedulers, and were it always the first, half of the schedulers would run all
+  // the recurrences; so it changes with every second pair of warp slots.
+  __shared__ int s_role;
+  if (threadIdx.x == 0) {
+    uint32_t slot;
+    asm volatile("mov.u32 %0, %%warpid;" : "=r"(slot));
+    s_role = slot >> 2 & 1;
+  }
+  __syncthreads();
+  const bool runs = threadIdx.x / 32 == s_role;
+  const int thread = threadIdx.x % 32;
 
+  if (!runs) {
   // staging: this thread's pair of tokens and four channels; the places of the next loads move by a tile at a time
-  const int row = threadIdx.x / kQuads * 2;
-  const int col = threadIdx.x % kQuads * 4;
+  const int row = thread / kQuads * 2;
+  const int col = thread % kQuads * 4;
   const int count = max(0, min(4, ch.count - col));
   const int64_t x_st = kMode == kAdjoint ? p.dy_st : p.x_st;
   const T* x = kMode == kAdjoint ? static_cast<const T*>(p.dy) + batch * p.dy_sb : static_cast<const T*>(p.x) + batch * p.x_sb;
-  x += ch.first + col + (t0 + row) * x_st;
-  const T* delta = static_cast<const T*>(p.delta) + batch * p.delta_sb + ch.first + col + (t0 + row) * p.delta_st;
-  const T* z = static_cast<const T*>(p.z) + batch * p.z_sb + ch.first + col + (t0 + row) * p.z_st;
-  T* y = static_cast<T*>(p.y) + ((int64_t)batch * p.length + t0 + row) * p.channels + ch.first + col;
+  x += ch.first + col + (t_first + row) * x_st;
+  const T* delta = static_cast<const T*>(p.delta) + batch * p.delta_sb + ch.first + col + (t_first + row) * p.delta_st;
+  const T* z = static_cast<const T*>(p.z) + batch * p.z_sb + ch.first + col + (t_first + row) * p.z_st;
+  T* y = static_cast<T*>(p.y) + ((int64_t)batch * p.length + t_first + row) * p.channels + ch.first + col;
   const bool whole_x = (p.vec & (kMode == kAdjoint ? 64 : 1)) && count == 4, whole_d = (p.vec & 2) && count == 4;
   const bool whole_z = (p.vec & 4) && count == 4, whole_y = (p.vec & 8) && count == 4;
   const T* shared_at[kEach];  // B and C: pair of tokens, which of the two, four states
@@ -137,14 +150,14 @@ __global__ void __launch_bounds__(32) selective_scan_kernel(const __grid_constan
   bool whole_s[kEach];
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    const int i = k * 32 + threadIdx.x;
+    const int i = k * 32 + thread;
     const int n0 = i % (NP / 4) * 4;
     const bool second = kMode == kAdjoint || (kParts == 2 && i / (NP / 4) % 2);
     shared_t[k] = i / (NP / 4 * kParts) * 2;
     shared_n[k] = max(0, min(4, p.states - n0));
     whole_s[k] = (p.vec & (second ? 32 : 16)) && (shared_n[k] == 4 || shared_n[k] == 0);
-    shared_at[k] = second ? static_cast<const T*>(p.c) + batch * p.c_sb + ch.group * p.c_sg + n0 + (t0 + shared_t[k]) * p.c_st
-                          : static_cast<const T*>(p.b) + batch * p.b_sb + ch.group * p.b_sg + n0 + (t0 + shared_t[k]) * p.b_st;
+    shared_at[k] = second ? static_cast<const T*>(p.c) + batch * p.c_sb + ch.group * p.c_sg + n0 + (t_first + shared_t[k]) * p.c_st
+                          : static_cast<const T*>(p.b) + batch * p.b_sb + ch.group * p.b_sg + n0 + (t_first + shared_t[k]) * p.b_st;
   }
   float bias[4], skip[4];
 #pragma unroll
@@ -153,33 +166,10 @@ __global__ void __launch_bounds__(32) selective_scan_kernel(const __grid_constan
     skip[i] = !kStateOnly && p.d && i < count ? p.d[ch.first + col + i] : 0.0f;
   }
 
-  // recurrence: this thread's kC channels and S states of each
-  const int mine = threadIdx.x / kLanes * kC, lane = threadIdx.x % kLanes;
-  F2 a[kC][S];  // twice, for two tokens at a time
-  float h[kC][S];
-  const int64_t state_at = ((int64_t)batch * p.channels + ch.first + mine) * p.states + lane * S;
-#pragma unroll
-  for (int j = 0; j < kC; ++j) {
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const bool in = mine + j < ch.count && lane * S + s < p.states;
-      a[j][s] = both(in ? p.a[(int64_t)(ch.first + mine + j) * p.states + lane * S + s] * kLog2e : 0.0f);
-      h[j][s] = 0.0f;
-      if (!kStateOnly && in) {
-        if (p.segments > 1)
-          h[j][s] = p.segment_state[(int64_t)segment * p.batch * p.channels * p.states + state_at + j * p.states + s];
-        else if (p.state)
-          h[j][s] = p.state[state_at + j * p.states + s];
-      }
-    }
-  }
-  F2 delta_sum[kC] = {};
-  const int64_t checkpoint_rows = (p.length + kCheckpoint - 1) / kCheckpoint;
-  float* checkpoints = p.checkpoints + ((int64_t)batch * checkpoint_rows * p.channels + ch.first + mine) * NP + lane * S;
-
-  struct {
+  struct Loaded {
     Raw4<T> x, d, z;
-  } next[2];
+  };
+  Loaded next[2], staged[2], shown[2];  // of the tiles to come, on hand and to be put out
   Raw4<T> next_s[kEach][2];
   auto fetch = [&](int at) {
 #pragma unroll
@@ -194,7 +184,7 @@ __global__ void __launch_bounds__(32) selective_scan_kernel(const __grid_constan
     z += step * p.z_st;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-      const bool second = kMode == kAdjoint || (kParts == 2 && (k * 32 + threadIdx.x) / (NP / 4) % 2);
+      const bool second = kMode == kAdjoint || (kParts == 2 && (k * 32 + thread) / (NP / 4) % 2);
       const int64_t st = second ? p.c_st : p.b_st;
 #pragma unroll
       for (int q = 0; q < 2; ++q)
@@ -202,14 +192,13 @@ __global__ void __launch_bounds__(32) selective_scan_kernel(const __grid_constan
       shared_at[k] += step * st;
     }
   };
-  if (tiles > 0) fetch(t0);
-  for (int tile = 0; tile < tiles; ++tile, t0 += step) {
+  auto stage = [&](int tile) {
+    const int t0 = t_first + tile * step;
     const bool in[2] = {t0 + row < live, t0 + row + 1 < live};
-    F2 xv[4];
-    Raw4<T> z_raw[2] = {next[0].z, next[1].z};
+    float2 du[2][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      xv[i] = pack2(value4<T>(next[0].x, i), value4<T>(next[1].x, i));
+      const F2 xv = pack2(value4<T>(next[0].x, i), value4<T>(next[1].x, i));
       F2 d = add2(pack2(value4<T>(next[0].d, i), value4<T>(next[1].d, i)), both(bias[i]));
       if (p.softplus) d = softplus2(d);
       float2 dd = unpack2(d);
@@ -217,102 +206,42 @@ __global__ void __launch_bounds__(32) selective_scan_kernel(const __grid_constan
       if (!in[1]) dd.y = 0.0f;
       F2 u;
       if (kMode == kAdjoint)
-        u = p.z ? gate2(xv[i], pack2(value4<T>(z_raw[0], i), value4<T>(z_raw[1], i))) : xv[i];
+        u = p.z ? gate2(xv, pack2(value4<T>(next[0].z, i), value4<T>(next[1].z, i))) : xv;
       else
-        u = mul2(pack2(dd.x, dd.y), xv[i]);
+        u = mul2(pack2(dd.x, dd.y), xv);
       const float2 uu = unpack2(u);
-      s_du[row / 2][col + i] = make_float4(dd.x, dd.y, uu.x, uu.y);
+      du[0][i] = make_float2(dd.x, uu.x);
+      du[1][i] = make_float2(dd.y, uu.y);
     }
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      float4* at = reinterpret_cast<float4*>(s_bc + (k * 32 + threadIdx.x) * 4);
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int i = 0; i < 4; i += 2)
-        at[i / 2] = make_float4(value4<T>(next_s[k][0], i), value4<T>(next_s[k][1], i), value4<T>(next_s[k][0], i + 1),
-                                value4<T>(next_s[k][1], i + 1));
+        *reinterpret_cast<float4*>(&s_du[tile & 1][row + q][col + i]) =
+            make_float4(du[q][i].x, du[q][i].y, du[q][i + 1].x, du[q][i + 1].y);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int i = k * 32 + thread;  // pair of tokens, which of the two, four states
+      float* at = s_bc[tile & 1] + ((i / (NP / 4 * kParts) * 2) * kParts + i / (NP / 4) % kParts) * NP + i % (NP / 4) * 4;
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        *reinterpret_cast<float4*>(at + q * kParts * NP) = make_float4(
+            value4<T>(next_s[k][q], 0), value4<T>(next_s[k][q], 1), value4<T>(next_s[k][q], 2), value4<T>(next_s[k][q], 3));
     }
-    __syncwarp();
-    if (tile + 1 < tiles) fetch(t0 + step);
-    if (t0 < live || (!kStateOnly && p.checkpoints)) {
-#pragma unroll 1
-      for (int t1 = 0; t1 < kTile; t1 += kRun) {
-        if (!kStateOnly && p.checkpoints && (t0 + t1) % kCheckpoint == 0 && t0 + t1 < p.length) {
-#pragma unroll
-          for (int j = 0; j < kC; ++j) {
-            float* at = checkpoints + ((int64_t)((t0 + t1) / kCheckpoint) * p.channels + j) * NP;
-            if (mine + j < ch.count) {
-#pragma unroll
-              for (int s = 0; s < S; s += 4)
-                *reinterpret_cast<float4*>(at + s) = make_float4(h[j][s], h[j][s + 1], h[j][s + 2], h[j][s + 3]);
-            }
-          }
-        }
-#pragma unroll
-        for (int t2 = 0; t2 < kRun; t2 += 4) {
-          float v[kC][4];
-#pragma unroll
-          for (int k = 0; k < 4; k += 2) {
-            const int pair = (kMode == kAdjoint ? kTile - 2 - (t1 + t2 + k) : t1 + t2 + k) / 2;
-            // B, or C in the adjoint recurrence
-            const ulonglong2* bv = reinterpret_cast<const ulonglong2*>(s_bc + (pair * kParts) * NP + lane * S);
-            const ulonglong2* cv = bv + NP / 2;
-            ulonglong2 du[kC];
-            F2 sum[kC];
-#pragma unroll
-            for (int j = 0; j < kC; ++j) {
-              du[j] = *reinterpret_cast<const ulonglong2*>(&s_du[pair][mine + j]);
-              if (kStateOnly) delta_sum[j] = add2(delta_sum[j], du[j].x);
-            }
-#pragma unroll
-            for (int s = 0; s < S; ++s) {
-              const F2 b2 = s % 2 ? bv[s / 2].y : bv[s / 2].x;
-#pragma unroll
-              for (int j = 0; j < kC; ++j) {
-                const float2 e = unpack2(exp2_fast2(mul2(du[j].x, a[j][s])));
-                const float2 u = unpack2(mul2(du[j].y, b2));
-                if (kMode == kAdjoint) {
-                  h[j][s] = e.y * (h[j][s] + u.y);
-                  h[j][s] = e.x * (h[j][s] + u.x);
-                } else {
-                  const float first = fmaf(e.x, h[j][s], u.x);
-                  h[j][s] = fmaf(e.y, first, u.y);
-                  if (!kStateOnly) {
-                    const F2 c2 = s % 2 ? cv[s / 2].y : cv[s / 2].x;
-                    const F2 hh = pack2(first, h[j][s]);
-                    sum[j] = s == 0 ? mul2(c2, hh) : fma2(c2, hh, sum[j]);
-                  }
-                }
-              }
-            }
-            if (!kStateOnly) {
-#pragma unroll
-              for (int j = 0; j < kC; ++j) {
-                const float2 q = unpack2(sum[j]);
-                v[j][k] = q.x, v[j][k + 1] = q.y;
-              }
-            }
-          }
-          if (!kStateOnly) {
-            float* at = reinterpret_cast<float*>(&s_v[(t1 + t2 + lane) / 2][mine]) + lane % 2;
-#pragma unroll
-            for (int j = 0; j < kC; ++j) at[2 * j] = transpose_sum<4>(v[j], lane);
-          }
-        }
-      }
-    }
-    __syncwarp();
+  };
+  auto put_out = [&](int tile) {
     if (!kStateOnly) {
+      const int t0 = t_first + tile * step;
+      const bool in[2] = {t0 + row < live, t0 + row + 1 < live};
       float o[2][4];
+      const float4 v0 = *reinterpret_cast<const float4*>(&s_v[tile & 1][row][col]);
+      const float4 v1 = *reinterpret_cast<const float4*>(&s_v[tile & 1][row + 1][col]);
 #pragma unroll
-      for (int i = 0; i < 4; i += 2) {
-        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(&s_v[row / 2][col + i]);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          F2 v = fma2(both(skip[i + k]), xv[i + k], k ? q.y : q.x);
-          if (p.z) v = gate2(v, pack2(value4<T>(z_raw[0], i + k), value4<T>(z_raw[1], i + k)));
-          const float2 f = unpack2(v);
-          o[0][i + k] = f.x, o[1][i + k] = f.y;
-        }
+      for (int i = 0; i < 4; ++i) {
+        F2 v = fma2(both(skip[i]), pack2(value4<T>(shown[0].x, i), value4<T>(shown[1].x, i)), pack2((&v0.x)[i], (&v1.x)[i]));
+        if (p.z) v = gate2(v, pack2(value4<T>(shown[0].z, i), value4<T>(shown[1].z, i)));
+        const float2 f = unpack2(v);
+        o[0][i] = f.x, o[1][i] = f.y;
       }
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
@@ -322,9 +251,125 @@ __global__ void __launch_bounds__(32) selective_scan_kernel(const __grid_constan
         }
       }
       y += (int64_t)kTile * p.channels;
-      __syncwarp();
+    }
+  };
+  if (tiles > 0) {
+    fetch(t_first);
+    stage(0);
+  }
+  for (int tile = 0; tile < tiles; ++tile) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      shown[q] = staged[q];
+      staged[q] = next[q];
+    }
+    if (tile + 1 < tiles) fetch(t_first + (tile + 1) * step);
+    __syncthreads();
+    if (tile > 0) put_out(tile - 1);
+    if (tile + 1 < tiles) stage(tile + 1);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 2; ++q) shown[q] = staged[q];
+  if (tiles > 0) put_out(tiles - 1);
+  return;
+  }
+
+  // recurrence: this thread's kC channels and S states of each
+  const int mine = thread / kLanes * kC, lane = thread % kLanes;
+  F2 a[kC][S / 2], h[kC][S / 2];
+  const int64_t state_at = ((int64_t)batch * p.channels + ch.first + mine) * p.states + lane * S;
+#pragma unroll
+  for (int j = 0; j < kC; ++j) {
+    float a1[S], h1[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const bool in = mine + j < ch.count && lane * S + s < p.states;
+      a1[s] = in ? p.a[(int64_t)(ch.first + mine + j) * p.states + lane * S + s] * kLog2e : 0.0f;
+      h1[s] = 0.0f;
+      if (!kStateOnly && in) {
+        if (p.segments > 1)
+          h1[s] = p.segment_state[(int64_t)segment * p.batch * p.channels * p.states + state_at + j * p.states + s];
+        else if (p.state)
+          h1[s] = p.state[state_at + j * p.states + s];
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < S / 2; ++s) {
+      a[j][s] = pack2(a1[2 * s], a1[2 * s + 1]);
+      h[j][s] = pack2(h1[2 * s], h1[2 * s + 1]);
     }
   }
+  float delta_sum[kC] = {};
+  const int64_t checkpoint_rows = (p.length + kCheckpoint - 1) / kCheckpoint;
+  float* checkpoints = p.checkpoints + ((int64_t)batch * checkpoint_rows * p.channels + ch.first + mine) * NP + lane * S;
+
+  for (int tile = 0; tile < tiles; ++tile) {
+    __syncthreads();
+    const int t0 = t_first + tile * step;
+    if (t0 < live || (!kStateOnly && p.checkpoints)) {
+#pragma unroll
+      for (int t1 = 0; t1 < kTile; t1 += kRun) {
+        if (!kStateOnly && p.checkpoints && (t0 + t1) % kCheckpoint == 0 && t0 + t1 < p.length) {
+#pragma unroll
+          for (int j = 0; j < kC; ++j) {
+            float* at = checkpoints + ((int64_t)((t0 + t1) / kCheckpoint) * p.channels + j) * NP;
+            if (mine + j < ch.count) {
+#pragma unroll
+              for (int s = 0; s < S / 2; s += 2)
+                *reinterpret_cast<ulonglong2*>(at + 2 * s) = make_ulonglong2(h[j][s], h[j][s + 1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int t2 = 0; t2 < kRun; t2 += 4) {
+          float v[kC][4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int t = kMode == kAdjoint ? kTile - 1 - (t1 + t2 + k) : t1 + t2 + k;
+            float2 du[kC];
+            if constexpr (kC == 2)
+              *reinterpret_cast<float4*>(du) = *reinterpret_cast<const float4*>(&s_du[tile & 1][t][mine]);
+            else
+              du[0] = s_du[tile & 1][t][mine];
+            // B, or C in the adjoint recurrence
+            const ulonglong2* bv = reinterpret_cast<const ulonglong2*>(s_bc[tile & 1] + t * kParts * NP + lane * S);
+            const ulonglong2* cv = bv + NP / 4;
+#pragma unroll
+            for (int j = 0; j < kC; ++j) {
+              const F2 d2 = both(du[j].x), u2 = both(du[j].y);
+              F2 sum = 0;
+              if (kStateOnly) delta_sum[j] += du[j].x;
+#pragma unroll
+              for (int s = 0; s < S / 2; ++s) {
+                const F2 e = exp2_fast2(mul2(d2, a[j][s])), b2 = s % 2 ? bv[s / 2].y : bv[s / 2].x;
+                if (kMode == kAdjoint)
+                  h[j][s] = mul2(e, fma2(u2, b2, h[j][s]));
+                else
+                  h[j][s] = fma2(e, h[j][s], mul2(u2, b2));
+                if (!kStateOnly) {
+                  const F2 c2 = s % 2 ? cv[s / 2].y : cv[s / 2].x;
+                  sum = s == 0 ? mul2(c2, h[j][s]) : fma2(c2, h[j][s], sum);
+                }
+              }
+              if (!kStateOnly) {
+                const float2 q = unpack2(sum);
+                v[j][k] = q.x + q.y;
+              }
+            }
+          }
+          if (!kStateOnly) {
+            float* at = &s_v[tile & 1][t1 + t2 + lane][mine];
+            if constexpr (kC == 2)
+              *reinterpret_cast<float2*>(at) = make_float2(transpose_sum<4>(v[0], lane), transpose_sum<4>(v[1], lane));
+            else
+              at[0] = transpose_sum<4>(v[0], lane);
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < kC; ++j) {
     if (mine + j >= ch.count) continue;
@@ -335,13 +380,13 @@ __global__ void __launch_bounds__(32) selective_scan_kernel(const __grid_constan
       out = p.state_out + state_at + j * p.states;
     if (out) {
 #pragma unroll
-      for (int s = 0; s < S; ++s)
-        if (lane * S + s < p.states) out[s] = h[j][s];
+      for (int s = 0; s < S; ++s) {
+        const float2 q = unpack2(h[j][s / 2]);
+        if (lane * S + s < p.states) out[s] = s % 2 ? q.y : q.x;
+      }
     }
-    if (kStateOnly && lane == 0) {
-      const float2 q = unpack2(delta_sum[j]);
-      p.segment_delta[((int64_t)segment * p.batch + batch) * p.channels + ch.first + mine + j] = q.x + q.y;
-    }
+    if (kStateOnly && lane == 0)
+      p.segment_delta[((int64_t)segment * p.batch + batch) * p.channels + ch.first + mine + j] = delta_sum[j];
   }
 }
 

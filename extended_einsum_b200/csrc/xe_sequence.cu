@@ -309,11 +309,11 @@ xe_status launch_scan(const ScanParams& p, const ScanPlan& plan, int32_t dtype, 
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
     if (p.states <= 16)
-      selective_scan_kernel<T, 4, 2, kMode><<<grid, 32, 0, stream>>>(p);
+      selective_scan_kernel<T, 4, 2, kMode><<<grid, 64, 0, stream>>>(p);
     else if (p.states <= 32)
-      selective_scan_kernel<T, 8, 2, kMode><<<grid, 32, 0, stream>>>(p);
+      selective_scan_kernel<T, 8, 2, kMode><<<grid, 64, 0, stream>>>(p);
     else
-      selective_scan_kernel<T, 16, 1, kMode><<<grid, 32, 0, stream>>>(p);
+      selective_scan_kernel<T, 16, 1, kMode><<<grid, 64, 0, stream>>>(p);
   });
   return launched("selective scan");
 }
