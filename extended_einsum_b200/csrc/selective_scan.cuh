@@ -757,55 +757,70 @@ __global__ void __launch_bounds__(256) selective_scan_dbc_kernel(const float* pa
   (which ? dc : db)[(token * groups + group) * states + n] = from_f32<T>(sum);
 }
 
-// One token: every state is read and written once, kLanes lanes on a channel.
-template <typename T, int kLanes>
-__global__ void __launch_bounds__(128) selective_scan_step_kernel(Params p) {
-  const int64_t at = (int64_t)blockIdx.x * (blockDim.x / kLanes) + threadIdx.x / kLanes;
+// One token: every state is read and written once, four lanes on a channel with four states at a time.  The
+// first four states' loads and those of everything else go out together; `four`: states, A, B and C come
+// in aligned groups of four.
+template <typename T>
+__global__ void __launch_bounds__(128) selective_scan_step_kernel(const __grid_constant__ Params p, int four) {
+  constexpr int kLanes = 4;
+  const int64_t at = (int64_t)blockIdx.x * (128 / kLanes) + threadIdx.x / kLanes;
   const int lane = threadIdx.x % kLanes;
   const bool in = at < (int64_t)p.batch * p.channels;
   const int b = in ? (int)(at / p.channels) : 0;
-  const int c = in ? (int)(at % p.channels) : 0;
-  const int group = c / (p.channels / p.groups);
-  const float x = to_f32(static_cast<const T*>(p.x)[b * p.x_sb + c]);
-  float delta = to_f32(static_cast<const T*>(p.delta)[b * p.delta_sb + c]) + (p.bias ? p.bias[c] : 0.0f);
-  if (p.softplus) delta = softplus(delta);
+  const int c = in ? (int)(at - (int64_t)b * p.channels) : 0;
+  const int group = p.groups == 1 ? 0 : c / (p.channels / p.groups);
   const T* bv = static_cast<const T*>(p.b) + b * p.b_sb + group * p.b_sg;
   const T* cv = static_cast<const T*>(p.c) + b * p.c_sb + group * p.c_sg;
+  float* state = p.state_out + at * p.states;
+  const float* a = p.a + (int64_t)c * p.states;
+  float4 h4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), a4 = h4;
+  Raw4<T> b4, c4;
+  const bool first = in && four && lane * 4 < p.states;
+  if (first) {
+    h4 = *reinterpret_cast<const float4*>(state + lane * 4);
+    a4 = *reinterpret_cast<const float4*>(a + lane * 4);
+  }
+  b4 = load4_if<T>(bv + lane * 4, first, 4, true);
+  c4 = load4_if<T>(cv + lane * 4, first, 4, true);
+  const float x = to_f32(static_cast<const T*>(p.x)[b * p.x_sb + c]);
+  float delta = to_f32(static_cast<const T*>(p.delta)[b * p.delta_sb + c]) + (p.bias ? p.bias[c] : 0.0f);
+  const float zv = p.z ? to_f32(static_cast<const T*>(p.z)[b * p.z_sb + c]) : 0.0f;
+  const float skip = p.d ? p.d[c] : 0.0f;
+  if (p.softplus) delta = softplus(delta);
+  const float u = delta * x, d2 = delta * kLog2e;
   float v = 0.0f;
-  if (in) {
-    float* state = p.state_out + at * p.states;
-    const float* a = p.a + (int64_t)c * p.states;
-    const bool four = p.states % 4 == 0 && (p.vec & 8);
-    if (four) {
-      for (int n = lane * 4; n < p.states; n += kLanes * 4) {
-        float4 h = *reinterpret_cast<const float4*>(state + n);
-        const float4 r = *reinterpret_cast<const float4*>(a + n);
-        h.x = fmaf(exp2_fast(delta * kLog2e * r.x), h.x, delta * x * to_f32(bv[n]));
-        h.y = fmaf(exp2_fast(delta * kLog2e * r.y), h.y, delta * x * to_f32(bv[n + 1]));
-        h.z = fmaf(exp2_fast(delta * kLog2e * r.z), h.z, delta * x * to_f32(bv[n + 2]));
-        h.w = fmaf(exp2_fast(delta * kLog2e * r.w), h.w, delta * x * to_f32(bv[n + 3]));
-        v = fmaf(to_f32(cv[n]), h.x, v);
-        v = fmaf(to_f32(cv[n + 1]), h.y, v);
-        v = fmaf(to_f32(cv[n + 2]), h.z, v);
-        v = fmaf(to_f32(cv[n + 3]), h.w, v);
-        *reinterpret_cast<float4*>(state + n) = h;
-      }
-    } else {
-      for (int n = lane; n < p.states; n += kLanes) {
-        const float h = fmaf(exp2_fast(delta * kLog2e * a[n]), state[n], delta * x * to_f32(bv[n]));
-        v = fmaf(to_f32(cv[n]), h, v);
-        state[n] = h;
-      }
+  auto quad = [&](int n) {
+    h4.x = fmaf(exp2_fast(d2 * a4.x), h4.x, u * value4<T>(b4, 0));
+    h4.y = fmaf(exp2_fast(d2 * a4.y), h4.y, u * value4<T>(b4, 1));
+    h4.z = fmaf(exp2_fast(d2 * a4.z), h4.z, u * value4<T>(b4, 2));
+    h4.w = fmaf(exp2_fast(d2 * a4.w), h4.w, u * value4<T>(b4, 3));
+    *reinterpret_cast<float4*>(state + n) = h4;
+    v = fmaf(value4<T>(c4, 0), h4.x, v);
+    v = fmaf(value4<T>(c4, 1), h4.y, v);
+    v = fmaf(value4<T>(c4, 2), h4.z, v);
+    v = fmaf(value4<T>(c4, 3), h4.w, v);
+  };
+  if (first) {
+    quad(lane * 4);
+    for (int n = (lane + kLanes) * 4; n < p.states; n += kLanes * 4) {
+      h4 = *reinterpret_cast<const float4*>(state + n);
+      a4 = *reinterpret_cast<const float4*>(a + n);
+      b4 = load4_if<T>(bv + n, true, 4, true);
+      c4 = load4_if<T>(cv + n, true, 4, true);
+      quad(n);
+    }
+  } else if (in && !four) {
+    for (int n = lane; n < p.states; n += kLanes) {
+      const float h = fmaf(exp2_fast(d2 * a[n]), state[n], u * to_f32(bv[n]));
+      v = fmaf(to_f32(cv[n]), h, v);
+      state[n] = h;
     }
   }
 #pragma unroll
   for (int o = 1; o < kLanes; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (in && lane == 0) {
-    if (p.d) v = fmaf(p.d[c], x, v);
-    if (p.z) {
-      const float zv = to_f32(static_cast<const T*>(p.z)[b * p.z_sb + c]);
-      v *= zv * sigmoid(zv);
-    }
+    v = fmaf(skip, x, v);
+    if (p.z) v *= zv * sigmoid(zv);
     static_cast<T*>(p.y)[at] = from_f32<T>(v);
   }
 }

@@ -380,13 +380,14 @@ xe_status xe_selective_scan_step(const xe_selective_scan_args* q, void* stream) 
   if (q->batch == 0 || q->channels == 0) return XE_OK;
   if (!q->y || !q->state_out) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   ScanParams p = scan_params(q);
-  // bit 3: states and A in groups of four
-  p.vec = reinterpret_cast<uintptr_t>(q->state_out) % 16 == 0 && reinterpret_cast<uintptr_t>(q->a) % 16 == 0 ? 8 : 0;
-  constexpr int kLanes = 4;
-  const int64_t blocks = ceil_div(q->batch * q->channels, 128 / kLanes);
+  // states, A, B and C in aligned groups of four
+  const int four = q->states % 4 == 0 && reinterpret_cast<uintptr_t>(q->state_out) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(q->a) % 16 == 0 && fours(q->b, q->dtype, {q->b_sb, q->b_sg}) &&
+                   fours(q->c, q->dtype, {q->c_sb, q->c_sg});
+  const int64_t blocks = ceil_div(q->batch * q->channels, 32);
   if (blocks > INT_MAX) return fail(XE_ERR_NOT_SUPPORTED, "%s: a size is above its limit", what);
   by_type(q->dtype, [&](auto t) {
-    xe::scan::selective_scan_step_kernel<decltype(t), kLanes><<<(unsigned)blocks, 128, 0, as_stream(stream)>>>(p);
+    xe::scan::selective_scan_step_kernel<decltype(t)><<<(unsigned)blocks, 128, 0, as_stream(stream)>>>(p, four);
   });
   return launched(what);
 }

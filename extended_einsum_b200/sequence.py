@@ -66,13 +66,23 @@ def _pointer(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_entries: dict[str, object] = {}
+
+
+def _entry(name: str):
+    entry = _entries.get(name)
+    if entry is None:
+        entry = _entries[name] = getattr(_lib.load(), name)
+    return entry
+
+
 def _call(device: torch.device, name: str, *args) -> None:
     """Calls an entry point on the device's current stream (its last argument)."""
     index = device.index
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return _call(device, name, *args)
-    status = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    status = _entry(name)(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _lib.check(status, name)
 
@@ -211,7 +221,7 @@ def causal_conv1d_backward(x, weight, bias, state, activation, lengths, dy, dsta
     if dstate_out is not None:
         dstate_out = _operand(what, "the state's gradient", dstate_out, x, (batch, width - 1, channels), x.dtype).contiguous()
     dweight = torch.empty((width + 1, channels), device=x.device, dtype=torch.float32)
-    size = _lib.load().xe_causal_conv1d_backward_workspace_size(batch, length, channels, width)
+    size = _entry("xe_causal_conv1d_backward_workspace_size")(batch, length, channels, width)
     workspace = _workspace(size, x.device)
     _call(
         x.device, "xe_causal_conv1d_backward", x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _pointer(bias),
@@ -312,7 +322,6 @@ def _scan_forward(x, delta, a, b, c, d, z, delta_bias, softplus, state, lengths,
     x = kept[0]
     batch, length, channels = x.shape
     states = a.shape[1]
-    lib = _lib.load()
     y = _like(x)
     args.y = y.data_ptr()
     new = checkpoints = None
@@ -320,10 +329,10 @@ def _scan_forward(x, delta, a, b, c, d, z, delta_bias, softplus, state, lengths,
         new = torch.empty((batch, channels, states), device=x.device, dtype=torch.float32)
         args.state_out = new.data_ptr()
     if training:
-        size = lib.xe_selective_scan_checkpoint_size(batch, length, channels, states)
+        size = _entry("xe_selective_scan_checkpoint_size")(batch, length, channels, states)
         checkpoints = torch.empty(size // 4, device=x.device, dtype=torch.float32)
         args.checkpoints = checkpoints.data_ptr()
-    size = lib.xe_selective_scan_workspace_size(batch, length, channels, states, groups)
+    size = _entry("xe_selective_scan_workspace_size")(batch, length, channels, states, groups)
     workspace = _workspace(size, x.device)
     _call(x.device, "xe_selective_scan", args, _pointer(workspace), size)
     return y, new, checkpoints
@@ -411,7 +420,7 @@ def selective_scan_backward(x, delta, a, b, c, d, z, delta_bias, softplus, state
             dy.data_ptr(), _pointer(dstate_out), dx.data_ptr(), ddelta.data_ptr(), _pointer(dz), db.data_ptr(),
             dc.data_ptr(), da.data_ptr(), dd.data_ptr(), _pointer(dstate), dy.stride(0), dy.stride(1),
         )
-        size = _lib.load().xe_selective_scan_backward_workspace_size(batch, length, channels, states, groups)
+        size = _entry("xe_selective_scan_backward_workspace_size")(batch, length, channels, states, groups)
         workspace = _workspace(size, device)
         _call(device, "xe_selective_scan_backward", args, grads, _pointer(workspace), size)
     else:
@@ -521,7 +530,7 @@ def rms_norm_backward(total, addend, weight, dy, dtotal, eps, need_dweight):
         return dx, None if dweight is None else dweight.zero_()
     if weight is not None:
         weight = weight.contiguous()
-    size = _lib.load().xe_rms_norm_backward_workspace_size(rows.shape[0], columns) if need_dweight else 0
+    size = _entry("xe_rms_norm_backward_workspace_size")(rows.shape[0], columns) if need_dweight else 0
     workspace = _workspace(size, device)
     _call(
         device, "xe_rms_norm_backward", rows.data_ptr(), rows.stride(0), _pointer(addend),
@@ -588,7 +597,7 @@ def int4_linear(
     if x_scale is not None:
         x_scale = _operand(what, "x_scale", x_scale, x, x.shape[:-1], torch.float32).contiguous() if x.dim() > 1 else x_scale
     y = torch.empty((*x.shape[:-1], outputs), device=device, dtype=dtype)
-    size = _lib.load().xe_int4_linear_workspace_size(rows.shape[0], inputs, outputs, code)
+    size = _entry("xe_int4_linear_workspace_size")(rows.shape[0], inputs, outputs, code)
     workspace = _workspace(size, device)
     _call(
         device, "xe_int4_linear", rows.data_ptr(), rows.stride(0), _pointer(x_scale), packed.data_ptr(), packed.stride(0),
