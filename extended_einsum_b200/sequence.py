@@ -97,7 +97,7 @@ def _like(x: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
 def _needs_grad(*tensors: torch.Tensor | None) -> bool:
     if torch.is_grad_enabled():
         for t in tensors:
-            if t is not None and t.requires_grad:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
                 return True
     return False
 
