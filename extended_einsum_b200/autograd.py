@@ -305,52 +305,51 @@ class CausalConv1d(torch.autograd.Function):
     """(y, new state) of the causal convolution; the state's gradient joins those of the last inputs."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, state, activation, lengths):
-        y, new = ops.causal_conv1d(
-            x, weight, bias, activation=activation, state=state, lengths=lengths, return_state=True)
+    def forward(ctx, x, weight, bias, state, activation, lengths, return_state: bool):
+        y, new = sequence._conv_forward(x, weight, bias, activation, state, lengths, return_state)
         ctx.save_for_backward(x, weight, bias, state, lengths)
         ctx.activation = activation
         ctx.set_materialize_grads(False)
-        return y, new
+        return (y, new) if return_state else y
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dy, dnew):
+    def backward(ctx, dy, dnew=None):
         if dy is None and dnew is None:
-            return (None,) * 6
+            return (None,) * 7
         x, weight, bias, state, lengths = ctx.saved_tensors
         if dy is None:
             dy = torch.zeros_like(x)
         dx, dweight, dbias, dstate = sequence.causal_conv1d_backward(
             x, weight, bias, state, ctx.activation, lengths, dy, dnew, state is not None and ctx.needs_input_grad[3])
-        return dx, dweight, dbias if bias is not None else None, dstate, None, None
+        return dx, dweight, dbias if bias is not None else None, dstate, None, None, None
 
 
 class SelectiveScan(torch.autograd.Function):
-    """(y, last state) of the selective scan.  The forward call stores the state before every 16th token, and the
-    backward pass runs the states of 16 tokens again from each (csrc/selective_scan.cuh)."""
+    """(y, last state) of the selective scan.  The forward call stores the state before every 8th token, and the
+    backward pass runs the states of 8 tokens again from each (csrc/selective_scan.cuh)."""
 
     @staticmethod
-    def forward(ctx, x, delta, a, b, c, d, z, delta_bias, state, softplus: bool, lengths):
+    def forward(ctx, x, delta, a, b, c, d, z, delta_bias, state, softplus: bool, lengths, return_state: bool):
         y, new, checkpoints = sequence._scan_forward(
-            x, delta, a, b, c, d, z, delta_bias, softplus, state, lengths, True, True)
+            x, delta, a, b, c, d, z, delta_bias, softplus, state, lengths, return_state, True)
         ctx.save_for_backward(x, delta, a, b, c, d, z, delta_bias, state, lengths, checkpoints)
         ctx.softplus = softplus
         ctx.set_materialize_grads(False)
-        return y, new
+        return (y, new) if return_state else y
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dy, dnew):
+    def backward(ctx, dy, dnew=None):
         if dy is None and dnew is None:
-            return (None,) * 11
+            return (None,) * 12
         x, delta, a, b, c, d, z, delta_bias, state, lengths, checkpoints = ctx.saved_tensors
         if dy is None:
             dy = torch.zeros_like(x)
         g = sequence.selective_scan_backward(
             x, delta, a, b, c, d, z, delta_bias, ctx.softplus, state, lengths, checkpoints, dy, dnew)
         return (g["x"], g["delta"], g["a"], g["b"], g["c"], g["d"] if d is not None else None, g["z"],
-                g["delta_bias"] if delta_bias is not None else None, g["state"], None, None)
+                g["delta_bias"] if delta_bias is not None else None, g["state"], None, None, None)
 
 
 class RmsNorm(torch.autograd.Function):
@@ -369,11 +368,11 @@ class RmsNorm(torch.autograd.Function):
             ctx.save_for_backward(residual, x, weight)
         ctx.eps, ctx.dtype = eps, x.dtype
         ctx.set_materialize_grads(False)
-        return y, None if residual is None else total
+        return y if residual is None else (y, total)
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dy, dtotal):
+    def backward(ctx, dy, dtotal=None):
         total, addend, weight = ctx.saved_tensors
         if dy is None:
             if dtotal is None:

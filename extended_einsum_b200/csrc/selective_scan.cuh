@@ -19,6 +19,10 @@
 // Few channels: the length is split into segments.  A first pass runs each segment from a zero state
 // and keeps its last state and sum of delta (the product of its e is exp(A sum delta)), a second
 // joins them into every segment's first state, and the scan then runs all segments at once.
+// Measured on a B200, 16 states, bf16: 4 x 4096 tokens of 4096 channels 529 us (the special function unit's
+// floor is 274 us; 3.5 warps to a scheduler issue in about half of its slots); 2 x 2048 tokens of 2048 channels
+// forward 140 us in four segments, of them 73 us the scan itself, backward 262 us and 51 us for the segments'
+// adjoints; one token of 64 x 4096 channels 12.9 us (36 MB, 2.8 TB/s).
 #pragma once
 
 #include "seq_common.cuh"

@@ -136,8 +136,12 @@ def causal_conv1d(
     if _needs_grad(x, weight, bias, state):
         from .autograd import CausalConv1d
 
-        y, new = CausalConv1d.apply(x, weight, bias, state, activation, lengths)
-        return (y, new) if return_state else y
+        return CausalConv1d.apply(x, weight, bias, state, activation, lengths, return_state)
+    y, new = _conv_forward(x, weight, bias, activation, state, lengths, return_state)
+    return (y, new) if return_state else y
+
+
+def _conv_forward(x, weight, bias, activation, state, lengths, return_state):
     x, weight, bias, state, lengths, code = _conv_operands("causal_conv1d", x, weight, bias, state, lengths, activation)
     batch, length, channels = x.shape
     width = weight.shape[1]
@@ -148,7 +152,7 @@ def causal_conv1d(
         _pointer(state), y.data_ptr(), _pointer(new), _pointer(lengths), int(lengths is not None and lengths.dtype == torch.int64),
         batch, length, channels, width, _ACTIVATIONS[activation], code,
     )
-    return (y, new) if return_state else y
+    return y, new
 
 
 def _conv_operands(what, x, weight, bias, state, lengths, activation):
@@ -266,8 +270,7 @@ def selective_scan(
     if _needs_grad(x, delta, a, b, c, d, z, delta_bias, state):
         from .autograd import SelectiveScan
 
-        y, new = SelectiveScan.apply(x, delta, a, b, c, d, z, delta_bias, state, softplus, lengths)
-        return (y, new) if return_state else y
+        return SelectiveScan.apply(x, delta, a, b, c, d, z, delta_bias, state, softplus, lengths, return_state)
     y, new, _ = _scan_forward(x, delta, a, b, c, d, z, delta_bias, softplus, state, lengths, return_state, False)
     return (y, new) if return_state else y
 
@@ -456,8 +459,7 @@ def rms_norm(
             raise NotImplementedError(f"{what}: no backward pass through 8-bit outputs")
         from .autograd import RmsNorm
 
-        y, total = RmsNorm.apply(x, weight, residual, eps)
-        return y if residual is None else (y, total)
+        return RmsNorm.apply(x, weight, residual, eps)
     return _norm_forward(x, weight, residual, eps, quantize)
 
 
