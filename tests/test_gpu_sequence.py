@@ -612,3 +612,45 @@ def test_int4_quantize(symmetric):
     assert ((back - w.double()).abs() <= (0.5 if symmetric else 1.0) * step * (1 + 2.0**-20)).all()
     x = randn(gen, 2, 256)
     int4_close(ops.int4_linear(x.cuda(), packed, scales, zeros), x, packed.cpu(), scales.cpu(), None if zeros is None else zeros.cpu())
+
+
+def test_strides_past_32_bits():
+    """Two rows 2^31 elements apart: the second one's offset does not fit 32 bits."""
+    far = 2**31
+    base = torch.empty(far + 4096, device="cuda", dtype=torch.bfloat16)
+    gen = torch.Generator().manual_seed(13)
+
+    def spread(t):
+        view = base.as_strided(t.shape, (far, *t.stride()[1:]))
+        view.copy_(t.cuda())
+        return view
+
+    v = scan_inputs(14, 2, 9, 24, 16, 1, torch.bfloat16)
+    want, want_state = scan_reference(v, True)
+    w = {k: cuda(t) for k, t in v.items()}
+    for name in ("x", "delta", "z", "b", "c"):
+        y, state = scan_call({**w, name: spread(v[name])}, True, return_state=True)
+        close(y, want, 9)
+        close(state, want_state, 9)
+    x, weight = randn(gen, 2, 9, 24, dtype=torch.bfloat16), randn(gen, 24, 4)
+    close(ops.causal_conv1d(spread(x), weight.cuda()), oracle.causal_conv1d(x.double(), weight.double())[0], 4)
+    rows = randn(gen, 2, 256, dtype=torch.bfloat16)
+    close(ops.rms_norm(spread(rows)), oracle.rms_norm(rows.double())[0], 24)
+    _, packed, scales, z = int4_inputs(15, 256, 20, 64, True, torch.bfloat16)
+    int4_close(ops.int4_linear(spread(rows), packed.cuda(), scales.cuda(), z.cuda()), rows, packed, scales, z)
+
+
+@pytest.mark.parametrize("length,channels", [(700, 7), (2100, 20)])
+def test_scan_gradients_of_a_split_length(length, channels):
+    """Few channels: the length is run in segments, whose states and adjoints are joined."""
+    v = scan_inputs(16, 1, length, channels, 5)
+    names = list(v)
+    gen = torch.Generator().manual_seed(17)
+    dy, dstate = randn(gen, 1, length, channels), randn(gen, 1, channels, 5)
+    ends = torch.tensor([length - 150])
+    w = leaf({k: wide(t) for k, t in v.items()}, names)
+    want = grads_of(scan_reference(w, True, ends), [wide(dy), wide(dstate)], [w[k] for k in names])
+    g = leaf({k: cuda(t) for k, t in v.items()}, names)
+    got = grads_of(scan_call(g, True, ends.cuda(), return_state=True), [cuda(dy), cuda(dstate)], [g[k] for k in names])
+    for k, a, b in zip(names, got, want):
+        close(a, b, length + channels, factor=4.0)
