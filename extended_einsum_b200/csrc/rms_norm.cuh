@@ -12,7 +12,7 @@
 // Bound by memory: every row is read once, kept in registers between the statistics and the output,
 // and written once.
 // Measured on a B200: 16384 x 4096 bf16 with a residual into e4m3 81 us (5.8 TB/s; with loads ahead in registers
-// and two reductions 106 us); one row of 4096 3.5 us; forward and backward of 4099 x 2560 bf16 42 us.
+// and two reductions 106 us); 16384 x 4095 214 us (element by element 274 us); one row of 4096 3.5 us; forward and backward of 4099 x 2560 bf16 42 us.
 #pragma once
 
 #include <algorithm>
@@ -210,12 +210,47 @@ __device__ __forceinline__ uint32_t codes8(float a, float b, int quantize) {
   return (uint32_t)(i & 255) | (uint32_t)(j & 255) << 8;
 }
 
+// How rows lie: every one on a vector's boundary; all tensors' rows off it by the same number of elements, the
+// row's number times the columns (an odd number of columns), where groups begin on the boundaries and only a
+// row's two ends go by elements; or anyhow.
+enum Rows { kAnyhow, kAligned, kShifted };
+
+template <typename T>
+__device__ __forceinline__ void load_shifted(const T* row, int at, int columns, float (&v)[8]) {
+  if (at >= 0 && at + 8 <= columns) {
+    load8f<T>(row + at, 8, true, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = at + i >= 0 && at + i < columns ? to_f32(row[at + i]) : 0.0f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_shifted(T* row, int at, int columns, const float (&v)[8]) {
+  if (at >= 0 && at + 8 <= columns) {
+    store8<T>(row + at, 8, true, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (at + i >= 0 && at + i < columns) row[at + i] = from_f32<T>(v[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void load_weight_at(const void* weight, int weight_f32, int columns, int at, float (&w)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w[i] = 1.0f;
+    if (weight && at + i >= 0 && at + i < columns)
+      w[i] = weight_f32 ? static_cast<const float*>(weight)[at + i] : to_f32(static_cast<const T*>(weight)[at + i]);
+  }
+}
+
 // `wpr` warps on each row, blockDim.x / 32 / wpr rows at a time, the blocks persistent over the rows; a
 // thread holds kGroups groups of eight elements.  Rows to come are loaded ahead (aligned ones through the
 // ring), since the reductions' barriers would otherwise leave the memory idle.
-template <typename T, typename R, int kGroups, bool kVec>
+template <typename T, typename R, int kGroups, Rows kRows>
 __global__ void __launch_bounds__(kMaxThreads<kGroups>, 1) rms_norm_kernel(const __grid_constant__ Params p, int wpr) {
-  constexpr bool kKeep = kGroups <= 2;  // weights stay in registers
+  constexpr bool kVec = kRows == kAligned, kMoved = kRows == kShifted;
+  constexpr bool kKeep = kGroups <= 2 && !kMoved;  // weights stay in registers
   constexpr bool kRinged = kVec && kRing<kGroups>;
   constexpr int kStages = std::max(1, kForwardStages<T, R, kGroups>);
   constexpr int kPlaces = kGroups * (sizeof(T) + sizeof(R)) / 2;
@@ -258,6 +293,8 @@ __global__ void __launch_bounds__(kMaxThreads<kGroups>, 1) rms_norm_kernel(const
   for (int64_t base = (int64_t)blockIdx.x * slots; base < p.rows; base += stride, row += stride) {
     const int columns = row < p.rows ? p.columns : 0;
     const int64_t out = (columns ? row : 0) * p.columns;
+    const int shift = kMoved ? (int)(out % 8) : 0;
+    auto first = [&](int g) { return (g * lanes + lane) * 8 - shift; };  // kShifted: the group's first column
     float v[kGroups][8];
     float total = 0.0f;
     if (kRinged) {
@@ -271,17 +308,24 @@ __global__ void __launch_bounds__(kMaxThreads<kGroups>, 1) rms_norm_kernel(const
       const bool in = element<kVec>(g, 0, lane, lanes) < columns;
       if (kRinged)
         ring_get<T>(at, g * (sizeof(T) / 2), in, v[g]);
+      else if (kMoved)
+        load_shifted<T>(static_cast<const T*>(p.x) + (columns ? row : 0) * p.x_row, first(g), columns, v[g]);
       else
         load_group<T, kVec>(static_cast<const T*>(p.x) + (columns ? row : 0) * p.x_row, g, lane, lanes, columns, v[g]);
       if (p.residual) {
         float a[8];
         if (kRinged)
           ring_get<R>(at, kGroups * (sizeof(T) / 2) + g * (sizeof(R) / 2), in, a);
+        else if (kMoved)
+          load_shifted<R>(static_cast<const R*>(p.residual) + (columns ? row : 0) * p.r_row, first(g), columns, a);
         else
           load_group<R, kVec>(static_cast<const R*>(p.residual) + (columns ? row : 0) * p.r_row, g, lane, lanes, columns, a);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[g][i] += a[i];
-        store_group<R, kVec>(static_cast<R*>(p.sum) + out, g, lane, lanes, columns, v[g]);
+        if (kMoved)
+          store_shifted<R>(static_cast<R*>(p.sum) + out, first(g), columns, v[g]);
+        else
+          store_group<R, kVec>(static_cast<R*>(p.sum) + out, g, lane, lanes, columns, v[g]);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) total = fmaf(v[g][i], v[g][i], total);
@@ -290,7 +334,10 @@ __global__ void __launch_bounds__(kMaxThreads<kGroups>, 1) rms_norm_kernel(const
     uint32_t most = 0;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      if (!kKeep) load_weight<T, kVec>(p.weight, p.weight_f32, p.columns, g, lane, lanes, w[0]);
+      if (kMoved)
+        load_weight_at<T>(p.weight, p.weight_f32, p.columns, first(g), w[0]);
+      else if (!kKeep)
+        load_weight<T, kVec>(p.weight, p.weight_f32, p.columns, g, lane, lanes, w[0]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         v[g][i] *= w[kKeep ? g : 0][i];
@@ -308,7 +355,12 @@ __global__ void __launch_bounds__(kMaxThreads<kGroups>, 1) rms_norm_kernel(const
       for (int i = 0; i < 8; ++i) v[g][i] *= rstd;
     if (p.quantize == 0) {
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) store_group<T, kVec>(static_cast<T*>(p.y) + out, g, lane, lanes, columns, v[g]);
+      for (int g = 0; g < kGroups; ++g) {
+        if (kMoved)
+          store_shifted<T>(static_cast<T*>(p.y) + out, first(g), columns, v[g]);
+        else
+          store_group<T, kVec>(static_cast<T*>(p.y) + out, g, lane, lanes, columns, v[g]);
+      }
       continue;
     }
     float scale = __uint_as_float(most) * rstd / (p.quantize == XE_E4M3 ? 448.0f : 127.0f);
@@ -321,7 +373,16 @@ __global__ void __launch_bounds__(kMaxThreads<kGroups>, 1) rms_norm_kernel(const
       uint32_t c[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[i] = codes8(v[g][2 * i] * inverse, v[g][2 * i + 1] * inverse, p.quantize);
-      if constexpr (kVec) {
+      if constexpr (kMoved) {
+        const int at = first(g);
+        if (at >= 0 && at + 8 <= columns) {
+          *reinterpret_cast<uint2*>(q + at) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (at + i >= 0 && at + i < columns) q[at + i] = (uint8_t)(c[i / 2] >> (8 * (i % 2)));
+        }
+      } else if constexpr (kVec) {
         const int at = element<true>(g, 0, lane, lanes);
         if (at < columns) *reinterpret_cast<uint2*>(q + at) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
       } else {

@@ -566,6 +566,11 @@ xe_status xe_rms_norm(const void* x, int64_t x_row, const void* residual, int64_
   const bool vec = vectors(x, dtype, {x_row, columns}) && vectors(residual, residual_dtype, {residual_row}) &&
                    vectors(sum, residual_dtype, {columns}) && vectors(weight, weight_dtype, {}) && vectors(y, dtype, {}) &&
                    columns % 8 == 0;
+  // every tensor's row r starts r * columns elements past a boundary, modulo a vector
+  auto base = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 32 == 0; };
+  const bool shifted = !vec && x_row % 8 == columns % 8 && (!residual || residual_row % 8 == columns % 8) && base(x) &&
+                       base(residual) && base(sum) && base(y) && columns >= 64 && columns <= 65528;
+  if (shifted && !norm_shape(columns + 7, false, rows, shape)) return fail(XE_ERR_NOT_SUPPORTED, "%s: too many columns", what);
   by_types(dtype, residual_dtype, [&](auto t, auto r) {
     by_groups(shape.groups, [&](auto g) {
       auto go = [&](auto v) {
@@ -574,14 +579,17 @@ xe_status xe_rms_norm(const void* x, int64_t x_row, const void* residual, int64_
         using T = decltype(t);
         using R = decltype(r);
         constexpr int kGroups = decltype(g)::value;
-        const int bytes = decltype(v)::value ? xe::norm::kForwardStages<T, R, kGroups> * shape.threads * xe::norm::kForwardBytes<T, R, kGroups> : 0;
+        const int bytes = decltype(v)::value == xe::norm::kAligned ? xe::norm::kForwardStages<T, R, kGroups> * shape.threads * xe::norm::kForwardBytes<T, R, kGroups> : 0;
         const int64_t blocks = persistent_blocks<Tag>(kernel, shape.threads, bytes, ceil_div(rows, shape.rows_per_block));
         kernel<<<(unsigned)blocks, shape.threads, bytes, as_stream(stream)>>>(p, shape.warps_per_row);
       };
+      using xe::norm::Rows;
       if (vec)
-        go(std::true_type{});
+        go(std::integral_constant<Rows, xe::norm::kAligned>{});
+      else if (shifted)
+        go(std::integral_constant<Rows, xe::norm::kShifted>{});
       else
-        go(std::false_type{});
+        go(std::integral_constant<Rows, xe::norm::kAnyhow>{});
     });
   });
   return launched(what);

@@ -433,6 +433,25 @@ def test_norm(dtype, rows, columns, residual):
         close(got[1], want_s, 0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("columns", [65, 127, 1001, 2052, 9003])
+def test_norm_of_rows_that_drift_past_the_boundaries(dtype, columns):
+    """Odd numbers of columns: every row starts elsewhere within a vector, its ends beside its neighbours'."""
+    gen = torch.Generator().manual_seed(columns)
+    x, r, weight = randn(gen, 19, columns, dtype=dtype), randn(gen, 19, columns, dtype=dtype), randn(gen, columns)
+    want_y, want_s = oracle.rms_norm(x.double(), weight.double(), r.double())
+    y, s = ops.rms_norm(x.cuda(), weight.cuda(), residual=r.cuda())
+    close(y, want_y, 24)
+    close(s, want_s, 0)
+    wide_y, wide_s = ops.rms_norm(x.cuda(), weight.cuda().to(dtype), residual=r.cuda().float())
+    close(wide_y, oracle.rms_norm(x.double(), weight.to(dtype).double(), r.double())[0], 24)
+    close(wide_s, want_s, 0)
+    q, scale, _ = ops.rms_norm(x.cuda(), weight.cuda(), residual=r.cuda(), quantize="int8")
+    want_scale = want_y.abs().amax(1) / 127.0
+    assert ((q.double().cpu() - want_y / want_scale[:, None]).abs() <= 0.5 + 64 * 2.0**-21 * 127.0).all()
+    assert ((scale.double().cpu() - want_scale).abs() <= 32 * 2.0**-21 * want_scale).all()
+
+
 @pytest.mark.parametrize("quantize,most,step", [("e4m3", 448.0, 2.0**-4), ("int8", 127.0, None)])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,columns", [(1, 16), (4, 100), (70, 96), (2, 4096), (3, 9000)])
