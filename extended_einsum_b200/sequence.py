@@ -597,7 +597,7 @@ def int4_linear(
         zeros = _operand(what, "zeros", zeros, x, (outputs, groups), torch.uint8).contiguous()
     rows = _as_rows(x)
     if x_scale is not None:
-        x_scale = _operand(what, "x_scale", x_scale, x, x.shape[:-1], torch.float32).contiguous() if x.dim() > 1 else x_scale
+        x_scale = _operand(what, "x_scale", x_scale, x, x.shape[:-1], torch.float32).contiguous()
     y = torch.empty((*x.shape[:-1], outputs), device=device, dtype=dtype)
     size = _entry("xe_int4_linear_workspace_size")(rows.shape[0], inputs, outputs, code)
     workspace = _workspace(size, device)

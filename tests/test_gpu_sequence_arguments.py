@@ -1,0 +1,25 @@
+"""Operands of the sequence operators that are refused on the GPU, and what its calls leave behind."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from extended_einsum_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def test_int4_scale_of_a_single_row():
+    """One row in 8 bits with the scale of no dimensions that the norm gives it; a scale elsewhere is refused."""
+    gen = torch.Generator().manual_seed(1)
+    packed = torch.randint(0, 256, (7, 32), generator=gen, dtype=torch.uint8).cuda()
+    scales = torch.rand(7, 2, generator=gen).cuda()
+    q, scale = ops.rms_norm(torch.randn(64, generator=gen).cuda(), quantize="int8")
+    assert scale.shape == ()
+    y = ops.int4_linear(q, packed, scales, x_scale=scale)
+    assert torch.equal(y, ops.int4_linear(q[None], packed, scales, x_scale=scale[None])[0])
+    with pytest.raises(ValueError, match="device"):
+        ops.int4_linear(q, packed, scales, x_scale=scale.cpu())
+    with pytest.raises(NotImplementedError, match="x_scale"):
+        ops.int4_linear(q, packed, scales, x_scale=scale.double())
