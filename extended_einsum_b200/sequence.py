@@ -14,6 +14,7 @@ current stream, like the rest of ``ops``.
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -208,6 +209,7 @@ def causal_conv1d_step(
         x.device, "xe_causal_conv1d_step", x.data_ptr(), x.stride(0), weight.data_ptr(), _pointer(bias), state.data_ptr(),
         y.data_ptr(), batch, channels, width, _ACTIVATIONS[activation], code,
     )
+    increment_version(state)
     return y
 
 
@@ -397,6 +399,7 @@ def selective_scan_step(
         batch, 1, channels, states, groups, 0, int(softplus), code,
     )
     _call(x.device, "xe_selective_scan_step", args)
+    increment_version(state)
     return y
 
 

@@ -32,3 +32,29 @@ def test_int4_scale_of_a_single_row_is_checked(calls):
         with pytest.raises(TypeError, match="x_scale"):
             ops.int4_linear(x, packed, scales, x_scale=0.5)
     assert not calls
+
+
+def test_steps_tell_autograd_of_the_state(calls):
+    """The state is written through its address: its version moves on, so that a graph that saved it fails and does not use
+    what it has become."""
+    taps, held = torch.zeros(2, 3, 8), torch.zeros(2, 8, 4)
+    x, bc = torch.zeros(2, 8), torch.zeros(2, 4)
+    for state, step in (
+        (taps, lambda: ops.causal_conv1d_step(taps, x, torch.zeros(8, 4))),
+        (held, lambda: ops.selective_scan_step(held, x, x, torch.zeros(8, 4), bc, bc)),
+    ):
+        before = state._version
+        step()
+        assert state._version > before and len(calls) == 1
+        calls.clear()
+        scale = torch.ones((), requires_grad=True)
+        out = (state * scale).sum()  # saves the state
+        with torch.no_grad():
+            step()
+        calls.clear()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.backward()
+    with torch.inference_mode():  # such tensors have no version
+        ops.causal_conv1d_step(torch.zeros(2, 3, 8), x, torch.zeros(8, 4))
+        held = torch.zeros(2, 8, 4)
+    ops.selective_scan_step(held, x, x, torch.zeros(8, 4), bc, bc)
