@@ -14,6 +14,7 @@ current stream, like the rest of ``ops``.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _lib
@@ -95,7 +96,12 @@ def _like(x: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
     return torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
 
 
-def _needs_grad(*tensors: torch.Tensor | None) -> bool:
+def _needs_grad(what: str, *tensors: torch.Tensor | None) -> bool:
+    """Whether autograd records this call.  A forward-mode tangent is refused: it would be dropped."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what}: no forward-mode derivative")
     if torch.is_grad_enabled():
         for t in tensors:
             if isinstance(t, torch.Tensor) and t.requires_grad:
@@ -104,7 +110,7 @@ def _needs_grad(*tensors: torch.Tensor | None) -> bool:
 
 
 def _no_backward(what: str, *tensors: torch.Tensor | None) -> None:
-    if _needs_grad(*tensors):
+    if _needs_grad(what, *tensors):
         raise NotImplementedError(f"{what}: no backward pass on this path")
 
 
@@ -134,7 +140,7 @@ def causal_conv1d(
     ``causal_conv1d_step``.  ``lengths`` (batch,) int32 or int64: only the first so many tokens of
     each sequence count, y is zero after them.  Differentiable (autograd.CausalConv1d).
     """
-    if _needs_grad(x, weight, bias, state):
+    if _needs_grad("causal_conv1d", x, weight, bias, state):
         from .autograd import CausalConv1d
 
         return CausalConv1d.apply(x, weight, bias, state, activation, lengths, return_state)
@@ -269,7 +275,7 @@ def selective_scan(
     the last.  ``lengths`` (batch,): tokens past a sequence's length leave its state alone and give
     y = 0.  Differentiable in every floating operand (autograd.SelectiveScan).
     """
-    if _needs_grad(x, delta, a, b, c, d, z, delta_bias, state):
+    if _needs_grad("selective_scan", x, delta, a, b, c, d, z, delta_bias, state):
         from .autograd import SelectiveScan
 
         return SelectiveScan.apply(x, delta, a, b, c, d, z, delta_bias, state, softplus, lengths, return_state)
@@ -457,7 +463,7 @@ def rms_norm(
     (autograd.RmsNorm).
     """
     what = "rms_norm"
-    if _needs_grad(x, weight, residual):
+    if _needs_grad(what, x, weight, residual):
         if quantize is not None:
             raise NotImplementedError(f"{what}: no backward pass through 8-bit outputs")
         from .autograd import RmsNorm

@@ -5,6 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
+from torch.autograd import forward_ad
+
 from extended_einsum_b200 import ops, sequence
 
 
@@ -58,3 +60,31 @@ def test_steps_tell_autograd_of_the_state(calls):
         ops.causal_conv1d_step(torch.zeros(2, 3, 8), x, torch.zeros(8, 4))
         held = torch.zeros(2, 8, 4)
     ops.selective_scan_step(held, x, x, torch.zeros(8, 4), bc, bc)
+
+
+def test_forward_mode_is_refused():
+    """No operator here has a forward-mode derivative: a tangent is refused, not dropped."""
+    three, row = torch.zeros(2, 3, 8), torch.zeros(2, 8)
+    bc = torch.zeros(2, 3, 4)
+    uses = [
+        (three, lambda t: ops.causal_conv1d(t, torch.zeros(8, 4))),
+        (torch.zeros(8), lambda t: ops.causal_conv1d(three, torch.zeros(8, 4), t)),
+        (row, lambda t: ops.causal_conv1d_step(torch.zeros(2, 3, 8), t, torch.zeros(8, 4))),
+        (bc, lambda t: ops.selective_scan(three, three, torch.zeros(8, 4), t, bc)),
+        (torch.zeros(2, 8, 4), lambda t: ops.selective_scan(three, three, torch.zeros(8, 4), bc, bc, state=t)),
+        (row, lambda t: ops.selective_scan_step(torch.zeros(2, 8, 4), row, t, torch.zeros(8, 4), bc[:, 0], bc[:, 0])),
+        (three, lambda t: ops.rms_norm(t)),
+        (three, lambda t: ops.rms_norm(three, residual=t, quantize="int8")),
+        (torch.zeros(2, 64), lambda t: ops.int4_linear(t, torch.zeros(3, 32, dtype=torch.uint8), torch.zeros(3, 1))),
+        (torch.zeros(3, 1), lambda t: ops.int4_linear(torch.zeros(2, 64), torch.zeros(3, 32, dtype=torch.uint8), t)),
+    ]
+    for value, use in uses:
+        for grad in (False, True):
+            for requires in (False, True):
+                primal = value.clone().requires_grad_(requires)
+                with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                    dual = forward_ad.make_dual(primal, torch.ones_like(value))
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        use(dual)
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="CUDA"):
+        ops.rms_norm(three)  # no tangent: on to the next check
