@@ -571,7 +571,8 @@ def int4_linear(
     the same shape (None: 8); the group is a multiple of 32.  ``x`` (..., inputs) is float32, bfloat16 or
     float16, or 8-bit (float8_e4m3fn, int8) with ``x_scale`` (...) as ``rms_norm`` gives them.  ``dtype`` of
     the result: x's type, or bfloat16 for 8-bit x, unless given.  Integers q - zero and the activations
-    multiply exactly; sums and scales are float32.  Made for the few rows of token-by-token generation.
+    multiply exactly; sums and scales are float32.  Made for the few rows of token-by-token generation;
+    many rows go in slices that share a workspace of at most 512 MB.
     """
     what = "int4_linear"
     _no_backward(what, x, scales, x_scale)

@@ -572,7 +572,8 @@ xe_status xe_rms_norm_backward(const void* sum, int64_t sum_row, const void* add
  * 16-byte boundaries; scales (outputs, inputs / group) contiguous, of type XE_F32, XE_BF16 or
  * XE_F16; zeros one byte each, 0 to 15, or NULL for 8.  x: XE_F32, XE_BF16, XE_F16, or XE_E4M3 /
  * XE_I8 with x_scale per row (or NULL: 1).  `group` is a multiple of 32 that divides `inputs`.
- * Made for few rows (the weights are read again for every 64 of them, 21 with XE_F32). */
+ * Made for few rows (the weights are read again for every 64 of them, 21 with XE_F32); many
+ * rows go in slices, whose workspace stays within 512 MB or what 64 (21) rows need. */
 size_t xe_int4_linear_workspace_size(int64_t rows, int64_t inputs, int64_t outputs, int32_t x_dtype);
 xe_status xe_int4_linear(const void* x, int64_t x_row, const float* x_scale, const void* packed, int64_t packed_row,
                          const void* scales, const void* zeros, void* y, int64_t rows, int64_t inputs, int64_t outputs,

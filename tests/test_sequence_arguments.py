@@ -7,7 +7,7 @@ import torch
 
 from torch.autograd import forward_ad
 
-from extended_einsum_b200 import ops, sequence
+from extended_einsum_b200 import _lib, ops, sequence
 
 
 @pytest.fixture
@@ -88,3 +88,23 @@ def test_forward_mode_is_refused():
                         use(dual)
     with forward_ad.dual_level(), pytest.raises(ValueError, match="CUDA"):
         ops.rms_norm(three)  # no tangent: on to the next check
+
+
+@pytest.mark.parametrize("rows", [16384, 70000, 1 << 20])
+@pytest.mark.parametrize("dtype", [_lib.XE_F32, _lib.XE_BF16, _lib.XE_E4M3])
+@pytest.mark.parametrize("inputs,outputs", [(4096, 16384), (8192, 16384), (18432, 20)])
+def test_int4_workspace_of_many_rows_is_bounded(rows, dtype, inputs, outputs):
+    """Prompts go in slices: their partial sums do not grow with the rows without end (6.4 GB for 16384 rows of the second
+    shape at once)."""
+    lib = _lib.load()
+    one = lib.xe_int4_linear_workspace_size(21 if dtype == _lib.XE_F32 else 64, inputs, outputs, dtype)
+    assert 0 < one <= lib.xe_int4_linear_workspace_size(rows, inputs, outputs, dtype) <= 512 << 20
+
+
+def test_int4_entry_takes_many_rows():
+    """More rows than a grid holds are no reason to refuse."""
+    lib = _lib.load()
+    status = lib.xe_int4_linear(256, 64, None, 256, 32, None, None, 256, 70000, 64, 4, 32, 1, 1, 1, None, 0, None)
+    assert status == _lib.XE_ERR_INVALID_ARGUMENT and "null" in _lib.last_error()  # no scales: the size has passed
+    status = lib.xe_int4_linear(256, 8192, None, 256, 4096, 256, None, 256, 70000, 8192, 20, 32, 1, 1, 1, None, 0, None)
+    assert status == _lib.XE_ERR_INVALID_ARGUMENT and "workspace" in _lib.last_error()
