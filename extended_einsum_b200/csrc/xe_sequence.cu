@@ -38,6 +38,15 @@ bool aligned(int64_t bytes, const void* p, int32_t dtype, std::initializer_list<
 }
 bool vectors(const void* p, int32_t dtype, std::initializer_list<int64_t> strides) { return aligned(16, p, dtype, strides); }
 
+// A workspace of at least `need` bytes, on a boundary that suits every vector stored to it.
+xe_status check_workspace(const char* what, const void* workspace, size_t bytes, size_t need) {
+  if (need == 0) return XE_OK;
+  if (!workspace || bytes < need) return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace must be 256-byte aligned", what);
+  return XE_OK;
+}
+
 template <typename F>
 void by_type(int32_t dtype, F f) {
   if (dtype == XE_F32)
@@ -190,8 +199,9 @@ xe_status xe_causal_conv1d_backward(const void* x, int64_t x_sb, int64_t x_st, c
   if (channels == 0) return XE_OK;
   if ((batch * length != 0 && !dy) || !dweight) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (batch == 0) return fail(XE_ERR_INVALID_ARGUMENT, "%s: an empty batch has no gradients", what);
-  if (!workspace || workspace_bytes < xe_causal_conv1d_backward_workspace_size(batch, length, channels, width))
-    return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+  if (xe_status s = check_workspace(what, workspace, workspace_bytes,
+                                    xe_causal_conv1d_backward_workspace_size(batch, length, channels, width)))
+    return s;
   xe::conv::Params p{};
   p.x = x, p.weight = weight, p.bias = bias, p.state = state;
   p.dy = dy, p.dy_sb = dy_sb, p.dy_st = dy_st, p.dstate_out = dstate_out, p.dx = dx, p.dstate = dstate;
@@ -264,6 +274,8 @@ xe_status check_scan(const char* what, const xe_selective_scan_args* q, bool ste
   if (q->channels % q->groups)
     return fail(XE_ERR_INVALID_ARGUMENT, "%s: %lld channels do not divide into %lld groups", what, (long long)q->channels,
                 (long long)q->groups);
+  if (reinterpret_cast<uintptr_t>(q->checkpoints) % 16)
+    return fail(XE_ERR_INVALID_ARGUMENT, "%s: checkpoints must be 16-byte aligned", what);
   if (q->states > 64 && !step) return fail(XE_ERR_NOT_SUPPORTED, "%s: %lld states above 64", what, (long long)q->states);
   if ((!step && q->batch > 65535) || q->batch > INT_MAX / 2 || q->length > INT_MAX / 2 || q->channels > INT_MAX / 2 ||
       q->states > 65536)
@@ -365,8 +377,8 @@ xe_status xe_selective_scan(const xe_selective_scan_args* q, void* workspace, si
   if (q->batch == 0 || q->channels == 0) return XE_OK;
   if (q->length > 0 && !q->y) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   const ScanPlan plan = scan_plan(q->batch, q->length, q->channels, q->groups);
-  if (workspace_bytes < scan_segment_bytes(plan, q->batch, q->channels, q->states) || (plan.segments > 1 && !workspace))
-    return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+  if (xe_status s = check_workspace(what, workspace, workspace_bytes, scan_segment_bytes(plan, q->batch, q->channels, q->states)))
+    return s;
   ScanParams p = scan_params(q);
   scan_segments(p, plan, workspace);
   if (p.segments > 1) {
@@ -413,8 +425,10 @@ xe_status xe_selective_scan_backward(const xe_selective_scan_args* q, const xe_s
                                                         (q->z && !g->dz) || !q->checkpoints)))
     return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (q->batch == 0) return fail(XE_ERR_INVALID_ARGUMENT, "%s: an empty batch has no gradients", what);
-  if (!workspace || workspace_bytes < xe_selective_scan_backward_workspace_size(q->batch, q->length, q->channels, q->states, q->groups))
-    return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+  if (xe_status s = check_workspace(
+          what, workspace, workspace_bytes,
+          xe_selective_scan_backward_workspace_size(q->batch, q->length, q->channels, q->states, q->groups)))
+    return s;
   const ScanPlan plan = scan_plan(q->batch, q->length, q->channels, q->groups);
   ScanParams p = scan_params(q);
   scan_segments(p, plan, workspace);
@@ -609,8 +623,9 @@ xe_status xe_rms_norm_backward(const void* sum, int64_t sum_row, const void* add
   if (xe_status s = check_norm(what, rows, columns, dtype, residual_dtype, weight_dtype)) return s;
   if (!sum || !dy || !dx) return fail(XE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (rows == 0) return fail(XE_ERR_INVALID_ARGUMENT, "%s: no rows, no gradients", what);
-  if (dweight && (!workspace || workspace_bytes < xe_rms_norm_backward_workspace_size(rows, columns)))
-    return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+  if (xe_status s = check_workspace(what, workspace, workspace_bytes,
+                                    dweight ? xe_rms_norm_backward_workspace_size(rows, columns) : 0))
+    return s;
   NormShape shape;
   if (!norm_shape(columns, true, rows, shape)) return fail(XE_ERR_NOT_SUPPORTED, "%s: too many columns", what);
   int64_t blocks = norm_backward_blocks(rows, shape);
@@ -810,8 +825,8 @@ xe_status xe_int4_linear(const void* x, int64_t x_row, const float* x_scale, con
   p.pieces = x_dtype == XE_F32 ? 3 : 1;
   p.group_magic = group == 32 ? 0u : (uint32_t)((1ull << 32) / (uint64_t)(group / 32)) + 1u;
   p.x_vec = aligned(size_of(x_dtype) == 1 ? 8 : 16, x, x_dtype, {x_row});
-  const size_t need = xe_int4_linear_workspace_size(rows, inputs, outputs, x_dtype);
-  if (need && (!workspace || workspace_bytes < need)) return fail(XE_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+  if (xe_status s = check_workspace(what, workspace, workspace_bytes, xe_int4_linear_workspace_size(rows, inputs, outputs, x_dtype)))
+    return s;
   cudaStream_t st = as_stream(stream);
   const int64_t slice = int4_slice(rows, inputs, outputs, p.pieces);
   for (int64_t m = 0; m < rows; m += slice) {

@@ -465,7 +465,8 @@ xe_status xe_elementwise(int32_t op, const float* a, const int64_t* a_strides, c
  * contiguous and the other strides given in elements; outputs are contiguous.
  * Parameters (filters, A, D, biases) and states of the scan are float32, sums,
  * statistics and states are held in float32, and each output is rounded once.
- * Results do not depend on the order in which blocks run. */
+ * Results do not depend on the order in which blocks run.  Workspaces lie on 256-byte
+ * boundaries, checkpoints on 16-byte ones. */
 
 /* Element types. */
 typedef enum { XE_F32 = 0, XE_BF16 = 1, XE_F16 = 2, XE_E4M3 = 3, XE_I8 = 4 } xe_dtype;

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -108,3 +110,33 @@ def test_int4_entry_takes_many_rows():
     assert status == _lib.XE_ERR_INVALID_ARGUMENT and "null" in _lib.last_error()  # no scales: the size has passed
     status = lib.xe_int4_linear(256, 8192, None, 256, 4096, 256, None, 256, 70000, 8192, 20, 32, 1, 1, 1, None, 0, None)
     assert status == _lib.XE_ERR_INVALID_ARGUMENT and "workspace" in _lib.last_error()
+
+
+def test_entries_refuse_buffers_off_their_boundaries():
+    """Workspaces and the stored states are written in vectors: a place that does not allow it is refused, not faulted on."""
+    lib = _lib.load()
+    q = _lib.SelectiveScanArgs()
+    for name in ("x", "delta", "b", "c", "y", "a", "state_out", "checkpoints"):
+        setattr(q, name, 4096)
+    q.batch, q.length, q.channels, q.states, q.groups, q.dtype = 1, 4096, 8, 4, 1, _lib.XE_F32
+    grads = _lib.SelectiveScanGrads(*([4096] * 10), 8, 8)
+
+    def conv(workspace):
+        return lib.xe_causal_conv1d_backward(4096, 0, 8, 4096, None, None, 4096, 0, 8, None, 4096, None, 4096, None, 0, 1, 4, 8, 4,
+                                             1, 0, workspace, 1 << 30, None)
+
+    def norm(workspace):
+        return lib.xe_rms_norm_backward(4096, 8, None, 0, None, 4096, 8, None, 0, 4096, 4096, 2, 8, ctypes.c_float(1e-6), 0, 0, 0,
+                                        workspace, 1 << 30, None)
+
+    def int4(workspace):
+        return lib.xe_int4_linear(4096, 8192, None, 4096, 4096, 4096, None, 4096, 64, 8192, 64, 32, 1, 1, 1, workspace, 1 << 30, None)
+
+    for call in (conv, norm, int4, lambda w: lib.xe_selective_scan(q, w, 1 << 30, None),
+                 lambda w: lib.xe_selective_scan_backward(q, grads, w, 1 << 30, None)):
+        for workspace in (4096 + 4, 4096 + 128):
+            assert call(workspace) == _lib.XE_ERR_INVALID_ARGUMENT and "aligned" in _lib.last_error()
+    q.checkpoints = 4096 + 8
+    assert lib.xe_selective_scan(q, 4096, 1 << 30, None) == _lib.XE_ERR_INVALID_ARGUMENT and "aligned" in _lib.last_error()
+    assert lib.xe_selective_scan_backward(q, grads, 4096, 1 << 30, None) == _lib.XE_ERR_INVALID_ARGUMENT
+    assert "aligned" in _lib.last_error()
