@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(64) selective_scan_kernel(const __grid_constan
               if (kStateOnly) delta_sum[j] += du[j].x;
 #pragma unroll
               for (int s = 0; s < S / 2; ++s) {
-                const F2 e = exp2_fast2(mul2(d2, a[j][s])), b2 = s % 2 ? bv[s / 2].y : bv[s / 2].x;
+                const F2 e = decay2(d2, a[j][s]), b2 = s % 2 ? bv[s / 2].y : bv[s / 2].x;
                 if (kMode == kAdjoint)
                   h[j][s] = mul2(e, fma2(u2, b2, h[j][s]));
                 else
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(256) selective_scan_join_kernel(Params p) {
     const float own = last ? 0.0f : p.segment_state[k * total + i];
     const float sum = last ? 0.0f : p.segment_delta[k * (total / p.states) + bc];
     p.segment_state[k * total + i] = h;
-    h = fmaf(exp2_fast(sum * a), h, own);
+    h = fmaf(decay(sum, a), h, own);
   }
 }
 
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(kBackwardThreads) selective_scan_backward_kern
               const F2 d2 = both(j ? du.z : du.x), u2 = both(j ? du.w : du.y);
 #pragma unroll
               for (int s = 0; s < 2; ++s) {
-                e[t][j][s] = exp2_fast2(mul2(d2, a[nb][j][s]));
+                e[t][j][s] = decay2(d2, a[nb][j][s]);
                 h[t][j][s] = fma2(e[t][j][s], t == 0 ? h0[j][s] : h[t > 0 ? t - 1 : 0][j][s], mul2(u2, s ? bv.y : bv.x));
               }
               const float2 q = unpack2(fma2(cv.y, h[t][j][1], mul2(cv.x, h[t][j][0])));
@@ -794,10 +794,10 @@ __global__ void __launch_bounds__(128) selective_scan_step_kernel(const __grid_c
   const float u = delta * x, d2 = delta * kLog2e;
   float v = 0.0f;
   auto quad = [&](int n) {
-    h4.x = fmaf(exp2_fast(d2 * a4.x), h4.x, u * value4<T>(b4, 0));
-    h4.y = fmaf(exp2_fast(d2 * a4.y), h4.y, u * value4<T>(b4, 1));
-    h4.z = fmaf(exp2_fast(d2 * a4.z), h4.z, u * value4<T>(b4, 2));
-    h4.w = fmaf(exp2_fast(d2 * a4.w), h4.w, u * value4<T>(b4, 3));
+    h4.x = fmaf(decay(d2, a4.x), h4.x, u * value4<T>(b4, 0));
+    h4.y = fmaf(decay(d2, a4.y), h4.y, u * value4<T>(b4, 1));
+    h4.z = fmaf(decay(d2, a4.z), h4.z, u * value4<T>(b4, 2));
+    h4.w = fmaf(decay(d2, a4.w), h4.w, u * value4<T>(b4, 3));
     *reinterpret_cast<float4*>(state + n) = h4;
     v = fmaf(value4<T>(c4, 0), h4.x, v);
     v = fmaf(value4<T>(c4, 1), h4.y, v);
@@ -815,7 +815,7 @@ __global__ void __launch_bounds__(128) selective_scan_step_kernel(const __grid_c
     }
   } else if (in && !four) {
     for (int n = lane; n < p.states; n += kLanes) {
-      const float h = fmaf(exp2_fast(d2 * a[n]), state[n], u * to_f32(bv[n]));
+      const float h = fmaf(decay(d2, a[n]), state[n], u * to_f32(bv[n]));
       v = fmaf(to_f32(cv[n]), h, v);
       state[n] = h;
     }

@@ -1,0 +1,64 @@
+"""Errors of the sequence operators that would add up: means over many results, long sums, and single functions.
+
+Random errors of a float32 result are below 2^-24 of it; what the tests here look for is larger or has a mean.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from extended_einsum_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def decays(seed, batch, length, channels):
+    """Step sizes that make a state's exponents (base 2) lie between -0.01 and -0.001, and its logarithm after them."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    delta = (0.001 + 0.009 * torch.rand(batch, length, channels, generator=gen, device="cuda")) * 0.6931
+    return delta, -delta.double().sum(1)
+
+
+def mean_error(actual, log_expected):
+    return (actual.double() * torch.exp(-log_expected) - 1.0).mean().item()
+
+
+@pytest.mark.parametrize("batch,channels", [(3, 4096), (2, 96)])
+def test_scan_decays_have_no_bias(batch, channels):
+    """A state that only decays, forwards and (its gradient) backwards: exponentials rounded to nearest would have errors up
+    to 2^-25 of either sign; their mean over all channels stays below a quarter of that per token, 2^-27.  Whole
+    sequences (many channels) and ones run in segments (few)."""
+    length = 2048
+    delta, log_state = decays(1, batch, length, channels)
+    zero, none = torch.zeros_like(delta), torch.zeros(batch, length, 1, device="cuda")
+    a = -torch.ones(channels, 1, device="cuda")
+    state = torch.ones(batch, channels, 1, device="cuda", requires_grad=True)
+    _, last = ops.selective_scan(zero, delta, a, none, none, state=state, return_state=True)
+    assert abs(mean_error(last.detach()[..., 0], log_state)) <= length * 2.0**-27
+    (grad,) = torch.autograd.grad(last, state, torch.ones_like(last))
+    assert abs(mean_error(grad[..., 0], log_state)) <= length * 2.0**-27
+
+
+def test_step_decays_have_no_bias():
+    length, channels = 256, 4096
+    delta, log_state = decays(2, 8, length, channels)
+    zero, none = torch.zeros(8, channels, device="cuda"), torch.zeros(8, 1, device="cuda")
+    a = -torch.ones(channels, 1, device="cuda")
+    state = torch.ones(8, channels, 1, device="cuda")
+    for t in range(length):
+        ops.selective_scan_step(state, zero, delta[:, t], a, none, none)
+    assert abs(mean_error(state[..., 0], log_state)) <= length * 2.0**-27
+
+
+@pytest.mark.parametrize("rate", [-1.0, -1e30, 3.0])
+def test_a_step_size_of_zero_keeps_the_state_exactly(rate):
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    state = torch.randn(2, 40, 16, generator=gen, device="cuda")
+    zero, bc = torch.zeros(2, 50, 40, device="cuda"), torch.ones(2, 50, 16, device="cuda")
+    a = torch.full((40, 16), rate, device="cuda")
+    _, last = ops.selective_scan(zero, zero, a, bc, bc, state=state, return_state=True)
+    assert torch.equal(last, state)
+    held = state.clone()
+    ops.selective_scan_step(held, zero[:, 0], zero[:, 0], a, bc[:, 0], bc[:, 0])
+    assert torch.equal(held, state)
