@@ -411,8 +411,12 @@ struct BackwardParams {
   int weight_f32;
 };
 
-// Persistent blocks over the rows as above; each slot keeps its dw sums in registers and writes them once,
-// and sum_rows adds them in a fixed order.
+// Rows whose dw adds up in registers: one running sum over all of a slot's rows would lose its last bits (16M rows of 32
+// columns: 2.2e-6 of dw's norm, 2048 rows to a slot).
+constexpr int kFold = 64;
+
+// Persistent blocks over the rows as above; each slot keeps the dw sums of kFold rows in registers and adds them to a row of
+// its own in memory, and sum_rows adds these in a fixed order.
 template <typename T, typename R, int kGroups, bool kVec>
 __global__ void __launch_bounds__(kMaxBackwardThreads<kGroups>, 1)
     rms_norm_backward_kernel(const __grid_constant__ BackwardParams p, int wpr) {
@@ -462,8 +466,33 @@ __global__ void __launch_bounds__(kMaxBackwardThreads<kGroups>, 1)
     for (int g = 0; g < (kKeep ? kGroups : 1); ++g)
       load_weight<T, kVec>(p.weight, p.weight_f32, p.columns, g, lane, lanes, w[g]);
   }
-  int stage = 0;
+  // each slot's sums as a row of their own
+  float* partial = p.partial + ((int64_t)blockIdx.x * slots + slot) * p.columns;
+  bool folded = false;
+  auto fold = [&] {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      if (!folded) {
+        store_group<float, kVec>(partial, g, lane, lanes, p.columns, dw[g]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int at = element<kVec>(g, i, lane, lanes);
+          if (at < p.columns) partial[at] += dw[g][i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dw[g][i] = 0.0f;
+    }
+    folded = true;
+  };
+  int stage = 0, turns = 0;
   for (int64_t base = (int64_t)blockIdx.x * slots; base < p.rows; base += stride, row += stride) {
+    if (p.partial && turns == kFold) {
+      fold();
+      turns = 0;
+    }
+    ++turns;
     const int columns = row < p.rows ? p.columns : 0;
     const int64_t at = columns ? row : 0;
     float s[kGroups][8], du[kGroups][8];
@@ -534,11 +563,7 @@ __global__ void __launch_bounds__(kMaxBackwardThreads<kGroups>, 1)
       store_group<R, kVec>(static_cast<R*>(p.dx) + at * p.columns, g, lane, lanes, columns, o);
     }
   }
-  if (!p.partial) return;
-  // each slot's sums as a row of their own
-  float* out = p.partial + ((int64_t)blockIdx.x * slots + slot) * p.columns;
-#pragma unroll
-  for (int g = 0; g < kGroups; ++g) store_group<float, kVec>(out, g, lane, lanes, p.columns, dw[g]);
+  if (p.partial) fold();
 }
 
 }  // namespace norm

@@ -83,3 +83,34 @@ def test_scan_sums_over_a_long_length():
     ddelta, dd, dbias = torch.autograd.grad(y, [delta, d, bias], dy)
     assert relative(dd, sum((x[i].double() * dy[i].double()).sum(0) for i in range(batch))) <= 12 * 2.0**-25
     assert relative(dbias, sum(ddelta[i].double().sum(0) for i in range(batch))) <= 12 * 2.0**-25
+
+
+@pytest.mark.parametrize("rows,columns", [(1 << 24, 32), (3 << 20, 33)])
+def test_norm_sums_over_many_rows(rows, columns):
+    """dweight over millions of rows, in float32 sums of at most 64 rows, sums of these, and the blocks' sums: by the measure
+    above 2^-25 sqrt(32 + 32 + 64).  One running sum of a slot's 2000 to 3500 rows: 2^-25 sqrt(1000) and more."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x, dy = (torch.randn(rows, columns, generator=gen, device="cuda") for _ in range(2))
+    weight = torch.ones(columns, device="cuda", requires_grad=True)
+    (dweight,) = torch.autograd.grad(ops.rms_norm(x, weight), weight, dy)
+    want = 0.0
+    for part, grad in zip(x.chunk(16), dy.chunk(16)):
+        part = part.double()
+        want = want + (grad.double() * part * torch.rsqrt((part * part).mean(1, keepdim=True) + 1e-6)).sum(0)
+    assert relative(dweight, want) <= 12 * 2.0**-25
+
+
+def test_norm_sums_of_columns_over_rows_by_element_and_in_vectors():
+    """More than 64 rows to a slot in every width of the kernels, each column's sum by itself: all dy of one sign."""
+    for columns in (8, 33, 1000, 3000, 9001):
+        rows = 148 * 70 * max(1, 8 * 256 // columns)
+        gen = torch.Generator(device="cuda").manual_seed(columns)
+        x = torch.rand(rows, columns, generator=gen, device="cuda") + 0.5
+        weight = torch.ones(columns, device="cuda", requires_grad=True)
+        (dweight,) = torch.autograd.grad(ops.rms_norm(x, weight), weight, torch.ones_like(x))
+        want = 0.0
+        for part in x.chunk(8):
+            part = part.double()
+            want = want + (part * torch.rsqrt((part * part).mean(1, keepdim=True) + 1e-6)).sum(0)
+        # terms of one sign: up to 2^-25 per addition on average, of 64 + rows / slots / 64 + blocks' rows / 32 + 5
+        assert ((dweight.double() - want).abs() <= 256 * 2.0**-24 * want).all(), columns
