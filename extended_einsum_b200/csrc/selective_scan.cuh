@@ -431,6 +431,22 @@ __device__ __forceinline__ float channel_sum(float (&v)[8], int lane_in_warp) {
   return v[0];
 }
 
+// Zeros for the gradients of tokens `from` to `end` of the block's channels (a call of its own: its registers are not
+// the recurrence's).
+template <typename T>
+__device__ __noinline__ void clear_gradients(const Params& p, Channels ch, int batch, int from, int end, int padded) {
+  float* dbc = p.dbc + (((int64_t)blockIdx.x * p.batch + batch) * p.length + from) * 2 * padded;
+  for (int64_t i = threadIdx.x; i < (int64_t)(end - from) * 2 * padded; i += kBackwardThreads) dbc[i] = 0.0f;
+  for (int t = from + threadIdx.x / kBackwardChannels; t < end; t += kBackwardThreads / kBackwardChannels) {
+    const int c = threadIdx.x % kBackwardChannels;
+    if (c < ch.count) {
+      const int64_t at = ((int64_t)batch * p.length + t) * p.channels + ch.first + c;
+      static_cast<T*>(p.dx)[at] = static_cast<T*>(p.ddelta)[at] = from_f32<T>(0.0f);
+      if (p.z) static_cast<T*>(p.dz)[at] = from_f32<T>(0.0f);
+    }
+  }
+}
+
 // The backward pass.  With dv_t = dy_t silu(z_t) the adjoint of the state is
 //
 //   g_t = C_t dv_t + c_t,  c_{t-1} = e_t g_t  (c at the end: the gradient of the last state),
@@ -523,7 +539,14 @@ __global__ void __launch_bounds__(kBackwardThreads) selective_scan_backward_kern
   const float* checkpoints = p.checkpoints + ((int64_t)batch * checkpoint_rows * p.channels + ch.first + mine) * NP + quad * 4;
 
   const int tiles = (end - begin + kTile - 1) / kTile;
-  for (int t0 = begin + (tiles - 1) * kTile; t0 >= begin; t0 -= kTile) {
+  int t0 = begin + (tiles - 1) * kTile;
+  // Past the sequence's end all gradients are zero, and the adjoint stays as it is, be it finite or not.
+  if (t0 >= begin && t0 >= live) {
+    const int from = max(begin, (live - begin + kTile - 1) / kTile * kTile + begin);
+    clear_gradients<T>(p, ch, batch, from, end, NP);
+    t0 = from - kTile;
+  }
+  for (; t0 >= begin; t0 -= kTile) {
     struct {
       Raw4<T> x, d, g, z;
     } raw[2];
@@ -675,7 +698,7 @@ __global__ void __launch_bounds__(kBackwardThreads) selective_scan_backward_kern
         float sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < kWarps; ++k) sum += s_red[((nb * kWarps + k) * kTile) * 32 + i % (kTile * 32)];
-        p.dbc[(((int64_t)blockIdx.x * p.batch + batch) * p.length + t0 + t) * 2 * NP + (i / 16 % 2) * NP + nb * 16 + i % 16] = sum;
+        p.dbc[(((int64_t)blockIdx.x * p.batch + batch) * p.length + t0 + t) * 2 * NP + (i / 16 % 2) * NP + nb * 16 + i % 16] = t0 + t < live ? sum : 0.0f;
       }
     }
 #pragma unroll
@@ -692,7 +715,7 @@ __global__ void __launch_bounds__(kBackwardThreads) selective_scan_backward_kern
           o_x[i] = fmaf(dv, skip[i], s_du[row + q][col + i].x * gbi);
           o_d[i] = fmaf(xv, gbi, kLn2 * (&ga.x)[i]);
           if (p.softplus) o_d[i] *= sigmoid(value4<T>(raw[q].d, i) + bias[i]);
-          if (!in[q]) o_d[i] = 0.0f;
+          if (!in[q]) o_x[i] = o_d[i] = 0.0f;
           if (p.z) {
             const float zv = value4<T>(raw[q].z, i), sg = sigmoid(zv);
             o_z[i] = value4<T>(raw[q].g, i) * sg * (1.0f + zv * (1.0f - sg)) * fmaf(skip[i], xv, (&v4.x)[i]);

@@ -1,0 +1,46 @@
+"""Values that are not finite, at places where they must not spread (the scan's masked positions)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_sequence import close, cuda, leaf, randn, scan_call, scan_inputs, scan_reference
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("length,channels", [(50, 40), (700, 24)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scan_gradients_past_the_end_are_zero_whatever_comes_back(dtype, length, channels):
+    """A gradient of the last state that has overflowed, and a state that has: the positions past a sequence's end still have
+    zero gradients, a sequence of no tokens hands the gradient on, and the other sequences do not notice."""
+    ends = [0, 21, length, 5]
+    v = scan_inputs(61, 4, length, channels, 16, 1, dtype)
+    names = list(v)
+    gen = torch.Generator().manual_seed(62)
+    dy, dstate = randn(gen, 4, length, channels, dtype=dtype).cuda(), randn(gen, 4, channels, 16).cuda()
+    lengths = torch.tensor(ends).cuda()
+
+    def gradients(inputs, seed):
+        g = leaf({k: cuda(t) for k, t in inputs.items()}, names)
+        out = scan_call(g, True, lengths, return_state=True)
+        return dict(zip(names, torch.autograd.grad(out, [g[k] for k in names], [dy, seed])))
+
+    clean = gradients(v, dstate)
+    spoilt = dstate.clone()
+    spoilt[0] = float("inf")
+    got = gradients(v, spoilt)
+    assert torch.equal(got["state"][0], spoilt[0])
+    for k in names:
+        if k == "state":
+            assert torch.equal(got[k][1:], clean[k][1:])
+        else:
+            assert torch.equal(got[k], clean[k]), k
+    spoilt[1] = float("inf")
+    v["state"][3] = float("inf")
+    got = gradients(v, spoilt)
+    for k in ("x", "delta", "b", "c", "z"):
+        for i, end in enumerate(ends):
+            assert not got[k][i, end:].any(), (k, i)
+        assert torch.equal(got[k][2], clean[k][2])
