@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(64) selective_scan_kernel(const __grid_constan
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const bool in = mine + j < ch.count && lane * S + s < p.states;
-      a1[s] = in ? p.a[(int64_t)(ch.first + mine + j) * p.states + lane * S + s] * kLog2e : 0.0f;
+      a1[s] = in ? decay_rate(p.a[(int64_t)(ch.first + mine + j) * p.states + lane * S + s]) : 0.0f;
       h1[s] = 0.0f;
       if (!kStateOnly && in) {
         if (p.segments > 1)
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(256) selective_scan_join_kernel(Params p) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= total) return;
   const int64_t bc = i / p.states;
-  const float a = p.a[(bc % p.channels) * p.states + i % p.states] * kLog2e;
+  const float a = decay_rate(p.a[(bc % p.channels) * p.states + i % p.states]);
   const float* first = kReverse ? p.dstate_out : p.state;
   float h = first ? first[i] : 0.0f;
   for (int j = 0; j < p.segments; ++j) {
@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(kBackwardThreads) selective_scan_backward_kern
       for (int s = 0; s < 4; ++s) {
         const int n = nb * 16 + quad * 4 + s;
         const bool in = mine + j < ch.count && n < p.states;
-        a1[s] = in ? p.a[(int64_t)(ch.first + mine + j) * p.states + n] * kLog2e : 0.0f;
+        a1[s] = in ? decay_rate(p.a[(int64_t)(ch.first + mine + j) * p.states + n]) : 0.0f;
         c1[s] = 0.0f;
         if (in) {
           if (p.segments > 1)

@@ -259,6 +259,11 @@ __device__ __forceinline__ F2 exp2_fast2(F2 v) {
 // addition being part of the product's rounding: 0.7e-5, and the error of dA at 2 x 2048 x 2048 x 16 falls from
 // 2.1e-6 to 0.9e-6 of its norm.  2^2e-8 itself is one: d = 0 keeps a state as it is.
 constexpr float kDecayShift = 2e-8f;
+// a in base 2.  It stays finite: a token that does not count has d = 0 and has to leave the state alone, whatever a is.
+__device__ __forceinline__ float decay_rate(float a) {
+  const float v = a * kLog2e;
+  return v < -3.4028235e38f ? -3.4028235e38f : v;  // a NaN stays
+}
 __device__ __forceinline__ float decay(float d, float a) { return exp2_fast(fmaf(d, a, kDecayShift)); }
 __device__ __forceinline__ F2 decay2(F2 d, F2 a) { return exp2_fast2(fma2(d, a, both(kDecayShift))); }
 

@@ -44,3 +44,20 @@ def test_scan_gradients_past_the_end_are_zero_whatever_comes_back(dtype, length,
         for i, end in enumerate(ends):
             assert not got[k][i, end:].any(), (k, i)
         assert torch.equal(got[k][2], clean[k][2])
+
+
+@pytest.mark.parametrize("length,channels,ends", [(1, 24, None), (37, 40, None), (60, 24, [0, 5, 60]), (700, 24, [700, 0, 130])])
+def test_scan_rates_of_minus_infinity(length, channels, ends):
+    """A state that does not outlast a token (a = -exp(a large number)): beyond a sequence's end, and in the rest of a
+    tile, no token passes and the state stays."""
+    batch = 1 if ends is None else 3
+    v = scan_inputs(63 + length, batch, length, channels, 16)
+    v["a"][::2, 3], v["a"][1, :], v["a"][2, 5] = float("-inf"), float("-inf"), -3e38
+    lengths = None if ends is None else torch.tensor(ends).cuda()
+    g = leaf({k: cuda(t) for k, t in v.items()}, ["x", "delta"])
+    y, state = scan_call(g, True, lengths, return_state=True)
+    want_y, want_state = scan_reference(v, True, ends)
+    close(y.detach(), want_y, length)
+    close(state.detach(), want_state, length)
+    dx, ddelta = torch.autograd.grad((y, state), [g["x"], g["delta"]], [torch.ones_like(y), torch.ones_like(state)])
+    assert torch.isfinite(dx).all() and torch.isfinite(ddelta).all()
