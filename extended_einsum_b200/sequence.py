@@ -568,7 +568,7 @@ def int4_linear(
 
     ``packed`` (outputs, inputs / 2) uint8 holds two codes to a byte, the even k in the low nibble
     (``int4_pack``); ``scales`` (outputs, inputs / group) float32, bfloat16 or float16 and ``zeros`` uint8 of
-    the same shape (None: 8); the group is a multiple of 32.  ``x`` (..., inputs) is float32, bfloat16 or
+    the same shape, 0 to 15 as the codes are (None: 8); the group is a multiple of 32.  ``x`` (..., inputs) is float32, bfloat16 or
     float16, or 8-bit (float8_e4m3fn, int8) with ``x_scale`` (...) as ``rms_norm`` gives them.  ``dtype`` of
     the result: x's type, or bfloat16 for 8-bit x, unless given.  Integers q - zero and the activations
     multiply exactly; sums and scales are float32.  Made for the few rows of token-by-token generation;
@@ -623,6 +623,8 @@ def int4_pack(codes: torch.Tensor) -> torch.Tensor:
     """Codes 0 to 15, (outputs, inputs), two to a byte with the even input in the low nibble."""
     if codes.dim() != 2 or codes.shape[1] % 2:
         raise ValueError("int4_pack: expected (outputs, inputs) with an even number of inputs")
+    if ((codes < 0) | (codes > 15)).any():
+        raise ValueError("int4_pack: codes are whole numbers from 0 to 15")
     codes = codes.to(torch.uint8)
     return codes[:, 0::2] | (codes[:, 1::2] << 4)
 

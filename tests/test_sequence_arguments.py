@@ -140,3 +140,15 @@ def test_entries_refuse_buffers_off_their_boundaries():
     assert lib.xe_selective_scan(q, 4096, 1 << 30, None) == _lib.XE_ERR_INVALID_ARGUMENT and "aligned" in _lib.last_error()
     assert lib.xe_selective_scan_backward(q, grads, 4096, 1 << 30, None) == _lib.XE_ERR_INVALID_ARGUMENT
     assert "aligned" in _lib.last_error()
+
+
+@pytest.mark.parametrize("value", [16, 255, 300, -1])
+def test_int4_pack_refuses_codes_of_more_than_four_bits(value):
+    """They would change their neighbours' codes."""
+    codes = torch.full((2, 32), 5)
+    codes[1, 3] = value
+    with pytest.raises(ValueError, match="0 to 15"):
+        ops.int4_pack(codes)
+    codes[1, 3] = 15
+    assert ops.int4_pack(codes)[1, 1] == 0xF5
+    assert ops.int4_pack(codes[:0]).shape == (0, 16)
