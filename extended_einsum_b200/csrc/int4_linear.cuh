@@ -5,7 +5,7 @@
 // Bound by reading the codes.  They stay 4 bits wide up to the registers: a nibble becomes a 16-bit
 // float by two bit operations (the exponent of 128 for bf16, of 1024 for f16, with the nibble as the
 // last bits of the significand), and subtracting 128 + z (1024 + z) leaves the exact integer q - z.  The
-// tensor core sums these integers against the 16-bit activations exactly into float32 (the weights as
+// tensor core multiplies these integers by the 16-bit activations exactly and sums in float32 (the weights as
 // the 16-row operand, the tokens as the 8 columns), and each group's sum is scaled in float32.
 // Activations of 8 bits convert to f16 exactly; float32 ones enter as three bf16 parts (8 + 8 + 8
 // bits of significand, also exact) in columns of their own.
@@ -20,9 +20,9 @@
 // does not fit, one part of it.  Where blocks hold all of k, a tile's runs go to neighbouring warps, whose sums
 // meet in shared memory; sums of several parts go to a workspace and a second kernel adds them in order.
 //
-// Measured on a B200: a bf16 token against 8192 x 4096 10.3 us, against 28672 x 8192 58 us (2.1 TB/s of weights);
-// 16 e4m3 rows against 16384 x 8192 46.5 us.  Unpacking takes eleven integer and 16-bit instructions for eight
-// codes (eight in f16) beside one or two tensor instructions, and binds all but the smallest calls.
+// Measured on a B200: a bf16 token against 8192 x 4096 10.3 us, against 28672 x 8192 61 us (2.0 TB/s);
+// 16 e4m3 rows against 16384 x 8192 47 us.  Unpacking takes eleven integer and 16-bit instructions for eight
+// codes (nine, and one for the zero point, in f16) beside one or two tensor instructions: its pipe is the busiest (42 %).
 #pragma once
 
 #include "seq_common.cuh"

@@ -4,7 +4,7 @@
 //   h_tn = e_tn h_{t-1,n} + delta_t x_t B_tn,   v_t = sum_n C_tn h_tn + D_d x_t,   y_t = v_t silu(z_t),
 //
 // with B and C shared by the channels of a group.  Bound by the special function unit: one
-// exponential per token, channel and state at 16 results per clock and SM (plus four per token and
+// exponential per token, channel and state at 16 results per clock and SM (plus three per token and
 // channel for softplus and the gate); the 8 bytes of x, delta, z and y of a 16-bit type take a third of
 // that time.
 //
@@ -20,9 +20,9 @@
 // and keeps its last state and sum of delta (the product of its e is exp(A sum delta)), a second
 // joins them into every segment's first state, and the scan then runs all segments at once.
 // Measured on a B200, 16 states, bf16: 4 x 4096 tokens of 4096 channels 529 us (the special function unit's
-// floor is 274 us; 3.5 warps to a scheduler issue in about half of its slots); 2 x 2048 tokens of 2048 channels
-// forward 140 us in four segments, of them 73 us the scan itself, backward 262 us and 51 us for the segments'
-// adjoints; one token of 64 x 4096 channels 12.9 us (36 MB, 2.8 TB/s).
+// floor is 274 us; 3.3 warps to a scheduler issue in about half of its slots); 2 x 2048 tokens of 2048 channels
+// forward 122 us in four segments (140 us with the states stored for the backward pass), backward 262 us and 51 us for
+// the segments' adjoints; one token of 64 x 4096 channels 12.5 to 13 us (36 MB, 2.8 TB/s).
 #pragma once
 
 #include "seq_common.cuh"

@@ -477,7 +477,8 @@ typedef enum { XE_F32 = 0, XE_BF16 = 1, XE_F16 = 2, XE_E4M3 = 3, XE_I8 = 4 } xe_
  * state_out (or NULL) receives the last width - 1 entries of [state, x[:length]].
  * `lengths` (or NULL): per sequence, int32 or (lengths64 != 0) int64 on the
  * device, clamped to [0, length]; positions past it are not read and their y is 0.
- * width 1 to 4; XE_F32, XE_BF16 or XE_F16. */
+ * width 1 to 4, at most 65535 sequences (any number in the single-token form); XE_F32,
+ * XE_BF16 or XE_F16. */
 xe_status xe_causal_conv1d(const void* x, int64_t x_sb, int64_t x_st, const float* weight, const float* bias,
                            const void* state, void* y, void* state_out, const void* lengths, int32_t lengths64,
                            int64_t batch, int64_t length, int64_t channels, int64_t width, int32_t activation,
@@ -507,7 +508,7 @@ xe_status xe_causal_conv1d_backward(const void* x, int64_t x_sb, int64_t x_st, c
  * states) is h before the first token (NULL: zero), state_out (or NULL) h after the
  * last.  `lengths` as above: positions past a sequence's length leave its state as it is
  * and have y = 0.  x, delta, z, b, c and y share one type (XE_F32, XE_BF16, XE_F16); at
- * most 64 states (any number in the single-token form).
+ * most 64 states and 65535 sequences (any number in the single-token form).
  * checkpoints (or NULL) receives the states that xe_selective_scan_backward starts from,
  * xe_selective_scan_checkpoint_size() bytes. */
 typedef struct {

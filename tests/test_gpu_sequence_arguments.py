@@ -40,3 +40,31 @@ def test_a_state_stepped_after_it_was_saved_has_no_gradient():
     ops.causal_conv1d_step(taps, x[:, 0], weight)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_gradients_of_no_tokens():
+    """Of a length of zero the state's gradient comes back as it is, and the parameters' are zero."""
+    gen = torch.Generator().manual_seed(3)
+    x, bc = torch.zeros(2, 0, 8).cuda(), torch.zeros(2, 0, 4).cuda()
+    a, state, seed = (torch.randn(*s, generator=gen).cuda().requires_grad_() for s in ((8, 4), (2, 8, 4), (2, 8, 4)))
+    _, last = ops.selective_scan(x, x, a, bc, bc, state=state, return_state=True)
+    da, dstate = torch.autograd.grad(last, [a, state], seed.detach())
+    assert not da.any() and torch.equal(dstate, seed)
+    weight, taps, seed = (torch.randn(*s, generator=gen).cuda().requires_grad_() for s in ((8, 4), (2, 3, 8), (2, 3, 8)))
+    _, new = ops.causal_conv1d(x, weight, state=taps, return_state=True)
+    dweight, dtaps = torch.autograd.grad(new, [weight, taps], seed.detach())
+    assert not dweight.any() and torch.equal(dtaps, seed)
+
+
+def test_a_prompt_of_more_tokens_than_a_grid_holds():
+    """17 sequences of 4000 tokens through the quantised stack; the first of them alone gives the same logits (within the
+    few flips of 8-bit codes that test_gpu_state_space.py allows for)."""
+    from extended_einsum_b200.state_space import SelectiveStack, StackShape, init_parameters
+
+    shape = StackShape(layers=1, width=64, channels=64, states=4, outputs=32)
+    model = SelectiveStack(shape, init_parameters(shape, torch.Generator().manual_seed(4)), torch.float32).quantize()
+    tokens = torch.randint(shape.outputs, (17, 4000), generator=torch.Generator().manual_seed(5)).cuda()
+    logits = model.prompt(tokens, model.empty_state(17))
+    alone = model.prompt(tokens[:1], model.empty_state(1))
+    assert logits.shape == (17, 4000, 32) and torch.isfinite(logits).all()
+    torch.testing.assert_close(logits[:1].float(), alone.float(), rtol=0.05, atol=0.05 * alone.abs().max().item())

@@ -114,3 +114,18 @@ def test_norm_sums_of_columns_over_rows_by_element_and_in_vectors():
             want = want + (part * torch.rsqrt((part * part).mean(1, keepdim=True) + 1e-6)).sum(0)
         # terms of one sign: up to 2^-25 per addition on average, of 64 + rows / slots / 64 + blocks' rows / 32 + 5
         assert ((dweight.double() - want).abs() <= 256 * 2.0**-24 * want).all(), columns
+
+
+def test_softplus_keeps_small_results():
+    """A step's softplus seen through a state of no decay: 2^x is off by up to 2^-22 of itself, the rounding of v log2(e) in
+    front of it by 2^-23.7 |v|, the polynomial by 7.6e-8 and its evaluation by 2^-23: in all within 2^-21 + |v| 2^-23."""
+    v = torch.cat([torch.linspace(-80, 30, 40000), torch.tensor([-1e-6, 0.0, 1e-6, 19.9, 20.1, 80.0])]).cuda()
+    one, none = torch.ones(1, v.numel(), device="cuda"), torch.zeros(1, 1, device="cuda")
+    want = torch.nn.functional.softplus(v.double(), threshold=60.0)
+    room = (2.0**-21 + v.double().abs() * 2.0**-23) * want
+    zero = torch.zeros(v.numel(), 1, device="cuda")
+    _, state = ops.selective_scan(one[:, None], v[None, None], zero, none[:, None] + 1, none[:, None], softplus=True, return_state=True)
+    assert ((state[0, :, 0].double() - want).abs() <= room).all()
+    held = torch.zeros(1, v.numel(), 1, device="cuda")
+    ops.selective_scan_step(held, one, v[None], zero, none + 1, none, softplus=True)
+    assert ((held[0, :, 0].double() - want).abs() <= room).all()
