@@ -262,7 +262,7 @@ constexpr float kDecayShift = 2e-8f;
 // a in base 2.  It stays finite: a token that does not count has d = 0 and has to leave the state alone, whatever a is.
 __device__ __forceinline__ float decay_rate(float a) {
   const float v = a * kLog2e;
-  return v < -3.4028235e38f ? -3.4028235e38f : v;  // a NaN stays
+  return fabsf(v) > 3.4028235e38f ? copysignf(3.4028235e38f, v) : v;  // a NaN stays
 }
 __device__ __forceinline__ float decay(float d, float a) { return exp2_fast(fmaf(d, a, kDecayShift)); }
 __device__ __forceinline__ F2 decay2(F2 d, F2 a) { return exp2_fast2(fma2(d, a, both(kDecayShift))); }

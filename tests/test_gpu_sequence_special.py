@@ -61,3 +61,12 @@ def test_scan_rates_of_minus_infinity(length, channels, ends):
     close(state.detach(), want_state, length)
     dx, ddelta = torch.autograd.grad((y, state), [g["x"], g["delta"]], [torch.ones_like(y), torch.ones_like(state)])
     assert torch.isfinite(dx).all() and torch.isfinite(ddelta).all()
+
+
+@pytest.mark.parametrize("length", [0, 5, 300])
+def test_scan_rates_of_infinity_do_not_touch_a_sequence_of_no_tokens(length):
+    v = scan_inputs(64, 2, length, 24, 16)
+    v["a"][3], v["a"][5, 2] = float("inf"), float("-inf")
+    lengths = torch.zeros(2, dtype=torch.int32).cuda()
+    y, state = scan_call({k: cuda(t) for k, t in v.items()}, True, lengths, return_state=True)
+    assert torch.equal(state.cpu(), v["state"]) and not y.any()
