@@ -2,8 +2,8 @@
 // few rows m of tokens being generated.  Codes lie two to a byte, the even k in the low nibble; a
 // group of `group` consecutive k (a multiple of 32) shares a scale and a zero point (8 without them).
 //
-// Bound by reading the codes.  They stay 4 bits wide up to the registers: a nibble becomes a 16-bit
-// float by two bit operations (the exponent of 128 for bf16, of 1024 for f16, with the nibble as the
+// Bound by reading the codes.  They stay 4 bits wide up to the registers: by a published technique a nibble becomes a
+// 16-bit float by two bit operations (the exponent of 128 for bf16, of 1024 for f16, with the nibble as the
 // last bits of the significand), and subtracting 128 + z (1024 + z) leaves the exact integer q - z.  The
 // tensor core multiplies these integers by the 16-bit activations exactly and sums in float32 (the weights as
 // the 16-row operand, the tokens as the 8 columns), and each group's sum is scaled in float32.
